@@ -36,8 +36,9 @@
 extern "C" {
 #endif
 
-#define EXL3_ABI_VERSION 3       /* 2: exl3_gemv_f32, exl3_gemm_trellis_silu_in; 3: exl3_gemv_silu_prerot_rows,
-                                    exl3_gemm_trellis_workspace_bound, the plain GEMV up to 64 rows */
+#define EXL3_ABI_VERSION 4       /* 2: exl3_gemv_f32, exl3_gemm_trellis_silu_in; 3: exl3_gemv_silu_prerot_rows,
+                                    exl3_gemm_trellis_workspace_bound, the plain GEMV up to 64 rows;
+                                    4: exl3_batch_plan, exl3_rope_kv_write, exl3_paged_attention */
 #define EXL3_MAX_GROUPS 4       /* groups per grouped launch (reference EXL3_GEMV_MRG_MAX) */
 #define EXL3_GEMV_MAX_ROWS 64   /* rows the plain fused GEMV takes (exl3_gemv_mr and its grouped forms) */
 #define EXL3_GEMV_FUSED_MAX_ROWS 32 /* rows of the fused-epilogue forms (SiLU input, gated, approximate) */
@@ -329,6 +330,69 @@ int exl3_gemm(const void* x, int64_t ldx, const void* trellis, void* y, int64_t 
  * HIP graph capture, tight serving loops, harnesses that forbid hipMalloc. */
 int exl3_gemv_mr_noalloc(const void* x, int64_t ldx, const void* trellis, void* y, int64_t ldy, const void* suh,
                          const void* svh, int m, int k, int n, int K, int mcg, int mul1, void* stream);
+
+/* ---- the attention between a decoder layer's q/k/v and o projections, over a paged key/value cache ----------
+ * No counterpart in the reference, whose server has its own.  A cache page holds page_size consecutive tokens of one
+ * request for every kv head; k_cache and v_cache are [pages][page_size][kv_heads][head_dim] with any page, token and
+ * head strides.  Request r's row of the block table lists its pages in order: position p lies in page
+ * block_table[r][p / page_size], row p % page_size, and its slot is page * page_size + p % page_size.
+ * Element type: EXL3_FP16 or EXL3_BF16, one for q, k, v, caches and output.  head_dim: 64, 128 or 256.
+ * Alignment: every tensor 16 bytes, every stride a multiple of 8 elements; violations return EXL3_EINVAL before any
+ * launch.  Lengths, tables, positions and slots are read on the GPU alone and nothing is read back: what they
+ * hold is checked there, and a page or slot outside the cache is neither read nor written. */
+#define EXL3_FP16 0
+#define EXL3_BF16 1
+#define EXL3_PAGED_MAX_REQUESTS 16384
+#define EXL3_PAGED_MAX_TOKENS 4194304
+#define EXL3_PAGED_MAX_HEADS 1024
+#define EXL3_PAGED_MAX_PAGE 65536 /* tokens of a page */
+
+/* One step's bookkeeping from the requests' lengths.  Request r holds ctx_lens[r] tokens in the cache and adds
+ * new_lens[r] (negative lengths count as 0; all lengths together stay below 2^31):
+ *   cu_q[requests + 1]   its new tokens are [cu_q[r], cu_q[r + 1])
+ *   seq_lens[requests]   ctx_lens + new_lens
+ *   positions[tokens], slots[tokens]  of every new token; slot -1 where it has no page (stack or table row too
+ *                        short); tokens past cu_q[requests]: position 0, slot -1; new tokens past `tokens` are not written
+ *   block_table          columns ceil(ctx / page_size) .. ceil(seq / page_size) - 1 of a row that adds tokens take
+ *                        pages from the stack free_pages[0 .. free_count[0]) (at most n_free), its top first, in the
+ *                        order of the requests; -1 once it is empty.  Other entries stay.
+ *   free_left[1]         free_count less the pages taken: negative if that many were missing
+ * free_pages and free_count are not changed, so a repeated call gives the same.  Rows ld_table apart, table_cols columns. */
+int exl3_batch_plan(const int* ctx_lens, const int* new_lens, int* block_table, int64_t ld_table, int table_cols,
+                    const int* free_pages, int n_free, const int* free_count, int* cu_q, int* seq_lens, int64_t* positions,
+                    int64_t* slots, int* free_left, int requests, int page_size, int tokens, void* stream);
+
+/* Rotary embedding of q and k by position, with k and v written into the cache.  The first rot_dim (even) elements of
+ * a head are rot_dim / 2 pairs: elements (i, i + rot_dim / 2), or (2 i, 2 i + 1) if interleaved.  Pair i turns by
+ * position * inv_freq[i] radians (float64; long-context scaling is the caller's choice of inv_freq) and grows by
+ * mscale; the rest of the head is as it was.  q_out[tokens][q_heads][head_dim] receives the rotated q; the rotated k
+ * and v go to the token's slot (a slot outside [0, pages * page_size) writes nothing; two tokens of one slot race).
+ * Arithmetic in fp32, the angle in float64, one rounding to the element type.  Strides (token, head; cache: page,
+ * token, head) in elements.  q_out overlaps no input. */
+int exl3_rope_kv_write(const void* q, int64_t q_ldt, int64_t q_ldh, const void* k, int64_t k_ldt, int64_t k_ldh, const void* v,
+                       int64_t v_ldt, int64_t v_ldh, const int64_t* positions, const int64_t* slots, void* q_out, void* k_cache,
+                       int64_t kc_ldp, int64_t kc_ldt, int64_t kc_ldh, void* v_cache, int64_t vc_ldp, int64_t vc_ldt,
+                       int64_t vc_ldh, const double* inv_freq, float mscale, int tokens, int q_heads, int kv_heads, int head_dim,
+                       int rot_dim, int interleaved, int pages, int page_size, int dtype, void* stream);
+
+/* Workspace bytes of exl3_paged_attention (the first EXL3_ATTN_COUNTER_BYTES are zero before the first call, and every
+ * call leaves them zero; one workspace serves calls of any shape in stream order, overlapping calls race). */
+size_t exl3_paged_attention_workspace_size(int tokens, int requests, int q_heads, int kv_heads, int head_dim);
+
+/* out[t][h] = sum_j softmax_j(scale q[t][h] . k_j) v_j over the keys that token t sees: token i of request r's
+ * n = cu_q[r + 1] - cu_q[r] new tokens (rows [cu_q[r], cu_q[r + 1]) of q) lies at position p = seq_lens[r] - n + i of the
+ * cache and sees positions j <= p, and j > p - window if window > 0.  Query head h reads kv head h / (q_heads / kv_heads).
+ * One call takes decodes, drafts and prompt chunks together.  A row that sees nothing (a token of no request, a
+ * negative position) is 0.  Keys that a token does not see have no effect on its row, whatever they hold; so have
+ * positions whose table entry is no page and positions past table_cols * page_size.
+ * page_size: a multiple of 16.  cu_q: non-decreasing, 0 first; rows past `tokens` are dropped.
+ * Scores, maxima, sums and outputs in fp32; a probability is rounded to the element type for its product with V.
+ * Results are the same bits in every call with the same arguments. */
+int exl3_paged_attention(const void* q, int64_t q_ldt, int64_t q_ldh, const void* k_cache, int64_t k_ldp, int64_t k_ldt,
+                         int64_t k_ldh, const void* v_cache, int64_t v_ldp, int64_t v_ldt, int64_t v_ldh, const int* block_table,
+                         int64_t ld_table, int table_cols, const int* cu_q, const int* seq_lens, void* out, int64_t o_ldt,
+                         int64_t o_ldh, int tokens, int requests, int q_heads, int kv_heads, int head_dim, int pages,
+                         int page_size, float scale, int window, int dtype, void* workspace, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -16,7 +16,7 @@ MAX_GROUPS = 4
 GEMV_MAX_ROWS = 64
 GEMV_FUSED_MAX_ROWS = 32
 NOALLOC_SCRATCH_BYTES = 17039360
-ABI_VERSION = 3
+ABI_VERSION = 4
 
 _p, _i, _i64, _sz, _f = C.c_void_p, C.c_int, C.c_int64, C.c_size_t, C.c_float
 _pp = C.POINTER(C.c_void_p)
@@ -60,6 +60,12 @@ SIGNATURES = {
     "exl3_gemm_rd_check": (_i, [_i, _i, C.POINTER(C.c_int), _i]),
     "exl3_gemm": (_i, [_p, _i64, _p, _p, _i64, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p, _sz, _p]),
     "exl3_gemv_mr_approx": (_i, [_p, _i64, _p, _p, _i64, _p, _p, _p, _i, _i, _i, _i, _i, _p, _sz, _p]),
+    "exl3_batch_plan": (_i, [_p, _p, _p, _i64, _i, _p, _i, _p, _p, _p, _p, _p, _p, _i, _i, _i, _p]),
+    "exl3_rope_kv_write": (_i, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64,
+                                _p, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p]),
+    "exl3_paged_attention_workspace_size": (_sz, [_i, _i, _i, _i, _i]),
+    "exl3_paged_attention": (_i, [_p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i, _p, _p, _p, _i64, _i64,
+                                  _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _p, _sz, _p]),
     "exl3_gemv_mr_noalloc": (_i, [_p, _i64, _p, _p, _i64, _p, _p, _i, _i, _i, _i, _i, _i, _p]),
 }
 

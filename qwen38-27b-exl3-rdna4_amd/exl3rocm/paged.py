@@ -1,0 +1,220 @@
+"""
+The attention step of a decoder layer over a paged key/value cache, between the q/k/v and o modules:
+
+  batch_plan       block-table growth, token positions and cache slots of one step, from the requests' lengths
+  rope_kv_write    rotary embedding of q and k, with k and v written into the cache
+  paged_attention  causal attention of every request's new tokens (decodes, drafts and prompt chunks in one call)
+
+The lengths stay on the GPU: no call reads them back, so a step's calls can be captured in a HIP graph and replayed
+as the lengths grow.  Each function is also the torch op of its name (torch.ops.exl3rocm.*), one opaque node for
+torch.compile.  Inference only: no gradients.  `rope_frequencies` makes the rotary frequencies, `new_cache` a
+cache in the layout that the kernels read fastest.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib as L
+from .kernels import _need, _stream
+
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1}
+HEAD_DIMS = (64, 128, 256)
+
+
+def new_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=torch.float16, device="cuda") -> Tuple[torch.Tensor, torch.Tensor]:
+    """(k_cache, v_cache), each [pages, page_size, kv_heads, head_dim] of a memory order in which a page holds every head's
+    tokens together."""
+    return tuple(torch.zeros(pages, kv_heads, page_size, head_dim, dtype=dtype, device=device).transpose(1, 2) for _ in range(2))
+
+
+def rope_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[dict] = None, device="cuda") -> Tuple[torch.Tensor, float]:
+    """(inv_freq, mscale) for rope_kv_write: radians a position adds to each of the rot_dim / 2 pairs (float64), and the
+    factor on cosine and sine.  scaling (the keys of a model's `rope_scaling`):
+      None or rope_type "default"   base ** (-2 i / rot_dim)
+      "linear"   every frequency divided by factor
+      "yarn"     divided by factor where a pair makes fewer than beta_slow (1) turns in
+                 original_max_position_embeddings tokens, kept above beta_fast (32), a ramp over the pair's index
+                 between; mscale = attention_factor, or 0.1 ln(factor) + 1
+      "llama3"   divided by factor where its wavelength exceeds original / low_freq_factor, kept below original /
+                 high_freq_factor, blended between"""
+    _need(rot_dim >= 2 and rot_dim % 2 == 0, f"rope_frequencies: rot_dim must be even, got {rot_dim}")
+    _need(base > 1, f"rope_frequencies: base must be above 1, got {base}")
+    i = torch.arange(rot_dim // 2, dtype=torch.float64)
+    f = base ** (-2.0 * i / rot_dim)
+    s = scaling or {}
+    kind, mscale = s.get("rope_type", s.get("type", "default")), 1.0
+    if kind == "linear":
+        f = f / s["factor"]
+    elif kind == "yarn":
+        factor, orig = float(s["factor"]), float(s["original_max_position_embeddings"])
+        # the pair index that makes b turns in the original context
+        at = lambda b: rot_dim * math.log(orig / (2 * math.pi * b)) / (2 * math.log(base))  # noqa: E731
+        low = max(math.floor(at(s.get("beta_fast", 32))), 0)
+        high = min(math.ceil(at(s.get("beta_slow", 1))), rot_dim - 1)
+        slow = ((i - low) / max(high - low, 1e-3)).clamp(0, 1)
+        f = f / factor * slow + f * (1 - slow)
+        mscale = float(s.get("attention_factor") or (0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0))
+    elif kind == "llama3":
+        lo, hi = s["low_freq_factor"], s["high_freq_factor"]
+        turns = s["original_max_position_embeddings"] * f / (2 * math.pi)
+        keep = ((turns - lo) / (hi - lo)).clamp(0, 1)
+        f = f * keep + f / s["factor"] * (1 - keep)
+    else:
+        _need(kind == "default", f"rope_frequencies: unknown rope_type {kind!r}")
+    return f.to(device), mscale
+
+
+def _ints(name: str, t: torch.Tensor, device, dtype, numel: Optional[int] = None):
+    if t.dtype != dtype or t.device != device or not t.is_contiguous() or (numel is not None and t.numel() != numel):
+        _need(False, f"{name} must be a contiguous {dtype} tensor on {device}" + (f" of {numel} elements" if numel is not None else ""))
+
+
+def _on_gpu(t: torch.Tensor, what: str):
+    _need(t.is_cuda, f"{what}: tensors must be on a GPU (no CPU path)")
+
+
+def _ld(t: torch.Tensor, dims: int) -> list:
+    """Strides of t's first `dims` dimensions; 0 for one of a single element, whose stride addresses nothing."""
+    return [s if n > 1 else 0 for n, s in zip(t.shape[:dims], t.stride())]
+
+
+def batch_plan(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
+               free_count: torch.Tensor, page_size: int, num_tokens: int
+               ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(cu_q, seq_lens, positions, slots, free_left) of a step in which request r, with ctx_lens[r] tokens in the cache,
+    adds new_lens[r] (int32 [R]).  block_table (int32 [R, columns], rows any stride apart) gets the pages that the new
+    tokens need, popped from the stack free_pages[:free_count] (int32; its top first, in the order of the requests).
+    num_tokens: rows of the step's batch; rows past the last request get position 0 and slot -1, as a batch
+    padded for a captured graph has them.  free_left [1] is the next free_count; negative: that many pages were missing,
+    and the tokens without one have slot -1 (nothing is written for them).  The stack and its count are only read:
+    a repeated call gives the same result."""
+    _on_gpu(ctx_lens, "batch_plan")
+    dev, i32 = ctx_lens.device, torch.int32
+    R = ctx_lens.numel()
+    _ints("batch_plan: ctx_lens", ctx_lens, dev, i32)
+    _ints("batch_plan: new_lens", new_lens, dev, i32, R)
+    _ints("batch_plan: free_pages", free_pages, dev, i32)
+    _ints("batch_plan: free_count", free_count, dev, i32, 1)
+    _need(block_table.dtype == i32 and block_table.device == dev and block_table.dim() == 2 and block_table.shape[0] == R
+          and (block_table.shape[1] <= 1 or block_table.stride(1) == 1),
+          f"batch_plan: block_table must be int32 [{R}, columns] on {dev} with unit column stride")
+    _need(page_size >= 1 and num_tokens >= 0, "batch_plan: page_size from 1, num_tokens from 0")
+    cols = block_table.shape[1]
+    ld = block_table.stride(0) if R > 1 else cols
+    ints = torch.empty(2 * R + 2, dtype=i32, device=dev)          # one allocation: cu_q, seq_lens, free_left
+    tok = torch.empty((2, num_tokens), dtype=torch.int64, device=dev)
+    cu_q, seq, left = ints[:R + 1], ints[R + 1:2 * R + 1], ints[2 * R + 1:]
+    p = ints.data_ptr()
+    t = tok.data_ptr()
+    L.check(L.lib().exl3_batch_plan(ctx_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), ld, cols, free_pages.data_ptr(),
+                                    free_pages.numel(), free_count.data_ptr(), p, p + 4 * (R + 1), t, t + 8 * num_tokens,
+                                    p + 4 * (2 * R + 1), R, page_size, num_tokens, _stream(ctx_lens)), "batch_plan")
+    return cu_q, seq, tok[0], tok[1], left
+
+
+def _cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, dtype, device, hkv: int, d: int):
+    """Checks a cache against the heads that use it; its pages and page size."""
+    if not (k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype == dtype
+            and k_cache.device == v_cache.device == device and k_cache.stride(3) == v_cache.stride(3) == 1
+            and k_cache.shape[2] == hkv and k_cache.shape[3] == d):
+        _need(False, f"{what}: k_cache and v_cache must be {dtype} [pages, page_size, {hkv}, {d}] on {device} with unit last stride, "
+                     f"got {tuple(k_cache.shape)} {k_cache.dtype} and {tuple(v_cache.shape)} {v_cache.dtype}")
+    return k_cache.shape[0], k_cache.shape[1]
+
+
+def rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
+                  k_cache: torch.Tensor, v_cache: torch.Tensor, inv_freq: torch.Tensor, mscale: float = 1.0,
+                  interleaved: bool = False) -> torch.Tensor:
+    """Rotated q [T, q_heads, D]; the rotated k and v [T, kv_heads, D] are written to their tokens' slots of the cache
+    [pages, page_size, kv_heads, D].  q, k and v may be slices (any token and head strides that are multiples of
+    8, unit last stride), e.g. columns of the fused q/k/v module's output.  positions, slots: int64 [T]; a slot
+    outside the cache (-1) writes nothing.  inv_freq: float64 [rot_dim / 2], mscale: rope_frequencies; interleaved:
+    pairs (2 i, 2 i + 1) instead of (i, i + rot_dim / 2).  fp16 or bf16, D of 64, 128 or 256."""
+    _on_gpu(q, "rope_kv_write")
+    dev, dt = q.device, q.dtype
+    _need(q.dim() == 3 and k.dim() == 3 and v.shape == k.shape and q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2],
+          f"rope_kv_write: q [T, q_heads, D], k and v [T, kv_heads, D], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    T, hq, d = q.shape
+    hkv = k.shape[1]
+    _need(dt in _DTYPES and k.dtype == dt and v.dtype == dt and k.device == dev and v.device == dev and d in HEAD_DIMS,
+          f"rope_kv_write: q, k and v of one type, fp16 or bf16, on one GPU, heads of {HEAD_DIMS}; got {dt}, {k.dtype}, {v.dtype}, {d}")
+    _need(T == 0 or (q.stride(2) == 1 and k.stride(2) == 1 and v.stride(2) == 1), "rope_kv_write: q, k and v need unit last stride")
+    pages, page = _cache("rope_kv_write", k_cache, v_cache, dt, dev, hkv, d)
+    _ints("rope_kv_write: positions", positions, dev, torch.int64, T)
+    _ints("rope_kv_write: slots", slots, dev, torch.int64, T)
+    _ints("rope_kv_write: inv_freq", inv_freq, dev, torch.float64)
+    out = torch.empty((T, hq, d), dtype=dt, device=dev)
+    L.check(L.lib().exl3_rope_kv_write(q.data_ptr(), *_ld(q, 2), k.data_ptr(), *_ld(k, 2), v.data_ptr(),
+                                       *_ld(v, 2), positions.data_ptr(), slots.data_ptr(), out.data_ptr(),
+                                       k_cache.data_ptr(), *_ld(k_cache, 3), v_cache.data_ptr(), *_ld(v_cache, 3),
+                                       inv_freq.data_ptr(), mscale, T, hq, hkv, d, 2 * inv_freq.numel(), int(interleaved), pages, page,
+                                       _DTYPES[dt], _stream(q)), "rope_kv_write")
+    return out
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, cu_q: torch.Tensor,
+                    seq_lens: torch.Tensor, scale: float, window: int = 0) -> torch.Tensor:
+    """Causal attention [T, q_heads, D] of the rows of q [T, q_heads, D] (any token and head strides that are multiples of
+    8) over a paged cache [pages, page_size, kv_heads, D], page_size a multiple of 16.  Rows [cu_q[r], cu_q[r + 1])
+    belong to request r and are the last of its seq_lens[r] tokens, whose pages block_table[r] lists (int32, as batch_plan
+    makes them).  window: keys that a token sees, itself included (0: all).  A row that sees no key is 0; what a row
+    does not see has no effect on it, NaN included."""
+    _on_gpu(q, "paged_attention")
+    dev, dt = q.device, q.dtype
+    _need(q.dim() == 3 and dt in _DTYPES and q.shape[2] in HEAD_DIMS and k_cache.dim() == 4,
+          f"paged_attention: q must be fp16 or bf16 [T, q_heads, D] with D of {HEAD_DIMS}, got {dt} {tuple(q.shape)}")
+    T, hq, d = q.shape
+    hkv = k_cache.shape[2]
+    pages, page = _cache("paged_attention", k_cache, v_cache, dt, dev, hkv, d)
+    _need(hkv > 0 and hq > 0 and hq % hkv == 0, f"paged_attention: {hq} query heads are no multiple of {hkv} kv heads")
+    _need(page >= 16 and page % 16 == 0, f"paged_attention: page_size must be a multiple of 16, got {page}")
+    _need(T == 0 or q.stride(2) == 1, "paged_attention: q needs unit last stride")
+    R = seq_lens.numel()
+    _ints("paged_attention: seq_lens", seq_lens, dev, torch.int32)
+    _ints("paged_attention: cu_q", cu_q, dev, torch.int32, R + 1)
+    _need(block_table.dtype == torch.int32 and block_table.device == dev and block_table.dim() == 2 and block_table.shape[0] == R
+          and (block_table.shape[1] <= 1 or block_table.stride(1) == 1),
+          f"paged_attention: block_table must be int32 [{R}, columns] on {dev} with unit column stride")
+    _need(window >= 0, "paged_attention: window from 0 (0: none)")
+    cols = block_table.shape[1]
+    out = torch.empty((T, hq, d), dtype=dt, device=dev)
+    st = _stream(q)
+    L.check(L.lib().exl3_paged_attention(q.data_ptr(), *_ld(q, 2), k_cache.data_ptr(), *_ld(k_cache, 3),
+                                         v_cache.data_ptr(), *_ld(v_cache, 3), block_table.data_ptr(),
+                                         block_table.stride(0) if R > 1 else cols, cols, cu_q.data_ptr(), seq_lens.data_ptr(),
+                                         out.data_ptr(), hq * d, d, T, R, hq, hkv, d, pages, page, scale, window, _DTYPES[dt],
+                                         None, 0, st), "paged_attention")
+    return out
+
+
+# The ops are registered with their schemas and the functions above as their GPU kernels: torch.library.custom_op's
+# wrapper takes an eager call 14 us of host time (18 where the op changes an input), this way 5.
+_ops = torch.library.Library("exl3rocm", "FRAGMENT")
+_ops.define("batch_plan(Tensor ctx_lens, Tensor new_lens, Tensor(a!) block_table, Tensor free_pages, Tensor free_count, int page_size, "
+            "int num_tokens) -> (Tensor, Tensor, Tensor, Tensor, Tensor)")
+_ops.define("rope_kv_write(Tensor q, Tensor k, Tensor v, Tensor positions, Tensor slots, Tensor(a!) k_cache, Tensor(b!) v_cache, "
+            "Tensor inv_freq, float mscale=1.0, bool interleaved=False) -> Tensor")
+_ops.define("paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor cu_q, Tensor seq_lens, float scale, "
+            "int window=0) -> Tensor")
+for _f in (batch_plan, rope_kv_write, paged_attention):
+    _ops.impl(_f.__name__, _f, "CompositeExplicitAutograd")
+
+
+@torch.library.register_fake("exl3rocm::batch_plan")
+def _(ctx_lens, new_lens, block_table, free_pages, free_count, page_size, num_tokens):
+    R = ctx_lens.shape[0]
+    return (ctx_lens.new_empty(R + 1), ctx_lens.new_empty(R), ctx_lens.new_empty(num_tokens, dtype=torch.int64),
+            ctx_lens.new_empty(num_tokens, dtype=torch.int64), ctx_lens.new_empty(1))
+
+
+@torch.library.register_fake("exl3rocm::rope_kv_write")
+def _(q, k, v, positions, slots, k_cache, v_cache, inv_freq, mscale=1.0, interleaved=False):
+    return q.new_empty(q.shape)
+
+
+@torch.library.register_fake("exl3rocm::paged_attention")
+def _(q, k_cache, v_cache, block_table, cu_q, seq_lens, scale, window=0):
+    return q.new_empty(q.shape)
