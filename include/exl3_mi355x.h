@@ -346,6 +346,9 @@ int exl3_gemv_mr_noalloc(const void* x, int64_t ldx, const void* trellis, void* 
 #define EXL3_PAGED_MAX_TOKENS 4194304
 #define EXL3_PAGED_MAX_HEADS 1024
 #define EXL3_PAGED_MAX_PAGE 65536 /* tokens of a page */
+#define EXL3_ATTN_MAX_LDT 67108864 /* token stride of a cache, elements */
+#define EXL3_ATTN_MAX_WINDOW 1073741824
+#define EXL3_ATTN_COUNTER_BYTES 1024
 
 /* One step's bookkeeping from the requests' lengths.  Request r holds ctx_lens[r] tokens in the cache and adds
  * new_lens[r] (negative lengths count as 0; all lengths together stay below 2^31):
@@ -375,9 +378,10 @@ int exl3_rope_kv_write(const void* q, int64_t q_ldt, int64_t q_ldh, const void* 
                        int64_t vc_ldh, const double* inv_freq, float mscale, int tokens, int q_heads, int kv_heads, int head_dim,
                        int rot_dim, int interleaved, int pages, int page_size, int dtype, void* stream);
 
-/* Workspace bytes of exl3_paged_attention (the first EXL3_ATTN_COUNTER_BYTES are zero before the first call, and every
- * call leaves them zero; one workspace serves calls of any shape in stream order, overlapping calls race). */
-size_t exl3_paged_attention_workspace_size(int tokens, int requests, int q_heads, int kv_heads, int head_dim);
+/* Workspace bytes of exl3_paged_attention, for every shape (parts of tiles that several workgroups share, and their
+ * counters).  The first EXL3_ATTN_COUNTER_BYTES are zero before the first call, and every call leaves them zero.  One
+ * workspace serves calls of any shape in stream order; overlapping calls race: give concurrent streams their own. */
+size_t exl3_paged_attention_workspace_size(void);
 
 /* out[t][h] = sum_j softmax_j(scale q[t][h] . k_j) v_j over the keys that token t sees: token i of request r's
  * n = cu_q[r + 1] - cu_q[r] new tokens (rows [cu_q[r], cu_q[r + 1]) of q) lies at position p = seq_lens[r] - n + i of the
@@ -385,6 +389,7 @@ size_t exl3_paged_attention_workspace_size(int tokens, int requests, int q_heads
  * One call takes decodes, drafts and prompt chunks together.  A row that sees nothing (a token of no request, a
  * negative position) is 0.  Keys that a token does not see have no effect on its row, whatever they hold; so have
  * positions whose table entry is no page and positions past table_cols * page_size.
+ * A row whose scores are all minus infinity is 0 too.
  * page_size: a multiple of 16.  cu_q: non-decreasing, 0 first; rows past `tokens` are dropped.
  * Scores, maxima, sums and outputs in fp32; a probability is rounded to the element type for its product with V.
  * Results are the same bits in every call with the same arguments. */

@@ -26,4 +26,154 @@ inline bool multiples_of_8(std::initializer_list<int64_t> ld)
     return std::all_of(ld.begin(), ld.end(), [](int64_t s) { return s >= 0 && s % 8 == 0; });
 }
 
+// out = sum / l of four columns; a row that saw nothing (l = 0) is 0
+template <class T>
+__device__ __forceinline__ void store_out(__attribute__((address_space(1))) uint16_t* at, f32x4 sum, float l)
+{
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    const float r = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<__attribute__((address_space(1))) T4*>(at) = T4{(T) (sum[0] * r), (T) (sum[1] * r), (T) (sum[2] * r), (T) (sum[3] * r)};
+}
+
+// ---- attention: one launch's arguments, and the work that its workgroups share ------------------------------
+struct AttnArgs {
+    const uint16_t *q, *k, *v;
+    int64_t q_ldt, q_ldh, k_ldp, k_ldt, k_ldh, v_ldp, v_ldt, v_ldh, o_ldt, o_ldh, ld_table;
+    const int *table, *cu_q, *seq;
+    uint16_t* out;
+    int tokens, requests, group, hkv, pages, page, window;
+    int cap;                                            // positions that a row of the table holds
+    float scale;                                        // times log2(e)
+    UDiv d_page, d_group;
+    uint32_t* counters;                                 // one per workgroup, zero between calls
+    float* part;                                        // partial tiles: two a workgroup
+};
+
+constexpr int ATTN_GRID = 256;                          // workgroups: one per CU
+constexpr int ATTN_SLOT = 8256;                         // floats of a partial tile: rows x D outputs, then (max, sum) a row
+
+// A request's new rows for one kv head, (token, head of the group) in token order, are cut into tiles of `rows`; a tile
+// reads the keys that any of its rows sees, in steps of KEYS.  A launch's work is the steps of every (kv head,
+// request, tile) in that order, and each workgroup takes an equal, contiguous share of it (at least `least` steps), so
+// the launch is balanced for any mix of lengths, none of which the host knows.
+struct AttnTile {
+    int first, last;                                    // new tokens of its first and last row
+    int lo, hi;                                         // keys [lo, hi) that any row sees
+    int step0, steps;                                   // its steps; one (of no key) where no row sees any
+};
+
+template <int ROWS, int KEYS>
+struct AttnWork {
+    const AttnArgs& a;
+    int r, t, h;                                        // request, tile, kv head
+    int tok0, n, pos0;                                  // the request's first row of q, new tokens, first position
+    AttnTile tile;
+
+    __device__ __forceinline__ AttnWork(const AttnArgs& args) : a(args) {}
+
+    __device__ __forceinline__ void request(int req)
+    {
+        r = req;
+        tok0 = min(max(a.cu_q[r], 0), a.tokens);
+        const int all = max(a.cu_q[r + 1] - tok0, 0);
+        n = min(all, a.tokens - tok0);
+        pos0 = max(a.seq[r], 0) - all;
+    }
+    __device__ __forceinline__ int tiles() const { return (n * a.group + ROWS - 1) / ROWS; }
+    __device__ __forceinline__ AttnTile tile_of(int i) const
+    {
+        AttnTile x;
+        x.first = (int) a.d_group.div((uint32_t) (i * ROWS));
+        x.last = (int) a.d_group.div((uint32_t) (min((i + 1) * ROWS, n * a.group) - 1));
+        x.hi = max(0, min(pos0 + x.last + 1, a.cap));
+        x.lo = a.window ? min(max(pos0 + x.first + 1 - a.window, 0), x.hi) : 0;
+        x.step0 = x.lo / KEYS;
+        x.steps = max(1, (x.hi + KEYS - 1) / KEYS - x.step0);
+        return x;
+    }
+
+    // Every thread sums the steps of its range of requests; a scan gives the total and finds the tile of this
+    // workgroup's first step.  lds: THREADS / 64 + 4 64-bit words.  Returns this workgroup's share [w, w_end) of the
+    // launch's steps (64 bits: long contexts times heads pass 2^32), w_end <= w if it has none; `off`: the first
+    // step's place in its tile; `per`: steps of a share.
+    template <int THREADS>
+    __device__ __forceinline__ void find(int wg, int least, uint64_t* lds, int64_t& w, int64_t& w_end, int& off, uint32_t& per)
+    {
+        const int tid = threadIdx.x, each = (a.requests + THREADS - 1) / THREADS, r0 = min(tid * each, a.requests), r1 = min(r0 + each, a.requests);
+        uint64_t sum = 0;
+        for (int i = r0; i < r1; ++i) {
+            request(i);
+            const int m = tiles();
+            for (int j = 0; j < m; ++j) sum += (uint64_t) tile_of(j).steps;
+        }
+        uint64_t upto = sum;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint64_t x = __shfl_up(upto, d);
+            if ((tid & 63) >= d) upto += x;
+        }
+        if ((tid & 63) == 63) lds[tid >> 6] = upto;
+        __syncthreads();
+        uint64_t total = 0;
+#pragma unroll
+        for (int i = 0; i < THREADS / 64; ++i) {
+            if (i < (tid >> 6)) upto += lds[i];
+            total += lds[i];
+        }
+        const uint64_t all = total * (uint64_t) a.hkv;
+        const uint64_t share = max((all + ATTN_GRID - 1) / ATTN_GRID, (uint64_t) least);
+        per = (uint32_t) min(share, (uint64_t) 1 << 30);   // above every tile's steps it divides them alike
+        w = (int64_t) wg * (int64_t) share;
+        w_end = (int64_t) min((uint64_t) w + share, all);
+        off = 0;
+        if (w >= w_end) return;                        // uniform
+        h = (int) ((uint64_t) w / total);
+        const uint64_t u = (uint64_t) w - (uint64_t) h * total;
+        if (u >= upto - sum && u < upto) {
+            uint64_t left = u - (upto - sum);
+            for (int i = r0; i < r1; ++i) {
+                request(i);
+                const int m = tiles();
+                int j = 0;
+                for (; j < m; ++j) {
+                    const int s = tile_of(j).steps;
+                    if (left < (uint64_t) s) break;
+                    left -= (uint64_t) s;
+                }
+                if (j < m) {
+                    int* o = reinterpret_cast<int*>(lds + THREADS / 64);
+                    o[0] = i;
+                    o[1] = j;
+                    o[2] = (int) left;
+                    break;
+                }
+            }
+        }
+        __syncthreads();
+        const int* o = reinterpret_cast<const int*>(lds + THREADS / 64);
+        t = __builtin_amdgcn_readfirstlane(o[1]);
+        off = __builtin_amdgcn_readfirstlane(o[2]);
+        request(__builtin_amdgcn_readfirstlane(o[0]));
+        tile = tile_of(t);
+    }
+    // the tile after this one (there is one)
+    __device__ __forceinline__ void next()
+    {
+        if (++t < tiles()) {
+            tile = tile_of(t);
+            return;
+        }
+        t = 0;
+        int i = r;
+        do {
+            if (++i == a.requests) {
+                i = 0;
+                ++h;
+            }
+            request(i);
+        } while (n == 0);
+        tile = tile_of(0);
+    }
+};
+
 }  // namespace exl3

@@ -1,103 +1,497 @@
-// exl3_attn.hip -- causal attention of each request's new tokens over its paged key/value cache.
+// exl3_attn.hip -- causal attention of each request's new tokens over its paged key/value cache: the entry point, and
+// the kernel for few rows per request (decodes and drafts).
 #include "exl3_attn.h"
+#include <type_traits>
 
 using namespace exl3;
 
 namespace {
 
-struct AttnArgs {
-    const uint16_t *q, *k, *v;
-    int64_t q_ldt, q_ldh, k_ldp, k_ldt, k_ldh, v_ldp, v_ldt, v_ldh, o_ldt, o_ldh, ld_table;
-    const int *table, *cu_q, *seq;
-    uint16_t* out;
-    int tokens, requests, hq, hkv, pages, cols, page, window;
-    float scale;
-    UDiv d_page, d_group;
+typedef __attribute__((address_space(1))) const char gc_char;
+
+template <class T> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c);
+template <> __device__ __forceinline__ f32x4 mfma16<f16>(u32x4 a, u32x4 b, f32x4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f32x4 mfma16<__bf16>(u32x4 a, u32x4 b, f32x4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// max / sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float max_quads(float x)
+{
+    float lo, hi;
+    halves_x(x, lo, hi);
+    x = fmaxf(lo, hi);
+    const auto w = __builtin_amdgcn_permlane16_swap((uint32_t) __float_as_int(x), (uint32_t) __float_as_int(x), false, false);
+    return fmaxf(__int_as_float((int) w[0]), __int_as_float((int) w[1]));
+}
+__device__ __forceinline__ float sum_quads(float x)
+{
+    float lo, hi;
+    halves_x(x, lo, hi);
+    x = lo + hi;
+    const auto w = __builtin_amdgcn_permlane16_swap((uint32_t) __float_as_int(x), (uint32_t) __float_as_int(x), false, false);
+    return __int_as_float((int) w[0]) + __int_as_float((int) w[1]);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// 0xFFFF in each half of x that is an infinity or NaN: adding one to an exponent of all ones reaches the sign's place
+// (integer arithmetic: 64 compares at once would take the scalar registers of 64 results)
+template <class T>
+__device__ __forceinline__ uint32_t nonfinite2(uint32_t x)
+{
+    constexpr uint32_t ONE = std::is_same_v<T, f16> ? 0x04000400u : 0x00800080u;
+    const uint32_t n = ((x & 0x7FFF7FFFu) + ONE) & 0x80008000u;
+    return n | (n - (n >> 15));
+}
+
+template <int N> struct Words;
+template <> struct Words<4> { typedef u32x4 T; typedef gc_u32x4 G; };
+template <> struct Words<2> { typedef u32x2 T; typedef gc_u32x2 G; };
+
+constexpr float LOWEST = -3.0e38f;                      // a running maximum that no key has raised
+
+// ---- few rows: 16 NQ rows a tile, bound by the reading of K and V --------------------------------------------
+// Every wave takes whole steps of 32 keys of its tile, with a softmax of its own (running maximum, sum, output), and
+// loads their K and V from memory straight into matrix operands, so the loop has no LDS traffic for them and no
+// barrier.  The next step's K is requested once this one's scores are formed, its V once this one's products are, so a
+// wave has about a step (128 D bytes) in flight at all times and each buffer is there once:
+//   S^T = K Q^T  (16x16x32): lane l gives key l & 15 of a page's 16, elements 32 c + 8 (l >> 4) .. + 7
+//   O^T = V^T P^T: S^T leaves lane l with keys 4 (l >> 4) + i (i < 4) of both 16s, row l & 15.  Taken as operand elements
+//         8 (l >> 4) + j that is already P^T, if V^T's lane holds the same keys: its loads are 16 bytes of 8 rows
+//         of V (a row's 16 lanes read it whole), paired by v_perm, and column 8 (l & 15) + e is row l & 15 of product e
+// A lane's row of S^T and of O^T is the same (l & 15), so maxima, sums and corrections never leave the lane's column.
+template <class T, int D, int NQ, int WAVES>
+struct Decode {
+    static constexpr int ROWS = 16 * NQ, THREADS = 64 * WAVES;
+    static constexpr int KC = D / 32;                   // 16-byte pieces of a K row that a lane holds
+    static constexpr int VW = D >= 128 ? 16 : 8;        // bytes of a V row that a lane loads at once
+    static constexpr int VC = D * 2 / (16 * VW);        // ... and how many times
+    static constexpr int E = VW / 2;                    // V columns of one load: its products
+    static constexpr int PAD = D + 4;                   // LDS row (floats) of the waves' outputs
+    static constexpr bool Q_LDS = NQ * KC > 4;          // Q would take more than 16 registers: read from LDS at each step
+    static constexpr int Q_PAD = D + 8;                 // its LDS row (halves)
+    static_assert(ROWS * D + 2 * ROWS <= ATTN_SLOT);
+    // fp16 probabilities are held times 2^8: the smallest that a key keeps is then 2^-33 of its row's largest
+    static constexpr float SHIFT = std::is_same_v<T, f16> ? 8.f : 0.f;
+    using V = typename Words<VW / 4>::T;
+    using GV = typename Words<VW / 4>::G;
+    using K2 = u32x4[2][KC];
+    using V8 = V[8][VC];
+
+    struct Shared {
+        float o[WAVES][16][PAD];
+        float m[WAVES][ROWS], l[WAVES][ROWS];
+        uint16_t q[Q_LDS ? ROWS : 1][Q_PAD];
+        uint64_t find[WAVES + 4];
+        int last;
+    };
+
+    // operand element j of product e of piece u: column e of the lane's piece, key 16 (j >> 2) + 4 (l >> 4) + (j & 3)
+    static __device__ __forceinline__ u32x4 column(const V8& v, int u, int e)
+    {
+        u32x4 r;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[j] = __builtin_amdgcn_perm(v[2 * j + 1][u][e / 2], v[2 * j][u][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+        return r;
+    }
 };
 
-// One wave per (token, query head): a lane scores one key of 64, the running maximum and sum follow, then every lane
-// sums its D / 64 columns over the 64 keys.
-template <class T, int D>
-__global__ void __launch_bounds__(64) attn_simple_kernel(AttnArgs a)
+// A split tile's parts, summed in the order of their workgroups: part c of workgroup c lies in slot 2 c, the first
+// one's in 2 c + 1.
+template <class T, int D, int ROWS, int THREADS, class At>
+__device__ __forceinline__ void join_parts(__amdgpu_buffer_rsrc_t prs, int first, int last, int rows, At&& out_at)
 {
-    constexpr int E = D / 64;
-    __shared__ float qs[D];
-    __shared__ float ps[64];
-    __shared__ int slots[64];
-    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, hk = (int) a.d_group.div((uint32_t) h);
-    for (int e = lane; e < D; e += 64) qs[e] = (float) __builtin_bit_cast(T, a.q[(int64_t) t * a.q_ldt + h * a.q_ldh + e]) * a.scale;
-    // the last request that starts at or before the token
-    int lo = 0, hi = a.requests;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (a.cu_q[mid] <= t) lo = mid;
-        else hi = mid;
-    }
-    int first = 0, end = 0;
-    if (a.requests > 0 && t >= a.cu_q[lo] && t < a.cu_q[lo + 1]) {
-        const int n = a.cu_q[lo + 1] - a.cu_q[lo], p = a.seq[lo] - n + (t - a.cu_q[lo]);
-        end = min(p + 1, a.cols * a.page);
-        if (a.window > 0) first = max(0, p + 1 - a.window);
-    }
-    float m = -INFINITY, l = 0.f, acc[E] = {};
-    for (int j0 = first; j0 < end; j0 += 64) {
-        const int j = j0 + lane;
-        float s = -INFINITY;
-        int slot = -1;
-        if (j < end) {
-            const int col = (int) a.d_page.div((uint32_t) j), page = a.table[(int64_t) lo * a.ld_table + col];
-            if ((unsigned) page < (unsigned) a.pages) {
-                slot = page * a.page + (j - col * a.page);
-                const uint16_t* kp = a.k + (int64_t) page * a.k_ldp + (int64_t) (j - col * a.page) * a.k_ldt + hk * a.k_ldh;
-                s = 0.f;
-                for (int e = 0; e < D; e += 8) {
-                    const auto kv = __builtin_bit_cast(typename Elem<T>::x8, *reinterpret_cast<const u32x4*>(kp + e));
+    auto slot = [&](int c) __attribute__((always_inline)) { return (uint32_t) (2 * c + (c == first ? 1 : 0)) * (uint32_t) ATTN_SLOT; };
+    for (int z = threadIdx.x; z < rows * (D / 4); z += THREADS) {
+        const int x = z / (D / 4), col = 4 * (z % (D / 4));
+        const uint32_t at = (uint32_t) (x * D + col), ml = (uint32_t) (ROWS * D + 2 * x);
+        float m = LOWEST, l = 0.f;
+        f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
+        constexpr int B = 8;
+        for (int c0 = first; c0 <= last; c0 += B) {
+            u32x2 mls[B];
+            f32x4 v[B];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) s = fmaf(qs[e + i], (float) kv[i], s);
+            for (int i = 0; i < B; ++i) {
+                const uint32_t s = slot(min(c0 + i, last));
+                mls[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(prs, (s + ml) * 4u, 0, SC1));
+                v[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(prs, (s + at) * 4u, 0, SC1));
+            }
+            float top = m;
+#pragma unroll
+            for (int i = 0; i < B; ++i) top = fmaxf(top, __int_as_float((int) mls[i][0]));
+            const float c = exp2_fast(m - top);
+            l *= c;
+            sum *= c;
+            m = top;
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                if (c0 + i > last) break;
+                const float f = exp2_fast(__int_as_float((int) mls[i][0]) - m);
+                l += f * __int_as_float((int) mls[i][1]);
+                sum += v[i] * f;
+            }
+        }
+        store_out<T>(out_at(x) + col, sum, l);
+    }
+}
+
+template <class T, int D, int NQ, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
+{
+    using X = Decode<T, D, NQ, WAVES>;
+    constexpr int KC = X::KC, VC = X::VC, E = X::E, ROWS = X::ROWS;
+    __shared__ typename X::Shared sh;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c16 = lane & 15, g4 = lane >> 4;
+    const int wg = blockIdx.x;
+
+    // rows of no request
+    const int used = a.requests ? min(max(a.cu_q[a.requests], 0), a.tokens) : 0;
+    for (int t = used + wg; t < a.tokens; t += ATTN_GRID)
+        for (int i = tid; i < a.group * a.hkv * (D / 8); i += X::THREADS)
+            *reinterpret_cast<g_u32x4*>(as_global(a.out) + (int64_t) t * a.o_ldt + (i / (D / 8)) * a.o_ldh + 8 * (i % (D / 8))) = u32x4{0u, 0u, 0u, 0u};
+
+    AttnWork<ROWS, 32> wk(a);
+    int64_t w, w_end;
+    int off;
+    uint32_t per;
+    wk.template find<X::THREADS>(wg, WAVES, sh.find, w, w_end, off, per);
+    if (w >= w_end) return;
+
+    const uint32_t k_lane = (uint32_t) (c16 * (int) a.k_ldt + 8 * g4) * 2u;
+    uint32_t v_lane[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v_lane[i] = (uint32_t) ((4 * g4 + i) * (int) a.v_ldt) * 2u + (uint32_t) (X::VW * c16);
+
+    while (w < w_end) {
+        const AttnTile tile = wk.tile;
+        const int n_steps = (int) min((int64_t) (tile.steps - off), w_end - w);
+        const int s0 = tile.step0 + off, s1 = s0 + n_steps;
+        const int* const row = a.table + (int64_t) wk.r * a.ld_table;
+        const char* const kh = reinterpret_cast<const char*>(a.k + (int64_t) wk.h * a.k_ldh);
+        const char* const vh = reinterpret_cast<const char*>(a.v + (int64_t) wk.h * a.v_ldh);
+
+        // Q^T: lane's row 16 i + c16 of the tile, elements 32 c + 8 g4 ..; and the position of the row's token
+        const int rows = wk.n * a.group;
+        auto q_at = [&](int x) __attribute__((always_inline)) {
+            const int y = min(wk.t * ROWS + x, rows - 1), tok = (int) a.d_group.div((uint32_t) y);
+            return as_global(a.q) + (int64_t) (wk.tok0 + tok) * a.q_ldt + (int64_t) (wk.h * a.group + y - tok * a.group) * a.q_ldh;
+        };
+        u32x4 q[NQ][X::Q_LDS ? 1 : KC];
+        int rpos[NQ];
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            const int x = wk.t * ROWS + 16 * i + c16;
+            rpos[i] = x < rows ? wk.pos0 + (int) a.d_group.div((uint32_t) x) : -1;  // a row past the tile's sees nothing
+            if constexpr (!X::Q_LDS) {
+                auto* const src = q_at(16 * i + c16) + 8 * g4;
+#pragma unroll
+                for (int c = 0; c < KC; ++c) q[i][c] = *reinterpret_cast<gc_u32x4*>(src + 32 * c);
+            }
+        }
+        if constexpr (X::Q_LDS) {
+            for (int z = tid; z < ROWS * D / 8; z += X::THREADS)
+                *reinterpret_cast<u32x4*>(&sh.q[z / (D / 8)][8 * (z % (D / 8))]) = *reinterpret_cast<gc_u32x4*>(q_at(z / (D / 8)) + 8 * (z % (D / 8)));
+            __syncthreads();
+        }
+        f32x4 o[NQ][VC][E];
+        float m[NQ], l[NQ];
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            m[i] = LOWEST;
+            l[i] = 0.f;
+#pragma unroll
+            for (int c = 0; c < VC; ++c)
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[i][c][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+
+        // pages of this wave's next 32 steps, lane 2 x + y: the y-th 16 keys of its x-th step; -1: none
+        auto pages_from = [&](int s) __attribute__((always_inline)) {
+            const int key = 32 * (s + WAVES * (lane >> 1)) + 16 * (lane & 1);
+            int p = -1;
+            if (key < tile.hi) {
+                p = row[a.d_page.div((uint32_t) key)];
+                if ((unsigned) p >= (unsigned) a.pages) p = -1;
+            }
+            return p;
+        };
+        // the first of 16 keys from `key` on of page p of a cache; -1 reads page 0, and its keys are seen by nobody
+        auto keys_at = [&](const char* base, int64_t ldp, int64_t ldt, int p, int key) __attribute__((always_inline)) {
+            const int in = key - (int) a.d_page.div((uint32_t) key) * a.page;
+            return as_global(base) + ((int64_t) max(p, 0) * ldp + (int64_t) in * ldt) * 2;
+        };
+        auto load_k = [&](typename X::K2& x, int s, int p0, int p1) __attribute__((always_inline)) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                gc_char* const kp = keys_at(kh, a.k_ldp, a.k_ldt, y ? p1 : p0, 32 * s + 16 * y);
+#pragma unroll
+                for (int c = 0; c < KC; ++c) x[y][c] = *reinterpret_cast<gc_u32x4*>(kp + k_lane + 64 * c);
+            }
+        };
+        auto load_v = [&](typename X::V8& x, int s, int p0, int p1) __attribute__((always_inline)) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                gc_char* const vp = keys_at(vh, a.v_ldp, a.v_ldt, y ? p1 : p0, 32 * s + 16 * y);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < VC; ++c) x[4 * y + i][c] = *reinterpret_cast<typename X::GV*>(vp + v_lane[i] + 16 * X::VW * c);
+            }
+        };
+
+        int s = s0 + wave;
+        if (s < s1 && tile.lo < tile.hi) {
+            typename X::K2 k;
+            typename X::V8 v;
+            int pg = pages_from(s), at = 0, p0 = __builtin_amdgcn_readlane(pg, 0), p1 = __builtin_amdgcn_readlane(pg, 1);
+            load_k(k, s, p0, p1);
+            load_v(v, s, p0, p1);
+            int pg_next = pages_from(s + 32 * WAVES);
+            while (true) {
+                const int next = s + WAVES;
+                int n0 = 0, n1 = 0;
+                if (next < s1) {
+                    if (++at == 32) {
+                        pg = pg_next;
+                        pg_next = pages_from(next + 32 * WAVES);
+                        at = 0;
+                    }
+                    n0 = __builtin_amdgcn_readlane(pg, 2 * at);
+                    n1 = __builtin_amdgcn_readlane(pg, 2 * at + 1);
+                }
+                // whether every row sees every key of the step
+                const bool whole = p0 >= 0 && p1 >= 0 && 32 * s + 31 <= wk.pos0 + tile.first && (!a.window || 32 * s > wk.pos0 + tile.last - a.window) &&
+                                   32 * s + 32 <= a.cap;
+                f32x4 st[NQ][2];
+#pragma unroll
+                for (int i = 0; i < NQ; ++i)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) st[i][y] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < KC; ++c)
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i) {
+                        u32x4 qc;
+                        if constexpr (X::Q_LDS) qc = *reinterpret_cast<const u32x4*>(&sh.q[16 * i + c16][32 * c + 8 * g4]);
+                        else qc = q[i][c];
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) st[i][y] = mfma16<T>(k[y][c], qc, st[i][y]);
+                    }
+                if (next < s1) load_k(k, next, n0, n1);
+                u32x4 pb[NQ];
+#pragma unroll
+                for (int i = 0; i < NQ; ++i) {
+                    float mx = m[i];
+#pragma unroll
+                    for (int y = 0; y < 2; ++y)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float x = st[i][y][e] * a.scale;
+                            if (!whole) {
+                                const int key = 32 * s + 16 * y + 4 * g4 + e;
+                                const bool seen = key <= rpos[i] && key < a.cap && (!a.window || key > rpos[i] - a.window) && (y ? p1 : p0) >= 0;
+                                x = seen ? x : -INFINITY;
+                            }
+                            st[i][y][e] = x;
+                            mx = fmaxf(mx, x);
+                        }
+                    mx = max_quads(mx);
+                    if (__any(mx > m[i])) {
+                        const float c = exp2_fast(m[i] - mx);
+                        l[i] *= c;
+#pragma unroll
+                        for (int u = 0; u < VC; ++u)
+#pragma unroll
+                            for (int e = 0; e < E; ++e) o[i][u][e] *= c;
+                        m[i] = mx;
+                    }
+                    const float base = m[i] - X::SHIFT;
+                    typename Elem<T>::x8 p;
+#pragma unroll
+                    for (int y = 0; y < 2; ++y)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float x = exp2_fast(st[i][y][e] - base);
+                            l[i] += x;
+                            p[4 * y + e] = (T) x;
+                        }
+                    pb[i] = __builtin_bit_cast(u32x4, p);
+                }
+                // What V holds for keys that a row does not see must not reach it, and a probability of 0 does not hide
+                // an infinity or NaN: V of keys that no row sees is zeroed, and where rows of several tokens differ in what
+                // they see, such elements are zeroed too and added afterwards to the rows that see them.
+                bool odd = false;
+                if (!whole) {
+                    uint32_t f = 0;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int key = 32 * s + 16 * (i >> 2) + 4 * g4 + (i & 3);
+                        const bool live = key >= tile.lo && key < tile.hi && (i < 4 ? p0 : p1) >= 0;
+#pragma unroll
+                        for (int c = 0; c < VC; ++c)
+#pragma unroll
+                            for (int e = 0; e < E / 2; ++e) {
+                                v[i][c][e] = live ? v[i][c][e] : 0u;
+                                f |= nonfinite2<T>(v[i][c][e]);
+                            }
+                    }
+                    odd = tile.first != tile.last && __any(f != 0u);
+                    if (odd) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+#pragma unroll
+                            for (int c = 0; c < VC; ++c)
+#pragma unroll
+                                for (int e = 0; e < E / 2; ++e) v[i][c][e] &= ~nonfinite2<T>(v[i][c][e]);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < VC; ++u)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const u32x4 vt = X::column(v, u, e);
+#pragma unroll
+                        for (int i = 0; i < NQ; ++i) o[i][u][e] = mfma16<T>(vt, pb[i], o[i][u][e]);
+                    }
+                if (odd) {
+#pragma unroll 1
+                    for (int y = 0; y < 32; ++y) {
+                        const int key = 32 * s + y, j = 2 * (y >> 4) + ((y & 3) >> 1);
+                        if (key < tile.lo || key >= tile.hi || (y < 16 ? p0 : p1) < 0) continue;
+                        gc_u16* const vr = reinterpret_cast<gc_u16*>(keys_at(vh, a.v_ldp, a.v_ldt, y < 16 ? p0 : p1, 32 * s + (y & 16)) + (int64_t) (y & 15) * a.v_ldt * 2);
+#pragma unroll
+                        for (int i = 0; i < NQ; ++i) {
+                            uint32_t pw = j == 0 ? pb[i][0] : j == 1 ? pb[i][1] : j == 2 ? pb[i][2] : pb[i][3];
+                            pw = (uint32_t) __shfl((int) pw, 16 * ((y >> 2) & 3) + c16);
+                            const float p = (float) __builtin_bit_cast(T, (uint16_t) (y & 1 ? pw >> 16 : pw));
+                            const uint32_t seen = key <= rpos[i] && (!a.window || key > rpos[i] - a.window) ? 0xFFFFu : 0u;
+#pragma unroll
+                            for (int u = 0; u < VC; ++u)
+#pragma unroll
+                                for (int e = 0; e < E; ++e)
+#pragma unroll
+                                    for (int d = 0; d < 4; ++d) {
+                                        const uint32_t b = vr[16 * E * u + E * (4 * g4 + d) + e];
+                                        o[i][u][e][d] += p * (float) __builtin_bit_cast(T, (uint16_t) (b & seen & nonfinite2<T>(b)));
+                                    }
+                        }
+                    }
+                }
+                if (next >= s1) break;
+                load_v(v, next, n0, n1);
+                s = next;
+                p0 = n0;
+                p1 = n1;
+            }
+        }
+
+        // the waves' outputs joined: maxima and sums first, then 16 rows at a time
+        const bool starts = off == 0, ends = off + n_steps == tile.steps, split = !(starts && ends);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            l[i] = sum_quads(l[i]);
+            if (g4 == 0) {
+                sh.m[wave][16 * i + c16] = m[i];
+                sh.l[wave][16 * i + c16] = l[i];
+            }
+        }
+        __syncthreads();
+        const int first_wg = wg - (int) (((uint32_t) off + per - 1u) / per);        // workgroups back to the tile's first step
+        const uint32_t slot = 2u * (uint32_t) wg + (starts ? 1u : 0u);
+        const __amdgpu_buffer_rsrc_t prs = __builtin_amdgcn_make_buffer_rsrc(a.part, 0, 2 * ATTN_GRID * ATTN_SLOT * 4, RAW_BUFFER_FLAGS);
+        auto out_at = [&](int x) __attribute__((always_inline)) {                  // row x of the tile
+            const int y = wk.t * ROWS + x, tok = (int) a.d_group.div((uint32_t) y);
+            return as_global(a.out) + (int64_t) (wk.tok0 + tok) * a.o_ldt + (int64_t) (wk.h * a.group + y - tok * a.group) * a.o_ldh;
+        };
+        const int live_rows = min(ROWS, rows - wk.t * ROWS);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            if (16 * i >= live_rows) break;            // uniform
+            float top = LOWEST;
+#pragma unroll
+            for (int x = 0; x < WAVES; ++x) top = fmaxf(top, sh.m[x][16 * i + c16]);
+            const float c = exp2_fast(m[i] - top);
+            if (i) __syncthreads();
+#pragma unroll
+            for (int u = 0; u < VC; ++u)
+#pragma unroll
+                for (int y = 0; y < 4; ++y)            // product e holds columns E (4 g4 + y) + e of piece u
+#pragma unroll
+                    for (int e = 0; e < E; e += 4)
+                        *reinterpret_cast<f32x4*>(&sh.o[wave][c16][16 * E * u + E * (4 * g4 + y) + e]) =
+                            f32x4{o[i][u][e][y] * c, o[i][u][e + 1][y] * c, o[i][u][e + 2][y] * c, o[i][u][e + 3][y] * c};
+            __syncthreads();
+            for (int z = tid; z < 16 * D / 4; z += X::THREADS) {
+                const int x = z / (D / 4), col = 4 * (z % (D / 4));
+                if (16 * i + x >= live_rows) continue;
+                float mt = LOWEST, lt = 0.f;
+                f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int y = 0; y < WAVES; ++y) mt = fmaxf(mt, sh.m[y][16 * i + x]);
+#pragma unroll
+                for (int y = 0; y < WAVES; ++y) {
+                    lt += sh.l[y][16 * i + x] * exp2_fast(sh.m[y][16 * i + x] - mt);
+                    sum += *reinterpret_cast<const f32x4*>(&sh.o[y][x][col]);
+                }
+                if (!split) {
+                    store_out<T>(out_at(16 * i + x) + col, sum, lt);
+                } else {
+                    const uint32_t at = (slot * ATTN_SLOT + (uint32_t) (16 * i + x) * D + (uint32_t) col) * 4u;
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum), prs, at, 0, SC1);
+                    if (col == 0) {
+                        const u32x2 ml = u32x2{(uint32_t) __float_as_int(mt), (uint32_t) __float_as_int(lt)};
+                        __builtin_amdgcn_raw_buffer_store_b64(ml, prs, (slot * ATTN_SLOT + (uint32_t) (ROWS * D + 2 * (16 * i + x))) * 4u, 0, SC1);
+                    }
                 }
             }
         }
-        float mx = s;
-        for (int x = 1; x < 64; x <<= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
-        mx = fmaxf(mx, m);
-        if (mx == -INFINITY) continue;                  // nothing seen so far (uniform)
-        const float p = slot < 0 ? 0.f : __expf(s - mx), c = __expf(m - mx);
-        float sum = p;
-        for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
-        l = l * c + sum;
-        m = mx;
-        __syncthreads();
-        ps[lane] = p;
-        slots[lane] = slot;
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] *= c;
-        for (int i = 0; i < 64; ++i) {
-            const int sl = slots[i];
-            if (sl < 0) continue;
-            const int page = (int) a.d_page.div((uint32_t) sl);
-            const uint16_t* vp = a.v + (int64_t) page * a.v_ldp + (int64_t) (sl - page * a.page) * a.v_ldt + hk * a.v_ldh;
-#pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = fmaf(ps[i], (float) __builtin_bit_cast(T, vp[lane + 64 * e]), acc[e]);
+        if (split) {
+            // the workgroup that counts last joins the tile's parts, in the order of the workgroups
+            const int last_wg = wg + (int) (((uint32_t) (tile.steps - off - n_steps) + per - 1u) / per);
+            __builtin_amdgcn_s_waitcnt(0x0F70);        // vmcnt(0): the part has landed
+            __syncthreads();
+            if (tid == 0) {
+                const uint32_t before = __hip_atomic_fetch_add(&a.counters[first_wg], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                sh.last = before == (uint32_t) (last_wg - first_wg);
+                if (sh.last) __hip_atomic_store(&a.counters[first_wg], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            __syncthreads();
+            if (sh.last) join_parts<T, D, ROWS, X::THREADS>(prs, first_wg, last_wg, live_rows, out_at);
         }
+        __syncthreads();
+        w += n_steps;
+        off = 0;
+        if (w < w_end) wk.next();
     }
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-        a.out[(int64_t) t * a.o_ldt + h * a.o_ldh + lane + 64 * e] = __builtin_bit_cast(uint16_t, (T) (l == 0.f ? 0.f : acc[e] / l));
+}
+
+template <class T, int D, int NQ, int WAVES>
+void launch_decode(const AttnArgs& a, hipStream_t s)
+{
+    hipLaunchKernelGGL((attn_decode_kernel<T, D, NQ, WAVES>), dim3(ATTN_GRID), dim3(64 * WAVES), 0, s, a);
 }
 
 template <class T>
-void launch_simple(const AttnArgs& a, int d, hipStream_t s)
+void launch(const AttnArgs& a, int d, hipStream_t s)
 {
-    auto* kern = d == 64 ? attn_simple_kernel<T, 64> : d == 128 ? attn_simple_kernel<T, 128> : attn_simple_kernel<T, 256>;
-    hipLaunchKernelGGL(kern, dim3((unsigned) a.tokens, (unsigned) a.hq), dim3(64), 0, s, a);
+    // rows of an average request and kv head
+    const int64_t rows = a.requests ? (int64_t) a.tokens * a.group / a.requests : 0;
+    if (d == 64) rows <= 16 ? launch_decode<T, 64, 1, 16>(a, s) : launch_decode<T, 64, 4, 8>(a, s);
+    else if (d == 128) rows <= 16 ? launch_decode<T, 128, 1, 12>(a, s) : launch_decode<T, 128, 2, 8>(a, s);
+    else rows <= 16 ? launch_decode<T, 256, 1, 8>(a, s) : launch_decode<T, 256, 2, 4>(a, s);
 }
 
 }  // namespace
 
-extern "C" size_t exl3_paged_attention_workspace_size(int tokens, int requests, int q_heads, int kv_heads, int head_dim)
+extern "C" size_t exl3_paged_attention_workspace_size(void)
 {
-    return 0;
+    return EXL3_ATTN_COUNTER_BYTES + (size_t) 2 * ATTN_GRID * ATTN_SLOT * 4;
 }
 
 extern "C" int exl3_paged_attention(const void* q, int64_t q_ldt, int64_t q_ldh, const void* k_cache, int64_t k_ldp, int64_t k_ldt,
@@ -110,17 +504,23 @@ extern "C" int exl3_paged_attention(const void* q, int64_t q_ldt, int64_t q_ldh,
     if (tokens < 0 || tokens > EXL3_PAGED_MAX_TOKENS || requests < 0 || requests > EXL3_PAGED_MAX_REQUESTS) return EXL3_EINVAL;
     if (q_heads < 1 || q_heads > EXL3_PAGED_MAX_HEADS || kv_heads < 1 || q_heads % kv_heads || !paged_head_dim(head_dim) || !paged_dtype(dtype))
         return EXL3_EINVAL;
+    if ((int64_t) tokens * (q_heads / kv_heads) > INT32_MAX - 1024) return EXL3_EINVAL;
     if (pages < 0 || page_size < 16 || page_size % 16 || page_size > EXL3_PAGED_MAX_PAGE || (int64_t) pages * page_size > INT32_MAX) return EXL3_EINVAL;
-    if (table_cols < 0 || ld_table < table_cols || (int64_t) table_cols * page_size > INT32_MAX || window < 0) return EXL3_EINVAL;
+    if (table_cols < 0 || ld_table < table_cols || (int64_t) table_cols * page_size > INT32_MAX - 65536 || window < 0) return EXL3_EINVAL;
+    if (window > EXL3_ATTN_MAX_WINDOW) return EXL3_EINVAL;
+    if (k_ldt > EXL3_ATTN_MAX_LDT || v_ldt > EXL3_ATTN_MAX_LDT) return EXL3_EINVAL;
     if (tokens == 0) return EXL3_OK;
     if (!q || !out || !cu_q || (pages && (!k_cache || !v_cache)) || (requests && !seq_lens) || (requests && table_cols && !block_table)) return EXL3_EINVAL;
     if (!aligned16({q, k_cache, v_cache, out}) ||
         !multiples_of_8({q_ldt, q_ldh, k_ldp, k_ldt, k_ldh, v_ldp, v_ldt, v_ldh, o_ldt, o_ldh}))
         return EXL3_EINVAL;
+    if (!workspace || ((uintptr_t) workspace & 15u) || ws_bytes < exl3_paged_attention_workspace_size()) return EXL3_EWORKSPACE;
     AttnArgs a{(const uint16_t*) q, (const uint16_t*) k_cache, (const uint16_t*) v_cache, q_ldt, q_ldh, k_ldp, k_ldt, k_ldh, v_ldp, v_ldt,
-               v_ldh, o_ldt, o_ldh, ld_table, block_table, cu_q, seq_lens, (uint16_t*) out, tokens, requests, q_heads, kv_heads, pages,
-               table_cols, page_size, window, scale, UDiv::of((uint32_t) page_size), UDiv::of((uint32_t) (q_heads / kv_heads))};
-    if (dtype == EXL3_FP16) launch_simple<f16>(a, head_dim, (hipStream_t) stream);
-    else launch_simple<__bf16>(a, head_dim, (hipStream_t) stream);
+               v_ldh, o_ldt, o_ldh, ld_table, block_table, cu_q, seq_lens, (uint16_t*) out, tokens, requests, q_heads / kv_heads, kv_heads,
+               pages, page_size, window, pages ? table_cols * page_size : 0, scale * 1.44269504f, UDiv::of((uint32_t) page_size),
+               UDiv::of((uint32_t) (q_heads / kv_heads)), (uint32_t*) workspace,
+               reinterpret_cast<float*>((char*) workspace + EXL3_ATTN_COUNTER_BYTES)};
+    if (dtype == EXL3_FP16) launch<f16>(a, head_dim, (hipStream_t) stream);
+    else launch<__bf16>(a, head_dim, (hipStream_t) stream);
     return hipGetLastError() == hipSuccess ? EXL3_OK : EXL3_ELAUNCH;
 }

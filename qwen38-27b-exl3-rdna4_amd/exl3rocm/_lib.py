@@ -63,7 +63,7 @@ SIGNATURES = {
     "exl3_batch_plan": (_i, [_p, _p, _p, _i64, _i, _p, _i, _p, _p, _p, _p, _p, _p, _i, _i, _i, _p]),
     "exl3_rope_kv_write": (_i, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64,
                                 _p, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p]),
-    "exl3_paged_attention_workspace_size": (_sz, [_i, _i, _i, _i, _i]),
+    "exl3_paged_attention_workspace_size": (_sz, []),
     "exl3_paged_attention": (_i, [_p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i, _p, _p, _p, _i64, _i64,
                                   _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _p, _sz, _p]),
     "exl3_gemv_mr_noalloc": (_i, [_p, _i64, _p, _p, _i64, _p, _p, _i, _i, _i, _i, _i, _i, _p]),

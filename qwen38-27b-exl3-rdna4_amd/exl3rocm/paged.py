@@ -155,6 +155,19 @@ def rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     return out
 
 
+_workspaces: dict = {}      # (device, stream) -> zeroed workspace of paged_attention
+
+
+def _workspace(device: torch.device, stream: int) -> torch.Tensor:
+    """The stream's workspace: one size serves every shape, so a stream that made one eager call can capture any."""
+    ws = _workspaces.get((device, stream))
+    if ws is None:
+        _need(not torch.cuda.is_current_stream_capturing(), "paged_attention: this stream made no eager call before graph capture")
+        ws = torch.zeros(int(L.lib().exl3_paged_attention_workspace_size()), dtype=torch.uint8, device=device)
+        _workspaces[(device, stream)] = ws
+    return ws
+
+
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, cu_q: torch.Tensor,
                     seq_lens: torch.Tensor, scale: float, window: int = 0) -> torch.Tensor:
     """Causal attention [T, q_heads, D] of the rows of q [T, q_heads, D] (any token and head strides that are multiples of
@@ -178,15 +191,16 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     _need(block_table.dtype == torch.int32 and block_table.device == dev and block_table.dim() == 2 and block_table.shape[0] == R
           and (block_table.shape[1] <= 1 or block_table.stride(1) == 1),
           f"paged_attention: block_table must be int32 [{R}, columns] on {dev} with unit column stride")
-    _need(window >= 0, "paged_attention: window from 0 (0: none)")
+    _need(0 <= window <= 1 << 30, "paged_attention: window from 0 (none) to 2 ** 30")
     cols = block_table.shape[1]
     out = torch.empty((T, hq, d), dtype=dt, device=dev)
     st = _stream(q)
+    ws = _workspace(dev, st)
     L.check(L.lib().exl3_paged_attention(q.data_ptr(), *_ld(q, 2), k_cache.data_ptr(), *_ld(k_cache, 3),
                                          v_cache.data_ptr(), *_ld(v_cache, 3), block_table.data_ptr(),
                                          block_table.stride(0) if R > 1 else cols, cols, cu_q.data_ptr(), seq_lens.data_ptr(),
                                          out.data_ptr(), hq * d, d, T, R, hq, hkv, d, pages, page, scale, window, _DTYPES[dt],
-                                         None, 0, st), "paged_attention")
+                                         ws.data_ptr(), ws.numel(), st), "paged_attention")
     return out
 
 
