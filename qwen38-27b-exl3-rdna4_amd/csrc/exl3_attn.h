@@ -26,6 +26,12 @@ inline bool multiples_of_8(std::initializer_list<int64_t> ld)
     return std::all_of(ld.begin(), ld.end(), [](int64_t s) { return s >= 0 && s % 8 == 0; });
 }
 
+__device__ __forceinline__ uint64_t uniform(uint64_t x)
+{
+    return (uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) (uint32_t) x) |
+           (uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) (uint32_t) (x >> 32)) << 32;
+}
+
 // out = sum / l of four columns; a row that saw nothing (l = 0) is 0
 template <class T>
 __device__ __forceinline__ void store_out(__attribute__((address_space(1))) uint16_t* at, f32x4 sum, float l)
@@ -93,11 +99,11 @@ struct AttnWork {
     }
 
     // Every thread sums the steps of its range of requests; a scan gives the total and finds the tile of this
-    // workgroup's first step.  lds: THREADS / 64 + 4 64-bit words.  Returns this workgroup's share [w, w_end) of the
-    // launch's steps (64 bits: long contexts times heads pass 2^32), w_end <= w if it has none; `off`: the first
-    // step's place in its tile; `per`: steps of a share.
+    // workgroup's first step.  lds: THREADS / 64 + 4 64-bit words.  False: this workgroup has no share.  off: the first
+    // step's place in its tile; left: the steps of the share (64 bits: long contexts times heads pass 2^32); per: those of
+    // a whole share, as far as a tile's steps can tell (below 2^30).  All but the sums is uniform, in scalar registers.
     template <int THREADS>
-    __device__ __forceinline__ void find(int wg, int least, uint64_t* lds, int64_t& w, int64_t& w_end, int& off, uint32_t& per)
+    __device__ __forceinline__ bool find(int wg, int least, uint64_t* lds, int& off, int64_t& left, uint32_t& per)
     {
         const int tid = threadIdx.x, each = (a.requests + THREADS - 1) / THREADS, r0 = min(tid * each, a.requests), r1 = min(r0 + each, a.requests);
         uint64_t sum = 0;
@@ -114,47 +120,52 @@ struct AttnWork {
         }
         if ((tid & 63) == 63) lds[tid >> 6] = upto;
         __syncthreads();
-        uint64_t total = 0;
-#pragma unroll
+        uint64_t sums = 0;
+#pragma unroll 4
         for (int i = 0; i < THREADS / 64; ++i) {
             if (i < (tid >> 6)) upto += lds[i];
-            total += lds[i];
+            sums += lds[i];
         }
-        const uint64_t all = total * (uint64_t) a.hkv;
+        const uint64_t total = uniform(sums), all = total * (uint64_t) a.hkv;
         const uint64_t share = max((all + ATTN_GRID - 1) / ATTN_GRID, (uint64_t) least);
-        per = (uint32_t) min(share, (uint64_t) 1 << 30);   // above every tile's steps it divides them alike
-        w = (int64_t) wg * (int64_t) share;
-        w_end = (int64_t) min((uint64_t) w + share, all);
-        off = 0;
-        if (w >= w_end) return;                        // uniform
-        h = (int) ((uint64_t) w / total);
-        const uint64_t u = (uint64_t) w - (uint64_t) h * total;
+        uint64_t u = (uint64_t) wg * share;
+        if (u >= all) return false;
+        per = (uint32_t) min(share, (uint64_t) 1 << 30);
+        left = (int64_t) min(share, all - u);
+        h = 0;
+        for (; u >= total; u -= total) ++h;
         if (u >= upto - sum && u < upto) {
-            uint64_t left = u - (upto - sum);
-            for (int i = r0; i < r1; ++i) {
+            uint64_t x = u - (upto - sum);
+            for (int i = r0;; ++i) {
                 request(i);
                 const int m = tiles();
-                int j = 0;
+                int j = 0, steps = 0;
                 for (; j < m; ++j) {
-                    const int s = tile_of(j).steps;
-                    if (left < (uint64_t) s) break;
-                    left -= (uint64_t) s;
+                    steps = tile_of(j).steps;
+                    if (x < (uint64_t) steps) break;
+                    x -= (uint64_t) steps;
                 }
-                if (j < m) {
-                    int* o = reinterpret_cast<int*>(lds + THREADS / 64);
-                    o[0] = i;
-                    o[1] = j;
-                    o[2] = (int) left;
-                    break;
-                }
+                if (j == m) continue;
+                int* o = reinterpret_cast<int*>(lds + THREADS / 64);
+                o[0] = i;
+                o[1] = j;
+                o[2] = (int) x;
+                o[3] = tok0;
+                o[4] = n;
+                o[5] = pos0;
+                break;
             }
         }
         __syncthreads();
         const int* o = reinterpret_cast<const int*>(lds + THREADS / 64);
+        r = __builtin_amdgcn_readfirstlane(o[0]);
         t = __builtin_amdgcn_readfirstlane(o[1]);
         off = __builtin_amdgcn_readfirstlane(o[2]);
-        request(__builtin_amdgcn_readfirstlane(o[0]));
+        tok0 = __builtin_amdgcn_readfirstlane(o[3]);
+        n = __builtin_amdgcn_readfirstlane(o[4]);
+        pos0 = __builtin_amdgcn_readfirstlane(o[5]);
         tile = tile_of(t);
+        return true;
     }
     // the tile after this one (there is one)
     __device__ __forceinline__ void next()
@@ -171,6 +182,9 @@ struct AttnWork {
                 ++h;
             }
             request(i);
+            tok0 = __builtin_amdgcn_readfirstlane(tok0);
+            n = __builtin_amdgcn_readfirstlane(n);
+            pos0 = __builtin_amdgcn_readfirstlane(pos0);
         } while (n == 0);
         tile = tile_of(0);
     }

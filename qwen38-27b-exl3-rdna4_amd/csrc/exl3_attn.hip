@@ -72,6 +72,7 @@ struct Decode {
     static constexpr int VW = D >= 128 ? 16 : 8;        // bytes of a V row that a lane loads at once
     static constexpr int VC = D * 2 / (16 * VW);        // ... and how many times
     static constexpr int E = VW / 2;                    // V columns of one load: its products
+    static constexpr int LEAST = 4;                     // steps of a share at least
     static constexpr int PAD = D + 4;                   // LDS row (floats) of the waves' outputs
     static constexpr bool Q_LDS = NQ * KC > 4;          // Q would take more than 16 registers: read from LDS at each step
     static constexpr int Q_PAD = D + 8;                 // its LDS row (halves)
@@ -85,7 +86,7 @@ struct Decode {
 
     struct Shared {
         float o[WAVES][16][PAD];
-        float m[WAVES][ROWS], l[WAVES][ROWS];
+        float m[WAVES][ROWS], l[WAVES][16];
         uint16_t q[Q_LDS ? ROWS : 1][Q_PAD];
         uint64_t find[WAVES + 4];
         int last;
@@ -131,8 +132,7 @@ __device__ __forceinline__ void join_parts(__amdgpu_buffer_rsrc_t prs, int first
             m = top;
 #pragma unroll
             for (int i = 0; i < B; ++i) {
-                if (c0 + i > last) break;
-                const float f = exp2_fast(__int_as_float((int) mls[i][0]) - m);
+                const float f = c0 + i <= last ? exp2_fast(__int_as_float((int) mls[i][0]) - m) : 0.f;
                 l += f * __int_as_float((int) mls[i][1]);
                 sum += v[i] * f;
             }
@@ -157,20 +157,19 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
             *reinterpret_cast<g_u32x4*>(as_global(a.out) + (int64_t) t * a.o_ldt + (i / (D / 8)) * a.o_ldh + 8 * (i % (D / 8))) = u32x4{0u, 0u, 0u, 0u};
 
     AttnWork<ROWS, 32> wk(a);
-    int64_t w, w_end;
+    int64_t left;
     int off;
     uint32_t per;
-    wk.template find<X::THREADS>(wg, WAVES, sh.find, w, w_end, off, per);
-    if (w >= w_end) return;
+    if (!wk.template find<X::THREADS>(wg, X::LEAST, sh.find, off, left, per)) return;
 
     const uint32_t k_lane = (uint32_t) (c16 * (int) a.k_ldt + 8 * g4) * 2u;
     uint32_t v_lane[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) v_lane[i] = (uint32_t) ((4 * g4 + i) * (int) a.v_ldt) * 2u + (uint32_t) (X::VW * c16);
 
-    while (w < w_end) {
+    while (true) {
         const AttnTile tile = wk.tile;
-        const int n_steps = (int) min((int64_t) (tile.steps - off), w_end - w);
+        const int n_steps = (int) min((int64_t) (tile.steps - off), left);
         const int s0 = tile.step0 + off, s1 = s0 + n_steps;
         const int* const row = a.table + (int64_t) wk.r * a.ld_table;
         const char* const kh = reinterpret_cast<const char*>(a.k + (int64_t) wk.h * a.k_ldh);
@@ -183,11 +182,13 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
             return as_global(a.q) + (int64_t) (wk.tok0 + tok) * a.q_ldt + (int64_t) (wk.h * a.group + y - tok * a.group) * a.q_ldh;
         };
         u32x4 q[NQ][X::Q_LDS ? 1 : KC];
-        int rpos[NQ];
+        int upto[NQ], from[NQ];                         // the lane's row sees keys from < key <= upto
 #pragma unroll
         for (int i = 0; i < NQ; ++i) {
             const int x = wk.t * ROWS + 16 * i + c16;
-            rpos[i] = x < rows ? wk.pos0 + (int) a.d_group.div((uint32_t) x) : -1;  // a row past the tile's sees nothing
+            const int pos = x < rows ? wk.pos0 + (int) a.d_group.div((uint32_t) x) : -1;  // a row past the tile's sees nothing
+            upto[i] = min(pos, a.cap - 1);
+            from[i] = a.window ? pos - a.window : -1;
             if constexpr (!X::Q_LDS) {
                 auto* const src = q_at(16 * i + c16) + 8 * g4;
 #pragma unroll
@@ -294,9 +295,8 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
                         for (int e = 0; e < 4; ++e) {
                             float x = st[i][y][e] * a.scale;
                             if (!whole) {
-                                const int key = 32 * s + 16 * y + 4 * g4 + e;
-                                const bool seen = key <= rpos[i] && key < a.cap && (!a.window || key > rpos[i] - a.window) && (y ? p1 : p0) >= 0;
-                                x = seen ? x : -INFINITY;
+                                const int key = 32 * s + 16 * y + 4 * g4 + e, end = (y ? p1 : p0) >= 0 ? upto[i] : -1;
+                                x = ((key <= end) & (key > from[i])) ? x : -INFINITY;
                             }
                             st[i][y][e] = x;
                             mx = fmaxf(mx, x);
@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const int key = 32 * s + 16 * (i >> 2) + 4 * g4 + (i & 3);
-                        const bool live = key >= tile.lo && key < tile.hi && (i < 4 ? p0 : p1) >= 0;
+                        const bool live = (key >= tile.lo) & (key < ((i < 4 ? p0 : p1) >= 0 ? tile.hi : 0));
 #pragma unroll
                         for (int c = 0; c < VC; ++c)
 #pragma unroll
@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
                             uint32_t pw = j == 0 ? pb[i][0] : j == 1 ? pb[i][1] : j == 2 ? pb[i][2] : pb[i][3];
                             pw = (uint32_t) __shfl((int) pw, 16 * ((y >> 2) & 3) + c16);
                             const float p = (float) __builtin_bit_cast(T, (uint16_t) (y & 1 ? pw >> 16 : pw));
-                            const uint32_t seen = key <= rpos[i] && (!a.window || key > rpos[i] - a.window) ? 0xFFFFu : 0u;
+                            const uint32_t seen = ((key <= upto[i]) & (key > from[i])) ? 0xFFFFu : 0u;
 #pragma unroll
                             for (int u = 0; u < VC; ++u)
 #pragma unroll
@@ -394,13 +394,8 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
         // the waves' outputs joined: maxima and sums first, then 16 rows at a time
         const bool starts = off == 0, ends = off + n_steps == tile.steps, split = !(starts && ends);
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-            l[i] = sum_quads(l[i]);
-            if (g4 == 0) {
-                sh.m[wave][16 * i + c16] = m[i];
-                sh.l[wave][16 * i + c16] = l[i];
-            }
-        }
+        for (int i = 0; i < NQ; ++i)
+            if (g4 == 0) sh.m[wave][16 * i + c16] = m[i];
         __syncthreads();
         const int first_wg = wg - (int) (((uint32_t) off + per - 1u) / per);        // workgroups back to the tile's first step
         const uint32_t slot = 2u * (uint32_t) wg + (starts ? 1u : 0u);
@@ -416,8 +411,9 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
             float top = LOWEST;
 #pragma unroll
             for (int x = 0; x < WAVES; ++x) top = fmaxf(top, sh.m[x][16 * i + c16]);
-            const float c = exp2_fast(m[i] - top);
+            const float c = exp2_fast(m[i] - top), lt = sum_quads(l[i]) * c;
             if (i) __syncthreads();
+            if (g4 == 0) sh.l[wave][c16] = lt;
 #pragma unroll
             for (int u = 0; u < VC; ++u)
 #pragma unroll
@@ -427,25 +423,25 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
                         *reinterpret_cast<f32x4*>(&sh.o[wave][c16][16 * E * u + E * (4 * g4 + y) + e]) =
                             f32x4{o[i][u][e][y] * c, o[i][u][e + 1][y] * c, o[i][u][e + 2][y] * c, o[i][u][e + 3][y] * c};
             __syncthreads();
-            for (int z = tid; z < 16 * D / 4; z += X::THREADS) {
+            for (int z = tid; z < min(16, live_rows - 16 * i) * (D / 4); z += X::THREADS) {
                 const int x = z / (D / 4), col = 4 * (z % (D / 4));
-                if (16 * i + x >= live_rows) continue;
-                float mt = LOWEST, lt = 0.f;
+                float lx = 0.f;
                 f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int y = 0; y < WAVES; ++y) mt = fmaxf(mt, sh.m[y][16 * i + x]);
-#pragma unroll
+#pragma unroll 4
                 for (int y = 0; y < WAVES; ++y) {
-                    lt += sh.l[y][16 * i + x] * exp2_fast(sh.m[y][16 * i + x] - mt);
+                    lx += sh.l[y][x];
                     sum += *reinterpret_cast<const f32x4*>(&sh.o[y][x][col]);
                 }
                 if (!split) {
-                    store_out<T>(out_at(16 * i + x) + col, sum, lt);
+                    store_out<T>(out_at(16 * i + x) + col, sum, lx);
                 } else {
                     const uint32_t at = (slot * ATTN_SLOT + (uint32_t) (16 * i + x) * D + (uint32_t) col) * 4u;
                     __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum), prs, at, 0, SC1);
                     if (col == 0) {
-                        const u32x2 ml = u32x2{(uint32_t) __float_as_int(mt), (uint32_t) __float_as_int(lt)};
+                        float mx = LOWEST;
+#pragma unroll 4
+                        for (int y = 0; y < WAVES; ++y) mx = fmaxf(mx, sh.m[y][16 * i + x]);
+                        const u32x2 ml = u32x2{(uint32_t) __float_as_int(mx), (uint32_t) __float_as_int(lx)};
                         __builtin_amdgcn_raw_buffer_store_b64(ml, prs, (slot * ATTN_SLOT + (uint32_t) (ROWS * D + 2 * (16 * i + x))) * 4u, 0, SC1);
                     }
                 }
@@ -465,9 +461,10 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
             if (sh.last) join_parts<T, D, ROWS, X::THREADS>(prs, first_wg, last_wg, live_rows, out_at);
         }
         __syncthreads();
-        w += n_steps;
+        left -= n_steps;
+        if (left <= 0) break;
         off = 0;
-        if (w < w_end) wk.next();
+        wk.next();
     }
 }
 
@@ -482,9 +479,9 @@ void launch(const AttnArgs& a, int d, hipStream_t s)
 {
     // rows of an average request and kv head
     const int64_t rows = a.requests ? (int64_t) a.tokens * a.group / a.requests : 0;
-    if (d == 64) rows <= 16 ? launch_decode<T, 64, 1, 16>(a, s) : launch_decode<T, 64, 4, 8>(a, s);
-    else if (d == 128) rows <= 16 ? launch_decode<T, 128, 1, 12>(a, s) : launch_decode<T, 128, 2, 8>(a, s);
-    else rows <= 16 ? launch_decode<T, 256, 1, 8>(a, s) : launch_decode<T, 256, 2, 4>(a, s);
+    if (d == 64) rows <= 16 ? launch_decode<T, 64, 1, 8>(a, s) : launch_decode<T, 64, 4, 8>(a, s);
+    else if (d == 128) rows <= 16 ? launch_decode<T, 128, 1, 8>(a, s) : launch_decode<T, 128, 2, 8>(a, s);
+    else rows <= 16 ? launch_decode<T, 256, 1, 4>(a, s) : launch_decode<T, 256, 2, 4>(a, s);
 }
 
 }  // namespace
