@@ -18,7 +18,7 @@ OUT = os.path.join(HERE, "exl3rocm", "libexl3_mi355x.so")
 OUT_TIMELINE = os.path.join(HERE, "exl3rocm", "libexl3_mi355x_timeline.so")
 SOURCES = ["exl3_gemv.hip", "exl3_gemv_gated.hip", "exl3_gemv_silu.hip", "exl3_gemv_approx.hip", "exl3_gemv_f32.hip",
            "exl3_gemm.hip", "exl3_gemm_rd.hip", "exl3_had.hip", "exl3_noalloc.hip",
-           "exl3_paged.hip", "exl3_attn.hip"]
+           "exl3_paged.hip", "exl3_attn.hip", "exl3_attn_prefill.hip"]
 # Per-source extra flags.  The trellis decode (the GEMV's loop and the prefill producers') is long
 # chains of packed-math (VOP3P) ops whose results need extra wait states on gfx950; the ILP
 # scheduler interleaves the independent chains so the hazards are hidden instead of padded with

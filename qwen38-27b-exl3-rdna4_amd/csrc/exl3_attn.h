@@ -3,6 +3,7 @@
 #include "exl3_device.h"
 #include <algorithm>
 #include <initializer_list>
+#include <type_traits>
 
 namespace exl3 {
 
@@ -32,6 +33,24 @@ __device__ __forceinline__ uint64_t uniform(uint64_t x)
            (uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) (uint32_t) (x >> 32)) << 32;
 }
 
+typedef __attribute__((address_space(1))) const char gc_char;
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// 0xFFFF in each half of x that is an infinity or NaN: adding one to an exponent of all ones reaches the sign's place
+// (integer arithmetic: 64 compares at once would take the scalar registers of 64 results)
+template <class T>
+__device__ __forceinline__ uint32_t nonfinite2(uint32_t x)
+{
+    constexpr uint32_t ONE = std::is_same_v<T, f16> ? 0x04000400u : 0x00800080u;
+    const uint32_t n = ((x & 0x7FFF7FFFu) + ONE) & 0x80008000u;
+    return n | (n - (n >> 15));
+}
+
+constexpr float LOWEST = -3.0e38f;                      // a running maximum that no key has raised
+
+__device__ __forceinline__ u32x4 flipped(u32x4 x, uint32_t f) { return u32x4{x[0] ^ f, x[1] ^ f, x[2] ^ f, x[3] ^ f}; }
+
 // out = sum / l of four columns; a row that saw nothing (l = 0) is 0
 template <class T>
 __device__ __forceinline__ void store_out(__attribute__((address_space(1))) uint16_t* at, f32x4 sum, float l)
@@ -49,14 +68,17 @@ struct AttnArgs {
     uint16_t* out;
     int tokens, requests, group, hkv, pages, page, window;
     int cap;                                            // positions that a row of the table holds
-    float scale;                                        // times log2(e)
+    float scale;                                        // its size times log2(e): above 0
+    uint32_t flip;                                      // sign bits of two halves of q: 0 but for a negative scale
     UDiv d_page, d_group;
     uint32_t* counters;                                 // one per workgroup, zero between calls
     float* part;                                        // partial tiles: two a workgroup
 };
 
-constexpr int ATTN_GRID = 256;                          // workgroups: one per CU
-constexpr int ATTN_SLOT = 8256;                         // floats of a partial tile: rows x D outputs, then (max, sum) a row
+// a partial tile, floats: rows x D outputs, then (maximum, sum) a row; two for each workgroup of a grid
+constexpr int attn_slot(int rows, int d) { return rows * (d + 2); }
+constexpr int ATTN_COUNTERS = EXL3_ATTN_COUNTER_BYTES / 4;                      // the largest grid
+constexpr size_t ATTN_PART_BYTES = (size_t) 2 * 512 * attn_slot(128, 128) * 4;  // the largest grid times slot (all kernels assert it)
 
 // A request's new rows for one kv head, (token, head of the group) in token order, are cut into tiles of `rows`; a tile
 // reads the keys that any of its rows sees, in steps of KEYS.  A launch's work is the steps of every (kv head,
@@ -68,7 +90,7 @@ struct AttnTile {
     int step0, steps;                                   // its steps; one (of no key) where no row sees any
 };
 
-template <int ROWS, int KEYS>
+template <int ROWS, int KEYS, int GRID>
 struct AttnWork {
     const AttnArgs& a;
     int r, t, h;                                        // request, tile, kv head
@@ -127,7 +149,7 @@ struct AttnWork {
             sums += lds[i];
         }
         const uint64_t total = uniform(sums), all = total * (uint64_t) a.hkv;
-        const uint64_t share = max((all + ATTN_GRID - 1) / ATTN_GRID, (uint64_t) least);
+        const uint64_t share = max((all + GRID - 1) / GRID, (uint64_t) least);
         uint64_t u = (uint64_t) wg * share;
         if (u >= all) return false;
         per = (uint32_t) min(share, (uint64_t) 1 << 30);
@@ -189,5 +211,46 @@ struct AttnWork {
         tile = tile_of(0);
     }
 };
+
+// A split tile's parts, summed in the order of their workgroups: part c of workgroup c lies in slot 2 c, the first
+// one's in 2 c + 1; B of them are in flight.
+template <class T, int D, int ROWS, int THREADS, int SLOT, int B, class At>
+__device__ __forceinline__ void join_parts(__amdgpu_buffer_rsrc_t prs, int first, int last, int rows, At&& out_at)
+{
+    auto slot = [&](int c) __attribute__((always_inline)) { return (uint32_t) (2 * c + (c == first ? 1 : 0)) * (uint32_t) SLOT; };
+    for (int z = threadIdx.x; z < rows * (D / 4); z += THREADS) {
+        const int x = z / (D / 4), col = 4 * (z % (D / 4));
+        const uint32_t at = (uint32_t) (x * D + col), ml = (uint32_t) (ROWS * D + 2 * x);
+        float m = LOWEST, l = 0.f;
+        f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int c0 = first; c0 <= last; c0 += B) {
+            u32x2 mls[B];
+            f32x4 v[B];
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                const uint32_t s = slot(min(c0 + i, last));
+                mls[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(prs, (s + ml) * 4u, 0, SC1));
+                v[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(prs, (s + at) * 4u, 0, SC1));
+            }
+            float top = m;
+#pragma unroll
+            for (int i = 0; i < B; ++i) top = fmaxf(top, __int_as_float((int) mls[i][0]));
+            const float c = exp2_fast(m - top);
+            l *= c;
+            sum *= c;
+            m = top;
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                const float f = c0 + i <= last ? exp2_fast(__int_as_float((int) mls[i][0]) - m) : 0.f;
+                l += f * __int_as_float((int) mls[i][1]);
+                sum += v[i] * f;
+            }
+        }
+        store_out<T>(out_at(x) + col, sum, l);
+    }
+}
+
+// many rows a request (exl3_attn_prefill.hip)
+void launch_attn_prefill(const AttnArgs& a, int dtype, int head_dim, hipStream_t s);
 
 }  // namespace exl3

@@ -1,13 +1,11 @@
 // exl3_attn.hip -- causal attention of each request's new tokens over its paged key/value cache: the entry point, and
 // the kernel for few rows per request (decodes and drafts).
 #include "exl3_attn.h"
-#include <type_traits>
+#include <cmath>
 
 using namespace exl3;
 
 namespace {
-
-typedef __attribute__((address_space(1))) const char gc_char;
 
 template <class T> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c);
 template <> __device__ __forceinline__ f32x4 mfma16<f16>(u32x4 a, u32x4 b, f32x4 c)
@@ -37,23 +35,9 @@ __device__ __forceinline__ float sum_quads(float x)
     return __int_as_float((int) w[0]) + __int_as_float((int) w[1]);
 }
 
-__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// 0xFFFF in each half of x that is an infinity or NaN: adding one to an exponent of all ones reaches the sign's place
-// (integer arithmetic: 64 compares at once would take the scalar registers of 64 results)
-template <class T>
-__device__ __forceinline__ uint32_t nonfinite2(uint32_t x)
-{
-    constexpr uint32_t ONE = std::is_same_v<T, f16> ? 0x04000400u : 0x00800080u;
-    const uint32_t n = ((x & 0x7FFF7FFFu) + ONE) & 0x80008000u;
-    return n | (n - (n >> 15));
-}
-
 template <int N> struct Words;
 template <> struct Words<4> { typedef u32x4 T; typedef gc_u32x4 G; };
 template <> struct Words<2> { typedef u32x2 T; typedef gc_u32x2 G; };
-
-constexpr float LOWEST = -3.0e38f;                      // a running maximum that no key has raised
 
 // ---- few rows: 16 NQ rows a tile, bound by the reading of K and V --------------------------------------------
 // Every wave takes whole steps of 32 keys of its tile, with a softmax of its own (running maximum, sum, output), and
@@ -76,7 +60,9 @@ struct Decode {
     static constexpr int PAD = D + 4;                   // LDS row (floats) of the waves' outputs
     static constexpr bool Q_LDS = NQ * KC > 4;          // Q would take more than 16 registers: read from LDS at each step
     static constexpr int Q_PAD = D + 8;                 // its LDS row (halves)
-    static_assert(ROWS * D + 2 * ROWS <= ATTN_SLOT);
+    static constexpr int GRID = 256;                    // workgroups: one a CU
+    static constexpr int SLOT = attn_slot(ROWS, D);
+    static_assert(GRID <= ATTN_COUNTERS && (size_t) 2 * GRID * SLOT * 4 <= ATTN_PART_BYTES);
     // fp16 probabilities are held times 2^8: the smallest that a key keeps is then 2^-33 of its row's largest
     static constexpr float SHIFT = std::is_same_v<T, f16> ? 8.f : 0.f;
     using V = typename Words<VW / 4>::T;
@@ -102,45 +88,6 @@ struct Decode {
     }
 };
 
-// A split tile's parts, summed in the order of their workgroups: part c of workgroup c lies in slot 2 c, the first
-// one's in 2 c + 1.
-template <class T, int D, int ROWS, int THREADS, class At>
-__device__ __forceinline__ void join_parts(__amdgpu_buffer_rsrc_t prs, int first, int last, int rows, At&& out_at)
-{
-    auto slot = [&](int c) __attribute__((always_inline)) { return (uint32_t) (2 * c + (c == first ? 1 : 0)) * (uint32_t) ATTN_SLOT; };
-    for (int z = threadIdx.x; z < rows * (D / 4); z += THREADS) {
-        const int x = z / (D / 4), col = 4 * (z % (D / 4));
-        const uint32_t at = (uint32_t) (x * D + col), ml = (uint32_t) (ROWS * D + 2 * x);
-        float m = LOWEST, l = 0.f;
-        f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
-        constexpr int B = 8;
-        for (int c0 = first; c0 <= last; c0 += B) {
-            u32x2 mls[B];
-            f32x4 v[B];
-#pragma unroll
-            for (int i = 0; i < B; ++i) {
-                const uint32_t s = slot(min(c0 + i, last));
-                mls[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(prs, (s + ml) * 4u, 0, SC1));
-                v[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(prs, (s + at) * 4u, 0, SC1));
-            }
-            float top = m;
-#pragma unroll
-            for (int i = 0; i < B; ++i) top = fmaxf(top, __int_as_float((int) mls[i][0]));
-            const float c = exp2_fast(m - top);
-            l *= c;
-            sum *= c;
-            m = top;
-#pragma unroll
-            for (int i = 0; i < B; ++i) {
-                const float f = c0 + i <= last ? exp2_fast(__int_as_float((int) mls[i][0]) - m) : 0.f;
-                l += f * __int_as_float((int) mls[i][1]);
-                sum += v[i] * f;
-            }
-        }
-        store_out<T>(out_at(x) + col, sum, l);
-    }
-}
-
 template <class T, int D, int NQ, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
 {
@@ -152,11 +99,11 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
 
     // rows of no request
     const int used = a.requests ? min(max(a.cu_q[a.requests], 0), a.tokens) : 0;
-    for (int t = used + wg; t < a.tokens; t += ATTN_GRID)
+    for (int t = used + wg; t < a.tokens; t += X::GRID)
         for (int i = tid; i < a.group * a.hkv * (D / 8); i += X::THREADS)
             *reinterpret_cast<g_u32x4*>(as_global(a.out) + (int64_t) t * a.o_ldt + (i / (D / 8)) * a.o_ldh + 8 * (i % (D / 8))) = u32x4{0u, 0u, 0u, 0u};
 
-    AttnWork<ROWS, 32> wk(a);
+    AttnWork<ROWS, 32, X::GRID> wk(a);
     int64_t left;
     int off;
     uint32_t per;
@@ -192,12 +139,13 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
             if constexpr (!X::Q_LDS) {
                 auto* const src = q_at(16 * i + c16) + 8 * g4;
 #pragma unroll
-                for (int c = 0; c < KC; ++c) q[i][c] = *reinterpret_cast<gc_u32x4*>(src + 32 * c);
+                for (int c = 0; c < KC; ++c) q[i][c] = flipped(*reinterpret_cast<gc_u32x4*>(src + 32 * c), a.flip);
             }
         }
         if constexpr (X::Q_LDS) {
             for (int z = tid; z < ROWS * D / 8; z += X::THREADS)
-                *reinterpret_cast<u32x4*>(&sh.q[z / (D / 8)][8 * (z % (D / 8))]) = *reinterpret_cast<gc_u32x4*>(q_at(z / (D / 8)) + 8 * (z % (D / 8)));
+                *reinterpret_cast<u32x4*>(&sh.q[z / (D / 8)][8 * (z % (D / 8))]) =
+                    flipped(*reinterpret_cast<gc_u32x4*>(q_at(z / (D / 8)) + 8 * (z % (D / 8))), a.flip);
             __syncthreads();
         }
         f32x4 o[NQ][VC][E];
@@ -399,7 +347,7 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
         __syncthreads();
         const int first_wg = wg - (int) (((uint32_t) off + per - 1u) / per);        // workgroups back to the tile's first step
         const uint32_t slot = 2u * (uint32_t) wg + (starts ? 1u : 0u);
-        const __amdgpu_buffer_rsrc_t prs = __builtin_amdgcn_make_buffer_rsrc(a.part, 0, 2 * ATTN_GRID * ATTN_SLOT * 4, RAW_BUFFER_FLAGS);
+        const __amdgpu_buffer_rsrc_t prs = __builtin_amdgcn_make_buffer_rsrc(a.part, 0, (int) ATTN_PART_BYTES, RAW_BUFFER_FLAGS);
         auto out_at = [&](int x) __attribute__((always_inline)) {                  // row x of the tile
             const int y = wk.t * ROWS + x, tok = (int) a.d_group.div((uint32_t) y);
             return as_global(a.out) + (int64_t) (wk.tok0 + tok) * a.o_ldt + (int64_t) (wk.h * a.group + y - tok * a.group) * a.o_ldh;
@@ -435,14 +383,14 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
                 if (!split) {
                     store_out<T>(out_at(16 * i + x) + col, sum, lx);
                 } else {
-                    const uint32_t at = (slot * ATTN_SLOT + (uint32_t) (16 * i + x) * D + (uint32_t) col) * 4u;
+                    const uint32_t at = (slot * X::SLOT + (uint32_t) (16 * i + x) * D + (uint32_t) col) * 4u;
                     __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum), prs, at, 0, SC1);
                     if (col == 0) {
                         float mx = LOWEST;
 #pragma unroll 4
                         for (int y = 0; y < WAVES; ++y) mx = fmaxf(mx, sh.m[y][16 * i + x]);
                         const u32x2 ml = u32x2{(uint32_t) __float_as_int(mx), (uint32_t) __float_as_int(lx)};
-                        __builtin_amdgcn_raw_buffer_store_b64(ml, prs, (slot * ATTN_SLOT + (uint32_t) (ROWS * D + 2 * (16 * i + x))) * 4u, 0, SC1);
+                        __builtin_amdgcn_raw_buffer_store_b64(ml, prs, (slot * X::SLOT + (uint32_t) (ROWS * D + 2 * (16 * i + x))) * 4u, 0, SC1);
                     }
                 }
             }
@@ -458,7 +406,7 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
                 if (sh.last) __hip_atomic_store(&a.counters[first_wg], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
             __syncthreads();
-            if (sh.last) join_parts<T, D, ROWS, X::THREADS>(prs, first_wg, last_wg, live_rows, out_at);
+            if (sh.last) join_parts<T, D, ROWS, X::THREADS, X::SLOT, 8>(prs, first_wg, last_wg, live_rows, out_at);
         }
         __syncthreads();
         left -= n_steps;
@@ -471,7 +419,7 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
 template <class T, int D, int NQ, int WAVES>
 void launch_decode(const AttnArgs& a, hipStream_t s)
 {
-    hipLaunchKernelGGL((attn_decode_kernel<T, D, NQ, WAVES>), dim3(ATTN_GRID), dim3(64 * WAVES), 0, s, a);
+    hipLaunchKernelGGL((attn_decode_kernel<T, D, NQ, WAVES>), dim3(Decode<T, D, NQ, WAVES>::GRID), dim3(64 * WAVES), 0, s, a);
 }
 
 template <class T>
@@ -488,7 +436,7 @@ void launch(const AttnArgs& a, int d, hipStream_t s)
 
 extern "C" size_t exl3_paged_attention_workspace_size(void)
 {
-    return EXL3_ATTN_COUNTER_BYTES + (size_t) 2 * ATTN_GRID * ATTN_SLOT * 4;
+    return EXL3_ATTN_COUNTER_BYTES + (size_t) (int) ATTN_PART_BYTES;
 }
 
 extern "C" int exl3_paged_attention(const void* q, int64_t q_ldt, int64_t q_ldh, const void* k_cache, int64_t k_ldp, int64_t k_ldt,
@@ -514,10 +462,12 @@ extern "C" int exl3_paged_attention(const void* q, int64_t q_ldt, int64_t q_ldh,
     if (!workspace || ((uintptr_t) workspace & 15u) || ws_bytes < exl3_paged_attention_workspace_size()) return EXL3_EWORKSPACE;
     AttnArgs a{(const uint16_t*) q, (const uint16_t*) k_cache, (const uint16_t*) v_cache, q_ldt, q_ldh, k_ldp, k_ldt, k_ldh, v_ldp, v_ldt,
                v_ldh, o_ldt, o_ldh, ld_table, block_table, cu_q, seq_lens, (uint16_t*) out, tokens, requests, q_heads / kv_heads, kv_heads,
-               pages, page_size, window, pages ? table_cols * page_size : 0, scale * 1.44269504f, UDiv::of((uint32_t) page_size),
+               pages, page_size, window, pages ? table_cols * page_size : 0, std::max(std::fabs(scale) * 1.44269504f, 1e-30f), scale < 0.f ? 0x80008000u : 0u, UDiv::of((uint32_t) page_size),
                UDiv::of((uint32_t) (q_heads / kv_heads)), (uint32_t*) workspace,
                reinterpret_cast<float*>((char*) workspace + EXL3_ATTN_COUNTER_BYTES)};
-    if (dtype == EXL3_FP16) launch<f16>(a, head_dim, (hipStream_t) stream);
+    // rows of an average request and kv head: from 64 on the products with K and V are what bounds them
+    if (requests && (int64_t) tokens * a.group / requests >= 64) launch_attn_prefill(a, dtype, head_dim, (hipStream_t) stream);
+    else if (dtype == EXL3_FP16) launch<f16>(a, head_dim, (hipStream_t) stream);
     else launch<__bf16>(a, head_dim, (hipStream_t) stream);
     return hipGetLastError() == hipSuccess ? EXL3_OK : EXL3_ELAUNCH;
 }

@@ -1,0 +1,346 @@
+// exl3_attn_prefill.hip -- paged attention for many rows a request (prompt chunks), bound by the matrix products.
+#include "exl3_attn.h"
+
+using namespace exl3;
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <class T> __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c);
+template <> __device__ __forceinline__ f32x16 mfma32<f16>(u32x4 a, u32x4 b, f32x16 c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f32x16 mfma32<__bf16>(u32x4 a, u32x4 b, f32x16 c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// 128 rows a tile, 32 a wave, 64 keys a step.  K and V go through LDS once for the four waves: wave w requests keys
+// 16 w .. + 15 of step s + 2 (one page: page sizes are multiples of 16) while step s is computed, and stores those of
+// s + 1 into the other buffer after it, so a step has one barrier.
+//   S^T = K Q^T (32x32x16): lane l gives key l & 31, elements 16 c + 8 (l >> 5) ..; its result holds row l & 31,
+//         keys 8 (i >> 2) + 4 (l >> 5) + (i & 3)
+//   O^T = V^T P^T: results 8 b .. 8 b + 7 are operand elements of 16 keys as they lie; V^T's lane gets the same keys by
+//         transposing LDS reads (16 lanes read 4 keys x 16 columns, lane i gets column i of the 4)
+// A lane's row is the same in S^T and O^T, as in the decode kernel.  A row of LDS (2 D bytes) keeps its 16-byte pieces
+// in an order of its own, K's so that 16 keys' reads of one piece meet no bank twice, V's so that 8 keys' 64 bytes do not.
+template <class T, int D>
+struct Prefill {
+    static constexpr int ROWS = 128, KEYS = 64, WAVES = 4, THREADS = 256;
+    static constexpr int GRID = D == 256 ? 256 : 512;   // workgroups: one or two a CU
+    static constexpr int SLOT = attn_slot(ROWS, D);
+    static_assert(GRID <= ATTN_COUNTERS && (size_t) 2 * GRID * SLOT * 4 <= ATTN_PART_BYTES);
+    static constexpr int LEAST = 4;                     // steps of a share at least
+    static constexpr int CH = D / 8;                    // 16-byte pieces of a row
+    static constexpr int LI = D / 32;                   // ... of a wave's 16 keys that a lane moves
+    static constexpr int KS = D / 16;                   // products over D
+    static constexpr int DT = D / 32;                   // column tiles of the output
+    static constexpr float SHIFT = std::is_same_v<T, f16> ? 8.f : 0.f;   // fp16 probabilities are held times 2^8
+
+    struct Shared {
+        uint16_t k[2][KEYS * D], v[2][KEYS * D];
+        uint64_t find[WAVES + 4];
+        int page[2][WAVES];                             // of a wave's 16 keys: 1 its page is one, 2 zeroed elements are to be added
+        int last;
+    };
+    static __device__ __forceinline__ int k_piece(int key, int piece) { return piece ^ (D == 64 ? (key >> 1) & 7 : key & 15); }
+    static __device__ __forceinline__ int v_piece(int key, int piece) { return piece ^ (D == 64 ? ((key >> 1) & 1) << 2 : (key & 3) << 2); }
+};
+
+template <class T, int D>
+__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_prefill_kernel(AttnArgs a)
+{
+    using X = Prefill<T, D>;
+    constexpr int LI = X::LI, KS = X::KS, DT = X::DT, CH = X::CH;
+    __shared__ typename X::Shared sh;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c32 = lane & 31, h2 = lane >> 5;
+    // consecutive shares to one XCD (workgroups go round the 8 XCDs): they read the same head's K and V
+    const int wg = (int) (blockIdx.x % 8) * (X::GRID / 8) + (int) blockIdx.x / 8;
+
+    const int used = a.requests ? min(max(a.cu_q[a.requests], 0), a.tokens) : 0;
+    for (int t = used + wg; t < a.tokens; t += X::GRID)    // rows of no request
+        for (int i = tid; i < a.group * a.hkv * (D / 8); i += X::THREADS)
+            *reinterpret_cast<g_u32x4*>(as_global(a.out) + (int64_t) t * a.o_ldt + (i / (D / 8)) * a.o_ldh + 8 * (i % (D / 8))) = u32x4{0u, 0u, 0u, 0u};
+
+    AttnWork<X::ROWS, X::KEYS, X::GRID> wk(a);
+    int64_t left;
+    int off;
+    uint32_t per;
+    if (!wk.template find<X::THREADS>(wg, X::LEAST, sh.find, off, left, per)) return;
+
+    // the lane's place in its wave's 16 keys: row st_row + 64 / CH i, piece st_piece
+    const int st_row = lane / CH, st_piece = lane % CH;
+    // transposing reads: key 4 h2 + tr_row of 8, columns 32 dt + 16 tr_half + 4 tr_q ..
+    const int s16 = lane & 15, tr_row = s16 >> 2, tr_q = s16 & 3, tr_half = (lane >> 4) & 1;
+
+    while (true) {
+        const AttnTile tile = wk.tile;
+        const int n_steps = (int) min((int64_t) (tile.steps - off), left);
+        const int s0 = tile.step0 + off, s1 = s0 + n_steps, rows = wk.n * a.group;
+        const int* const table = a.table + (int64_t) wk.r * a.ld_table;
+        const char* const kh = reinterpret_cast<const char*>(a.k + (int64_t) wk.h * a.k_ldh);
+        const char* const vh = reinterpret_cast<const char*>(a.v + (int64_t) wk.h * a.v_ldh);
+
+        const int x0 = wk.t * X::ROWS + 32 * wave;      // the wave's first row
+        const bool rows_here = x0 < rows;
+        const int w_first = wk.pos0 + (int) a.d_group.div((uint32_t) x0), w_last = wk.pos0 + (int) a.d_group.div((uint32_t) (min(x0 + 32, rows) - 1));
+        const int xl = x0 + c32, tok = (int) a.d_group.div((uint32_t) min(xl, rows - 1)), pos = xl < rows ? wk.pos0 + tok : -1;
+        const int upto = min(pos, a.cap - 1), from = a.window ? pos - a.window : -1;
+        u32x4 q[KS];
+        {
+            gc_u16* const src = as_global(a.q) + (int64_t) (wk.tok0 + tok) * a.q_ldt + (int64_t) (wk.h * a.group + min(xl, rows - 1) - tok * a.group) * a.q_ldh + 8 * h2;
+#pragma unroll
+            for (int c = 0; c < KS; ++c) q[c] = flipped(*reinterpret_cast<gc_u32x4*>(src + 16 * c), a.flip);
+        }
+        f32x16 o[DT];
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+        float m = LOWEST, l = 0.f;
+
+        auto page_of = [&](int s) __attribute__((always_inline)) {
+            const int key = X::KEYS * s + 16 * wave;
+            int p = -1;
+            if (key < tile.hi) {
+                p = table[a.d_page.div((uint32_t) key)];
+                if ((unsigned) p >= (unsigned) a.pages) p = -1;
+            }
+            return p;
+        };
+        auto keys_at = [&](const char* base, int64_t ldp, int64_t ldt, int p, int key) __attribute__((always_inline)) {
+            const int in = key - (int) a.d_page.div((uint32_t) key) * a.page;
+            return as_global(base) + ((int64_t) max(p, 0) * ldp + (int64_t) in * ldt) * 2;
+        };
+        u32x4 kr[LI], vr[LI];
+        auto request = [&](int s, int p) __attribute__((always_inline)) {
+            gc_char* const kp = keys_at(kh, a.k_ldp, a.k_ldt, p, X::KEYS * s + 16 * wave);
+            gc_char* const vp = keys_at(vh, a.v_ldp, a.v_ldt, p, X::KEYS * s + 16 * wave);
+#pragma unroll
+            for (int i = 0; i < LI; ++i) {
+                const int row = st_row + 64 / CH * i;
+                kr[i] = *reinterpret_cast<gc_u32x4*>(kp + (uint32_t) (row * (int) a.k_ldt + 8 * st_piece) * 2u);
+                vr[i] = *reinterpret_cast<gc_u32x4*>(vp + (uint32_t) (row * (int) a.v_ldt + 8 * st_piece) * 2u);
+            }
+        };
+        auto store = [&](int buf, int s, int p) __attribute__((always_inline)) {
+            const int key0 = X::KEYS * s + 16 * wave;
+            // whether every row of the tile sees these keys; if not, V of keys that no row sees may hold anything and is
+            // zeroed, and so are infinities and NaN, which a probability of 0 does not hide from the rows that do not see them
+            const bool seen = p >= 0 && key0 + 15 <= wk.pos0 + tile.first && (!a.window || key0 > wk.pos0 + tile.last - a.window) && key0 + 16 <= a.cap;
+            int flags = p >= 0 ? 1 : 0;
+            if (!seen) {
+                uint32_t f = 0;
+#pragma unroll
+                for (int i = 0; i < LI; ++i) {
+                    const int key = key0 + st_row + 64 / CH * i;
+                    const bool live = (key >= tile.lo) & (key < (p >= 0 ? tile.hi : 0));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t x = live ? vr[i][e] : 0u, n = nonfinite2<T>(x);
+                        f |= n;
+                        vr[i][e] = x & ~n;
+                    }
+                }
+                if (__any(f != 0u)) flags |= 2;
+            }
+#pragma unroll
+            for (int i = 0; i < LI; ++i) {
+                const int key = 16 * wave + st_row + 64 / CH * i;
+                *reinterpret_cast<u32x4*>(&sh.k[buf][key * D + 8 * X::k_piece(key, st_piece)]) = kr[i];
+                *reinterpret_cast<u32x4*>(&sh.v[buf][key * D + 8 * X::v_piece(key, st_piece)]) = vr[i];
+            }
+            if (lane == 0) sh.page[buf][wave] = flags;
+        };
+        auto compute = [&](int buf, int s) __attribute__((always_inline)) {
+            const int k0 = X::KEYS * s;
+            // nothing for this wave's rows in the step
+            if (!rows_here || k0 > w_last || (a.window && k0 + X::KEYS - 1 <= w_first - a.window)) return;
+            const int fl0 = __builtin_amdgcn_readfirstlane(sh.page[buf][0]), fl1 = __builtin_amdgcn_readfirstlane(sh.page[buf][1]),
+                      fl2 = __builtin_amdgcn_readfirstlane(sh.page[buf][2]), fl3 = __builtin_amdgcn_readfirstlane(sh.page[buf][3]);
+            const bool whole = (fl0 & fl1 & fl2 & fl3 & 1) && k0 + X::KEYS - 1 <= w_first && (!a.window || k0 > w_last - a.window) && k0 + X::KEYS <= a.cap;
+            f32x16 st[2];
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) st[y][i] = 0.f;
+#pragma unroll
+            for (int c = 0; c < KS; ++c)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const u32x4 kf = *reinterpret_cast<const u32x4*>(&sh.k[buf][(32 * y + c32) * D + 8 * X::k_piece(c32, 2 * c + h2)]);
+                    st[y] = mfma32<T>(kf, q[c], st[y]);
+                }
+            if (!whole) {
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int key = k0 + 32 * y + 8 * (i >> 2) + 4 * h2 + (i & 3);
+                        const int end = ((y ? (i < 8 ? fl2 : fl3) : (i < 8 ? fl0 : fl1)) & 1) ? upto : -1;
+                        st[y][i] = ((key <= end) & (key > from)) ? st[y][i] : -INFINITY;
+                    }
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[y][i]);
+            float lo, hi;
+            halves_x(mx, lo, hi);
+            mx = fmaxf(m, fmaxf(lo, hi) * a.scale);     // a.scale > 0
+            if (__any(mx > m)) {
+                const float c = exp2_fast(m - mx);
+                l *= c;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[d] *= c;
+                m = mx;
+            }
+            const float base = X::SHIFT - m;
+            u32x4 pb[2][2];
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    typename Elem<T>::x8 p;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float x = exp2_fast(fmaf(st[y][8 * b + j], a.scale, base));
+                        l += x;
+                        p[j] = (T) x;
+                    }
+                    pb[y][b] = __builtin_bit_cast(u32x4, p);
+                }
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        u32x4 vf;
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const int key = 32 * y + 16 * b + 8 * x + 4 * h2 + tr_row;
+                            const s16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) (
+                                &sh.v[buf][key * D + 8 * X::v_piece(tr_row, 4 * d + 2 * tr_half + (tr_q >> 1)) + 4 * (tr_q & 1)]));
+                            const u32x2 w = __builtin_bit_cast(u32x2, r);
+                            vf[2 * x] = w[0];
+                            vf[2 * x + 1] = w[1];
+                        }
+                        o[d] = mfma32<T>(vf, pb[y][b], o[d]);
+                    }
+            if ((fl0 | fl1 | fl2 | fl3) & 2) {
+                // the infinities and NaN that were zeroed, added to the rows that see them
+#pragma unroll 1
+                for (int z = 0; z < X::KEYS; ++z) {
+                    const int key = k0 + z, fl = z < 16 ? fl0 : z < 32 ? fl1 : z < 48 ? fl2 : fl3;
+                    if (fl != 3 || key < tile.lo || key >= tile.hi) continue;
+                    const int p = table[a.d_page.div((uint32_t) key)], in = key - (int) a.d_page.div((uint32_t) key) * a.page;
+                    gc_u16* const vk = reinterpret_cast<gc_u16*>(as_global(vh) + ((int64_t) p * a.v_ldp + (int64_t) in * a.v_ldt) * 2);
+                    const int reg = 4 * (z >> 3) + (z & 3);                    // of 32: y, then i
+                    uint32_t pw = 0;
+#pragma unroll
+                    for (int y = 0; y < 16; ++y) pw = reg >> 1 == y ? pb[y >> 3][(y >> 2) & 1][y & 3] : pw;
+                    pw = (uint32_t) __shfl((int) pw, 32 * ((z >> 2) & 1) + c32);
+                    const float pr = (float) __builtin_bit_cast(T, (uint16_t) (reg & 1 ? pw >> 16 : pw));
+                    const uint32_t mask = ((key <= upto) & (key > from)) ? 0xFFFFu : 0u;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const uint32_t b = vk[32 * d + 8 * (i >> 2) + 4 * h2 + (i & 3)];
+                            o[d][i] += pr * (float) __builtin_bit_cast(T, (uint16_t) (b & mask & nonfinite2<T>(b)));
+                        }
+                }
+            }
+        };
+
+        if (tile.lo < tile.hi) {
+            int p0 = page_of(s0), p1 = page_of(s0 + 1), p2 = page_of(s0 + 2);
+            request(s0, p0);
+            store(0, s0, p0);
+            if (s0 + 1 < s1) request(s0 + 1, p1);
+            __syncthreads();
+            int buf = 0;
+            for (int s = s0;; ++s) {
+                compute(buf, s);
+                if (s + 1 == s1) break;
+                buf ^= 1;
+                store(buf, s + 1, p1);
+                p1 = p2;
+                p2 = page_of(s + 3);
+                if (s + 2 < s1) request(s + 2, p1);
+                __syncthreads();
+            }
+        }
+
+        // a wave's 32 rows, or their part
+        const bool starts = off == 0, ends = off + n_steps == tile.steps, split = !(starts && ends);
+        float lo, hi;
+        halves_x(l, lo, hi);
+        l = lo + hi;
+        const __amdgpu_buffer_rsrc_t prs = __builtin_amdgcn_make_buffer_rsrc(a.part, 0, (int) ATTN_PART_BYTES, RAW_BUFFER_FLAGS);
+        auto out_at = [&](int x) __attribute__((always_inline)) {                  // row x of the tile
+            const int y = wk.t * X::ROWS + x, tk = (int) a.d_group.div((uint32_t) y);
+            return as_global(a.out) + (int64_t) (wk.tok0 + tk) * a.o_ldt + (int64_t) (wk.h * a.group + y - tk * a.group) * a.o_ldh;
+        };
+        const uint32_t slot = (2u * (uint32_t) wg + (starts ? 1u : 0u)) * (uint32_t) X::SLOT;
+        if (xl < rows) {
+            const int x = 32 * wave + c32;
+            auto* const dst = out_at(x) + 4 * h2;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 v = f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+                    if (!split) store_out<T>(dst + 32 * d + 8 * i, v, l);
+                    else
+                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), prs, (slot + (uint32_t) (x * D + 32 * d + 8 * i + 4 * h2)) * 4u, 0, SC1);
+                }
+            if (split && h2 == 0) {
+                const u32x2 ml = u32x2{(uint32_t) __float_as_int(m), (uint32_t) __float_as_int(l)};
+                __builtin_amdgcn_raw_buffer_store_b64(ml, prs, (slot + (uint32_t) (X::ROWS * D + 2 * x)) * 4u, 0, SC1);
+            }
+        }
+        if (split) {
+            const int first_wg = wg - (int) (((uint32_t) off + per - 1u) / per);
+            const int last_wg = wg + (int) (((uint32_t) (tile.steps - off - n_steps) + per - 1u) / per);
+            __builtin_amdgcn_s_waitcnt(0x0F70);        // vmcnt(0): the part has landed
+            __syncthreads();
+            if (tid == 0) {
+                const uint32_t before = __hip_atomic_fetch_add(&a.counters[first_wg], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                sh.last = before == (uint32_t) (last_wg - first_wg);
+                if (sh.last) __hip_atomic_store(&a.counters[first_wg], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            __syncthreads();
+            if (sh.last) join_parts<T, D, X::ROWS, X::THREADS, X::SLOT, 4>(prs, first_wg, last_wg, min(X::ROWS, rows - wk.t * X::ROWS), out_at);
+        }
+        __syncthreads();
+        left -= n_steps;
+        if (left <= 0) break;
+        off = 0;
+        wk.next();
+    }
+}
+
+template <class T>
+void launch(const AttnArgs& a, int d, hipStream_t s)
+{
+    if (d == 64) hipLaunchKernelGGL((attn_prefill_kernel<T, 64>), dim3(Prefill<T, 64>::GRID), dim3(256), 0, s, a);
+    else if (d == 128) hipLaunchKernelGGL((attn_prefill_kernel<T, 128>), dim3(Prefill<T, 128>::GRID), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attn_prefill_kernel<T, 256>), dim3(Prefill<T, 256>::GRID), dim3(256), 0, s, a);
+}
+
+}  // namespace
+
+namespace exl3 {
+
+void launch_attn_prefill(const AttnArgs& a, int dtype, int head_dim, hipStream_t s)
+{
+    dtype == EXL3_FP16 ? launch<f16>(a, head_dim, s) : launch<__bf16>(a, head_dim, s);
+}
+
+}  // namespace exl3

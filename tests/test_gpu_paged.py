@@ -272,7 +272,7 @@ class Batch:
                     p, j = c + torch.arange(n, device="cuda")[:, None], torch.arange(c + n, device="cuda")
                     off = (j > p) | ((j <= p - window) if window else (j < 0))
                     w = torch.softmax(s.masked_fill(off, -math.inf), -1)
-                    size = (q[:, h].abs() @ k.abs().T * self.scale).masked_fill(off, 0).amax(-1, keepdim=True)
+                    size = (q[:, h].abs() @ k.abs().T * abs(self.scale)).masked_fill(off, 0).amax(-1, keepdim=True)
                     o = w @ v
                     out[t0:t0 + n, h] = o
                     bound[t0:t0 + n, h] += (u * o.abs() + (u + 2.0 ** -23 * self.d * size + 2.0 ** -18) * (w @ v.abs())
@@ -357,6 +357,14 @@ def test_large_scores():
     """Scores of hundreds: the running maximum carries them; keys far below it vanish."""
     Batch([(1000, 1), (700, 3), (0, 200)], 10, 2, 128, F16, q_scale=60.0).check()
     Batch([(1000, 1), (700, 3), (0, 200)], 10, 2, 128, BF16, q_scale=300.0).check()
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-3, 2.0])
+def test_scales(scale):
+    for lens in ([(300, 1), (20, 3)], [(50, 200)]):
+        b = Batch(lens, 6, 2, 64, F16)
+        b.scale = scale
+        b.check()
 
 
 def test_rows_that_see_nothing():
