@@ -25,8 +25,10 @@ template <> __device__ __forceinline__ f32x16 mfma32<__bf16>(u32x4 a, u32x4 b, f
 //         keys 8 (i >> 2) + 4 (l >> 5) + (i & 3)
 //   O^T = V^T P^T: results 8 b .. 8 b + 7 are operand elements of 16 keys as they lie; V^T's lane gets the same keys by
 //         transposing LDS reads (16 lanes read 4 keys x 16 columns, lane i gets column i of the 4)
-// A lane's row is the same in S^T and O^T, as in the decode kernel.  A row of LDS (2 D bytes) keeps its 16-byte pieces
-// in an order of its own, K's so that 16 keys' reads of one piece meet no bank twice, V's so that 8 keys' 64 bytes do not.
+// A lane's row is the same in S^T and O^T, as in the decode kernel.  LDS rows are padded, K's by 16 bytes so that 16
+// keys' reads of one piece meet no bank twice, V's by 64 so that 4 keys' 64 bytes do not; padded rows, unlike permuted
+// ones, let one address register and the instructions' offsets reach a whole step, and the two buffers are two copies of
+// the loop's body for the same reason: the registers are all taken (output 64, Q 32, scores 32, K and V on the way 32).
 template <class T, int D>
 struct Prefill {
     static constexpr int ROWS = 128, KEYS = 64, WAVES = 4, THREADS = 256;
@@ -40,14 +42,15 @@ struct Prefill {
     static constexpr int DT = D / 32;                   // column tiles of the output
     static constexpr float SHIFT = std::is_same_v<T, f16> ? 8.f : 0.f;   // fp16 probabilities are held times 2^8
 
-    struct Shared {
-        uint16_t k[2][KEYS * D], v[2][KEYS * D];
+    static constexpr int K_LD = D + 8, V_LD = D + 32;   // LDS rows, halves
+
+    struct alignas(16) Shared {
+        alignas(16) uint16_t k[2][KEYS * K_LD];
+        alignas(16) uint16_t v[2][KEYS * V_LD];
         uint64_t find[WAVES + 4];
-        int page[2][WAVES];                             // of a wave's 16 keys: 1 its page is one, 2 zeroed elements are to be added
+        alignas(16) int page[2][WAVES];                 // of a wave's 16 keys: 1 its page is one, 2 zeroed elements are to be added
         int last;
     };
-    static __device__ __forceinline__ int k_piece(int key, int piece) { return piece ^ (D == 64 ? (key >> 1) & 7 : key & 15); }
-    static __device__ __forceinline__ int v_piece(int key, int piece) { return piece ^ (D == 64 ? ((key >> 1) & 1) << 2 : (key & 3) << 2); }
 };
 
 template <class T, int D>
@@ -78,8 +81,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_prefill_kernel(Att
 
     while (true) {
         const AttnTile tile = wk.tile;
-        const int n_steps = (int) min((int64_t) (tile.steps - off), left);
-        const int s0 = tile.step0 + off, s1 = s0 + n_steps, rows = wk.n * a.group;
+        const int n_steps = __builtin_amdgcn_readfirstlane((int) min((int64_t) (tile.steps - off), left));
+        const int s0 = __builtin_amdgcn_readfirstlane(tile.step0) + off, s1 = s0 + n_steps, rows = wk.n * a.group;
         const int* const table = a.table + (int64_t) wk.r * a.ld_table;
         const char* const kh = reinterpret_cast<const char*>(a.k + (int64_t) wk.h * a.k_ldh);
         const char* const vh = reinterpret_cast<const char*>(a.v + (int64_t) wk.h * a.v_ldh);
@@ -126,11 +129,12 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_prefill_kernel(Att
                 vr[i] = *reinterpret_cast<gc_u32x4*>(vp + (uint32_t) (row * (int) a.v_ldt + 8 * st_piece) * 2u);
             }
         };
-        auto store = [&](int buf, int s, int p) __attribute__((always_inline)) {
+        auto store = [&](auto BUF, int s, int p) __attribute__((always_inline)) {
             const int key0 = X::KEYS * s + 16 * wave;
             // whether every row of the tile sees these keys; if not, V of keys that no row sees may hold anything and is
             // zeroed, and so are infinities and NaN, which a probability of 0 does not hide from the rows that do not see them
             const bool seen = p >= 0 && key0 + 15 <= wk.pos0 + tile.first && (!a.window || key0 > wk.pos0 + tile.last - a.window) && key0 + 16 <= a.cap;
+            constexpr int buf = BUF;
             int flags = p >= 0 ? 1 : 0;
             if (!seen) {
                 uint32_t f = 0;
@@ -150,12 +154,13 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_prefill_kernel(Att
 #pragma unroll
             for (int i = 0; i < LI; ++i) {
                 const int key = 16 * wave + st_row + 64 / CH * i;
-                *reinterpret_cast<u32x4*>(&sh.k[buf][key * D + 8 * X::k_piece(key, st_piece)]) = kr[i];
-                *reinterpret_cast<u32x4*>(&sh.v[buf][key * D + 8 * X::v_piece(key, st_piece)]) = vr[i];
+                *reinterpret_cast<u32x4*>(&sh.k[buf][key * X::K_LD + 8 * st_piece]) = kr[i];
+                *reinterpret_cast<u32x4*>(&sh.v[buf][key * X::V_LD + 8 * st_piece]) = vr[i];
             }
             if (lane == 0) sh.page[buf][wave] = flags;
         };
-        auto compute = [&](int buf, int s) __attribute__((always_inline)) {
+        auto compute = [&](auto BUF, int s) __attribute__((always_inline)) {
+            constexpr int buf = BUF;
             const int k0 = X::KEYS * s;
             // nothing for this wave's rows in the step
             if (!rows_here || k0 > w_last || (a.window && k0 + X::KEYS - 1 <= w_first - a.window)) return;
@@ -171,7 +176,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_prefill_kernel(Att
             for (int c = 0; c < KS; ++c)
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
-                    const u32x4 kf = *reinterpret_cast<const u32x4*>(&sh.k[buf][(32 * y + c32) * D + 8 * X::k_piece(c32, 2 * c + h2)]);
+                    const u32x4 kf = *reinterpret_cast<const u32x4*>(&sh.k[buf][(32 * y + c32) * X::K_LD + 16 * c + 8 * h2]);
                     st[y] = mfma32<T>(kf, q[c], st[y]);
                 }
             if (!whole) {
@@ -201,6 +206,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_prefill_kernel(Att
             }
             const float base = X::SHIFT - m;
             u32x4 pb[2][2];
+            float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int y = 0; y < 2; ++y)
 #pragma unroll
@@ -209,11 +215,12 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_prefill_kernel(Att
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const float x = exp2_fast(fmaf(st[y][8 * b + j], a.scale, base));
-                        l += x;
+                        ls[j & 3] += x;
                         p[j] = (T) x;
                     }
                     pb[y][b] = __builtin_bit_cast(u32x4, p);
                 }
+            l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -225,7 +232,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_prefill_kernel(Att
                         for (int x = 0; x < 2; ++x) {
                             const int key = 32 * y + 16 * b + 8 * x + 4 * h2 + tr_row;
                             const s16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) (
-                                &sh.v[buf][key * D + 8 * X::v_piece(tr_row, 4 * d + 2 * tr_half + (tr_q >> 1)) + 4 * (tr_q & 1)]));
+                                &sh.v[buf][key * X::V_LD + 32 * d + 16 * tr_half + 4 * tr_q]));
                             const u32x2 w = __builtin_bit_cast(u32x2, r);
                             vf[2 * x] = w[0];
                             vf[2 * x + 1] = w[1];
@@ -261,20 +268,21 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_prefill_kernel(Att
         if (tile.lo < tile.hi) {
             int p0 = page_of(s0), p1 = page_of(s0 + 1), p2 = page_of(s0 + 2);
             request(s0, p0);
-            store(0, s0, p0);
+            store(std::integral_constant<int, 0>{}, s0, p0);
             if (s0 + 1 < s1) request(s0 + 1, p1);
             __syncthreads();
-            int buf = 0;
-            for (int s = s0;; ++s) {
-                compute(buf, s);
-                if (s + 1 == s1) break;
-                buf ^= 1;
-                store(buf, s + 1, p1);
+            // step s from one buffer, with step s + 1 into the other; false: it was the last
+            auto turn = [&](auto BUF, int s) __attribute__((always_inline)) {
+                compute(BUF, s);
+                if (s + 1 == s1) return false;
+                store(std::integral_constant<int, 1 - BUF>{}, s + 1, p1);
                 p1 = p2;
                 p2 = page_of(s + 3);
                 if (s + 2 < s1) request(s + 2, p1);
                 __syncthreads();
-            }
+                return true;
+            };
+            for (int s = s0; turn(std::integral_constant<int, 0>{}, s) && turn(std::integral_constant<int, 1>{}, s + 1); s += 2) {}
         }
 
         // a wave's 32 rows, or their part
