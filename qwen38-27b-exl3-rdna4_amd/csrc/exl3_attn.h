@@ -180,22 +180,29 @@ struct AttnWork {
         }
         __syncthreads();
         const int* o = reinterpret_cast<const int*>(lds + THREADS / 64);
-        r = __builtin_amdgcn_readfirstlane(o[0]);
-        t = __builtin_amdgcn_readfirstlane(o[1]);
+        r = o[0];
+        t = o[1];
         off = __builtin_amdgcn_readfirstlane(o[2]);
-        tok0 = __builtin_amdgcn_readfirstlane(o[3]);
-        n = __builtin_amdgcn_readfirstlane(o[4]);
-        pos0 = __builtin_amdgcn_readfirstlane(o[5]);
-        tile = tile_of(t);
+        tok0 = o[3];
+        n = o[4];
+        pos0 = o[5];
         return true;
+    }
+    // all of it into scalar registers (the compiler keeps values that went through a loop or LDS in vector ones)
+    __device__ __forceinline__ void settle()
+    {
+        r = __builtin_amdgcn_readfirstlane(r);
+        t = __builtin_amdgcn_readfirstlane(t);
+        h = __builtin_amdgcn_readfirstlane(h);
+        tok0 = __builtin_amdgcn_readfirstlane(tok0);
+        n = __builtin_amdgcn_readfirstlane(n);
+        pos0 = __builtin_amdgcn_readfirstlane(pos0);
+        tile = tile_of(t);
     }
     // the tile after this one (there is one)
     __device__ __forceinline__ void next()
     {
-        if (++t < tiles()) {
-            tile = tile_of(t);
-            return;
-        }
+        if (++t < tiles()) return;
         t = 0;
         int i = r;
         do {
@@ -204,11 +211,7 @@ struct AttnWork {
                 ++h;
             }
             request(i);
-            tok0 = __builtin_amdgcn_readfirstlane(tok0);
-            n = __builtin_amdgcn_readfirstlane(n);
-            pos0 = __builtin_amdgcn_readfirstlane(pos0);
-        } while (n == 0);
-        tile = tile_of(0);
+        } while (__builtin_amdgcn_readfirstlane(n) == 0);
     }
 };
 

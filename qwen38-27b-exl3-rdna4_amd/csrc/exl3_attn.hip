@@ -115,8 +115,9 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
     for (int i = 0; i < 4; ++i) v_lane[i] = (uint32_t) ((4 * g4 + i) * (int) a.v_ldt) * 2u + (uint32_t) (X::VW * c16);
 
     while (true) {
+        wk.settle();
         const AttnTile tile = wk.tile;
-        const int n_steps = (int) min((int64_t) (tile.steps - off), left);
+        const int n_steps = __builtin_amdgcn_readfirstlane((int) min((int64_t) (tile.steps - off), left));
         const int s0 = tile.step0 + off, s1 = s0 + n_steps;
         const int* const row = a.table + (int64_t) wk.r * a.ld_table;
         const char* const kh = reinterpret_cast<const char*>(a.k + (int64_t) wk.h * a.k_ldh);

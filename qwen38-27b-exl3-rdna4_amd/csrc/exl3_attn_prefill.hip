@@ -6,6 +6,8 @@ using namespace exl3;
 namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) char lchar;
+typedef __attribute__((address_space(3))) u32x4 lu32x4;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 template <class T> __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c);
@@ -79,10 +81,18 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_prefill_kernel(Att
     // transposing reads: key 4 h2 + tr_row of 8, columns 32 dt + 16 tr_half + 4 tr_q ..
     const int s16 = lane & 15, tr_row = s16 >> 2, tr_q = s16 & 3, tr_half = (lane >> 4) & 1;
 
+    const uint32_t k_lane = (uint32_t) (st_row * (int) a.k_ldt + 8 * st_piece) * 2u, v_lane = (uint32_t) (st_row * (int) a.v_ldt + 8 * st_piece) * 2u;
+    // LDS addresses of the lane's writes and reads: what the instructions' offsets are added to
+    lchar* const k_put = (lchar*) &sh.k[0][(16 * wave + st_row) * X::K_LD + 8 * st_piece];
+    lchar* const v_put = (lchar*) &sh.v[0][(16 * wave + st_row) * X::V_LD + 8 * st_piece];
+    lchar* const k_get = (lchar*) &sh.k[0][c32 * X::K_LD + 8 * h2];
+    lchar* const v_get = (lchar*) &sh.v[0][(4 * h2 + tr_row) * X::V_LD + 16 * tr_half + 4 * tr_q];
+
     while (true) {
+        wk.settle();
         const AttnTile tile = wk.tile;
         const int n_steps = __builtin_amdgcn_readfirstlane((int) min((int64_t) (tile.steps - off), left));
-        const int s0 = __builtin_amdgcn_readfirstlane(tile.step0) + off, s1 = s0 + n_steps, rows = wk.n * a.group;
+        const int s0 = tile.step0 + off, s1 = s0 + n_steps, rows = wk.n * a.group;
         const int* const table = a.table + (int64_t) wk.r * a.ld_table;
         const char* const kh = reinterpret_cast<const char*>(a.k + (int64_t) wk.h * a.k_ldh);
         const char* const vh = reinterpret_cast<const char*>(a.v + (int64_t) wk.h * a.v_ldh);
@@ -112,7 +122,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_prefill_kernel(Att
                 p = table[a.d_page.div((uint32_t) key)];
                 if ((unsigned) p >= (unsigned) a.pages) p = -1;
             }
-            return p;
+            return __builtin_amdgcn_readfirstlane(p);
         };
         auto keys_at = [&](const char* base, int64_t ldp, int64_t ldt, int p, int key) __attribute__((always_inline)) {
             const int in = key - (int) a.d_page.div((uint32_t) key) * a.page;
@@ -124,9 +134,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_prefill_kernel(Att
             gc_char* const vp = keys_at(vh, a.v_ldp, a.v_ldt, p, X::KEYS * s + 16 * wave);
 #pragma unroll
             for (int i = 0; i < LI; ++i) {
-                const int row = st_row + 64 / CH * i;
-                kr[i] = *reinterpret_cast<gc_u32x4*>(kp + (uint32_t) (row * (int) a.k_ldt + 8 * st_piece) * 2u);
-                vr[i] = *reinterpret_cast<gc_u32x4*>(vp + (uint32_t) (row * (int) a.v_ldt + 8 * st_piece) * 2u);
+                kr[i] = *reinterpret_cast<gc_u32x4*>(kp + (int64_t) (128 / CH * i) * a.k_ldt + k_lane);
+                vr[i] = *reinterpret_cast<gc_u32x4*>(vp + (int64_t) (128 / CH * i) * a.v_ldt + v_lane);
             }
         };
         auto store = [&](auto BUF, int s, int p) __attribute__((always_inline)) {
@@ -153,9 +162,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_prefill_kernel(Att
             }
 #pragma unroll
             for (int i = 0; i < LI; ++i) {
-                const int key = 16 * wave + st_row + 64 / CH * i;
-                *reinterpret_cast<u32x4*>(&sh.k[buf][key * X::K_LD + 8 * st_piece]) = kr[i];
-                *reinterpret_cast<u32x4*>(&sh.v[buf][key * X::V_LD + 8 * st_piece]) = vr[i];
+                *reinterpret_cast<lu32x4*>(k_put + 2 * (buf * X::KEYS + 64 / CH * i) * X::K_LD) = kr[i];
+                *reinterpret_cast<lu32x4*>(v_put + 2 * (buf * X::KEYS + 64 / CH * i) * X::V_LD) = vr[i];
             }
             if (lane == 0) sh.page[buf][wave] = flags;
         };
@@ -167,100 +175,97 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_prefill_kernel(Att
             const int fl0 = __builtin_amdgcn_readfirstlane(sh.page[buf][0]), fl1 = __builtin_amdgcn_readfirstlane(sh.page[buf][1]),
                       fl2 = __builtin_amdgcn_readfirstlane(sh.page[buf][2]), fl3 = __builtin_amdgcn_readfirstlane(sh.page[buf][3]);
             const bool whole = (fl0 & fl1 & fl2 & fl3 & 1) && k0 + X::KEYS - 1 <= w_first && (!a.window || k0 > w_last - a.window) && k0 + X::KEYS <= a.cap;
-            f32x16 st[2];
 #pragma unroll
-            for (int y = 0; y < 2; ++y)
+            for (int y = 0; y < 2; ++y) {
+                const int ky = k0 + 32 * y;
+                f32x16 st;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) st[y][i] = 0.f;
+                for (int i = 0; i < 16; ++i) st[i] = 0.f;
+                u32x4 kf[KS];
 #pragma unroll
-            for (int c = 0; c < KS; ++c)
+                for (int c = 0; c < KS; ++c) kf[c] = *reinterpret_cast<lu32x4*>(k_get + 2 * ((buf * X::KEYS + 32 * y) * X::K_LD + 16 * c));
+                __builtin_amdgcn_sched_barrier(0);      // all the reads go out first: left alone, each product waits for its own
 #pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    const u32x4 kf = *reinterpret_cast<const u32x4*>(&sh.k[buf][(32 * y + c32) * X::K_LD + 16 * c + 8 * h2]);
-                    st[y] = mfma32<T>(kf, q[c], st[y]);
-                }
-            if (!whole) {
-#pragma unroll
-                for (int y = 0; y < 2; ++y)
+                for (int c = 0; c < KS; ++c) st = mfma32<T>(kf[c], q[c], st);
+                if (!whole) {
+                    const int end0 = (y ? fl2 : fl0) & 1 ? upto : -1, end1 = (y ? fl3 : fl1) & 1 ? upto : -1;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const int key = k0 + 32 * y + 8 * (i >> 2) + 4 * h2 + (i & 3);
-                        const int end = ((y ? (i < 8 ? fl2 : fl3) : (i < 8 ? fl0 : fl1)) & 1) ? upto : -1;
-                        st[y][i] = ((key <= end) & (key > from)) ? st[y][i] : -INFINITY;
+                        const int key = ky + 8 * (i >> 2) + 4 * h2 + (i & 3);
+                        st[i] = ((key <= (i < 8 ? end0 : end1)) & (key > from)) ? st[i] : -INFINITY;
                     }
-            }
-            float mx = -INFINITY;
+                }
+                float mx = -INFINITY;
 #pragma unroll
-            for (int y = 0; y < 2; ++y)
+                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[i]);
+                float lo, hi;
+                halves_x(mx, lo, hi);
+                mx = fmaxf(m, fmaxf(lo, hi) * a.scale); // a.scale > 0
+                if (__any(mx > m)) {
+                    const float c = exp2_fast(m - mx);
+                    l *= c;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[y][i]);
-            float lo, hi;
-            halves_x(mx, lo, hi);
-            mx = fmaxf(m, fmaxf(lo, hi) * a.scale);     // a.scale > 0
-            if (__any(mx > m)) {
-                const float c = exp2_fast(m - mx);
-                l *= c;
-#pragma unroll
-                for (int d = 0; d < DT; ++d) o[d] *= c;
-                m = mx;
-            }
-            const float base = X::SHIFT - m;
-            u32x4 pb[2][2];
-            float ls[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int y = 0; y < 2; ++y)
+                    for (int d = 0; d < DT; ++d) o[d] *= c;
+                    m = mx;
+                }
+                const float base = X::SHIFT - m;
+                u32x4 pb[2];
+                float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
                     typename Elem<T>::x8 p;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const float x = exp2_fast(fmaf(st[y][8 * b + j], a.scale, base));
+                        const float x = exp2_fast(fmaf(st[8 * b + j], a.scale, base));
                         ls[j & 3] += x;
                         p[j] = (T) x;
                     }
-                    pb[y][b] = __builtin_bit_cast(u32x4, p);
+                    pb[b] = __builtin_bit_cast(u32x4, p);
                 }
-            l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+                l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+                u32x4 vf[2][2];
+                auto read_v = [&](u32x4 (&f)[2], int d) __attribute__((always_inline)) {
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int y = 0; y < 2; ++y)
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        u32x4 vf;
+                    for (int b = 0; b < 2; ++b)
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            const int key = 32 * y + 16 * b + 8 * x + 4 * h2 + tr_row;
-                            const s16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) (
-                                &sh.v[buf][key * X::V_LD + 32 * d + 16 * tr_half + 4 * tr_q]));
-                            const u32x2 w = __builtin_bit_cast(u32x2, r);
-                            vf[2 * x] = w[0];
-                            vf[2 * x + 1] = w[1];
+                            const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                (__attribute__((address_space(3))) s16x4*) (v_get + 2 * ((buf * X::KEYS + 32 * y + 16 * b + 8 * x) * X::V_LD + 32 * d))));
+                            f[b][2 * x] = w[0];
+                            f[b][2 * x + 1] = w[1];
                         }
-                        o[d] = mfma32<T>(vf, pb[y][b], o[d]);
-                    }
-            if ((fl0 | fl1 | fl2 | fl3) & 2) {
-                // the infinities and NaN that were zeroed, added to the rows that see them
+                };
+                read_v(vf[0], 0);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    if (d + 1 < DT) read_v(vf[(d + 1) & 1], d + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) o[d] = mfma32<T>(vf[d & 1][b], pb[b], o[d]);
+                }
+                if ((y ? fl2 | fl3 : fl0 | fl1) & 2) {
+                    // the infinities and NaN that were zeroed, added to the rows that see them
 #pragma unroll 1
-                for (int z = 0; z < X::KEYS; ++z) {
-                    const int key = k0 + z, fl = z < 16 ? fl0 : z < 32 ? fl1 : z < 48 ? fl2 : fl3;
-                    if (fl != 3 || key < tile.lo || key >= tile.hi) continue;
-                    const int p = table[a.d_page.div((uint32_t) key)], in = key - (int) a.d_page.div((uint32_t) key) * a.page;
-                    gc_u16* const vk = reinterpret_cast<gc_u16*>(as_global(vh) + ((int64_t) p * a.v_ldp + (int64_t) in * a.v_ldt) * 2);
-                    const int reg = 4 * (z >> 3) + (z & 3);                    // of 32: y, then i
-                    uint32_t pw = 0;
+                    for (int z = 0; z < 32; ++z) {
+                        const int key = ky + z, fl = z < 16 ? (y ? fl2 : fl0) : (y ? fl3 : fl1);
+                        if (fl != 3 || key < tile.lo || key >= tile.hi) continue;
+                        const int p = table[a.d_page.div((uint32_t) key)], in = key - (int) a.d_page.div((uint32_t) key) * a.page;
+                        gc_u16* const vk = reinterpret_cast<gc_u16*>(as_global(vh) + ((int64_t) p * a.v_ldp + (int64_t) in * a.v_ldt) * 2);
+                        const int reg = 4 * (z >> 3) + (z & 3);                    // of the 16 of st
+                        uint32_t pw = 0;
 #pragma unroll
-                    for (int y = 0; y < 16; ++y) pw = reg >> 1 == y ? pb[y >> 3][(y >> 2) & 1][y & 3] : pw;
-                    pw = (uint32_t) __shfl((int) pw, 32 * ((z >> 2) & 1) + c32);
-                    const float pr = (float) __builtin_bit_cast(T, (uint16_t) (reg & 1 ? pw >> 16 : pw));
-                    const uint32_t mask = ((key <= upto) & (key > from)) ? 0xFFFFu : 0u;
+                        for (int w = 0; w < 8; ++w) pw = reg >> 1 == w ? pb[w >> 2][w & 3] : pw;
+                        pw = (uint32_t) __shfl((int) pw, 32 * ((z >> 2) & 1) + c32);
+                        const float pr = (float) __builtin_bit_cast(T, (uint16_t) (reg & 1 ? pw >> 16 : pw));
+                        const uint32_t mask = ((key <= upto) & (key > from)) ? 0xFFFFu : 0u;
 #pragma unroll
-                    for (int d = 0; d < DT; ++d)
+                        for (int d = 0; d < DT; ++d)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const uint32_t b = vk[32 * d + 8 * (i >> 2) + 4 * h2 + (i & 3)];
-                            o[d][i] += pr * (float) __builtin_bit_cast(T, (uint16_t) (b & mask & nonfinite2<T>(b)));
-                        }
+                            for (int i = 0; i < 16; ++i) {
+                                const uint32_t b = vk[32 * d + 8 * (i >> 2) + 4 * h2 + (i & 3)];
+                                o[d][i] += pr * (float) __builtin_bit_cast(T, (uint16_t) (b & mask & nonfinite2<T>(b)));
+                            }
+                    }
                 }
             }
         };
