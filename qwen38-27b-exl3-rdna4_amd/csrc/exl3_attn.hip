@@ -454,6 +454,11 @@ extern "C" int exl3_paged_attention(const void* q, int64_t q_ldt, int64_t q_ldh,
     if (pages < 0 || page_size < 16 || page_size % 16 || page_size > EXL3_PAGED_MAX_PAGE || (int64_t) pages * page_size > INT32_MAX) return EXL3_EINVAL;
     if (table_cols < 0 || ld_table < table_cols || (int64_t) table_cols * page_size > INT32_MAX - 65536 || window < 0) return EXL3_EINVAL;
     if (window > EXL3_ATTN_MAX_WINDOW) return EXL3_EINVAL;
+    // a stride that addresses nothing may be anything
+    if (tokens == 1) q_ldt = o_ldt = 0;
+    if (q_heads == 1) q_ldh = o_ldh = 0;
+    if (kv_heads == 1) k_ldh = v_ldh = 0;
+    if (pages <= 1) k_ldp = v_ldp = 0;
     if (k_ldt > EXL3_ATTN_MAX_LDT || v_ldt > EXL3_ATTN_MAX_LDT) return EXL3_EINVAL;
     if (tokens == 0) return EXL3_OK;
     if (!q || !out || !cu_q || (pages && (!k_cache || !v_cache)) || (requests && !seq_lens) || (requests && table_cols && !block_table)) return EXL3_EINVAL;

@@ -20,6 +20,12 @@ template <> __device__ __forceinline__ f32x16 mfma32<__bf16>(u32x4 a, u32x4 b, f
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+// values formed by here: they would be sunk to their first use, past the products that they are to run beside
+__device__ __forceinline__ void here(u32x4& a, u32x4& b, float& c)
+{
+    asm volatile("" : "+v"(a), "+v"(b), "+v"(c));
+}
+
 // 128 rows a tile, 32 a wave, 64 keys a step.  K and V go through LDS once for the four waves: wave w requests keys
 // 16 w .. + 15 of step s + 2 (one page: page sizes are multiples of 16) while step s is computed, and stores those of
 // s + 1 into the other buffer after it, so a step has one barrier.
@@ -175,97 +181,141 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_prefill_kernel(Att
             const int fl0 = __builtin_amdgcn_readfirstlane(sh.page[buf][0]), fl1 = __builtin_amdgcn_readfirstlane(sh.page[buf][1]),
                       fl2 = __builtin_amdgcn_readfirstlane(sh.page[buf][2]), fl3 = __builtin_amdgcn_readfirstlane(sh.page[buf][3]);
             const bool whole = (fl0 & fl1 & fl2 & fl3 & 1) && k0 + X::KEYS - 1 <= w_first && (!a.window || k0 > w_last - a.window) && k0 + X::KEYS <= a.cap;
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                const int ky = k0 + 32 * y;
-                f32x16 st;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) st[i] = 0.f;
-                u32x4 kf[KS];
+            // Two halves of 32 keys, each of scores, softmax and products with V; the matrix unit works on the second half's scores
+            // while the first's exponentials are formed, and on the first's products while the second's are.
+            f32x16 st[2];
+            u32x4 kf[KS], pb[2][2], vf[2][2];
+            auto read_k = [&](int y) __attribute__((always_inline)) {
 #pragma unroll
                 for (int c = 0; c < KS; ++c) kf[c] = *reinterpret_cast<lu32x4*>(k_get + 2 * ((buf * X::KEYS + 32 * y) * X::K_LD + 16 * c));
-                __builtin_amdgcn_sched_barrier(0);      // all the reads go out first: left alone, each product waits for its own
+            };
+            auto read_v = [&](u32x4 (&f)[2], int y, int d) __attribute__((always_inline)) {
 #pragma unroll
-                for (int c = 0; c < KS; ++c) st = mfma32<T>(kf[c], q[c], st);
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (__attribute__((address_space(3))) s16x4*) (v_get + 2 * ((buf * X::KEYS + 32 * y + 16 * b + 8 * x) * X::V_LD + 32 * d))));
+                        f[b][2 * x] = w[0];
+                        f[b][2 * x + 1] = w[1];
+                    }
+            };
+            auto scores = [&](int y) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) st[y][i] = 0.f;
+#pragma unroll
+                for (int c = 0; c < KS; ++c) st[y] = mfma32<T>(kf[c], q[c], st[y]);
+            };
+            // masked scores; the factor by which the row's new maximum shrinks what was summed
+            auto maximum = [&](int y) __attribute__((always_inline)) {
                 if (!whole) {
                     const int end0 = (y ? fl2 : fl0) & 1 ? upto : -1, end1 = (y ? fl3 : fl1) & 1 ? upto : -1;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const int key = ky + 8 * (i >> 2) + 4 * h2 + (i & 3);
-                        st[i] = ((key <= (i < 8 ? end0 : end1)) & (key > from)) ? st[i] : -INFINITY;
+                        const int key = k0 + 32 * y + 8 * (i >> 2) + 4 * h2 + (i & 3);
+                        st[y][i] = ((key <= (i < 8 ? end0 : end1)) & (key > from)) ? st[y][i] : -INFINITY;
                     }
                 }
                 float mx = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[i]);
+                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[y][i]);
                 float lo, hi;
                 halves_x(mx, lo, hi);
                 mx = fmaxf(m, fmaxf(lo, hi) * a.scale); // a.scale > 0
-                if (__any(mx > m)) {
-                    const float c = exp2_fast(m - mx);
-                    l *= c;
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) o[d] *= c;
-                    m = mx;
-                }
+                const float c = exp2_fast(m - mx);
+                m = mx;
+                return c;
+            };
+            auto exponentials = [&](int y) __attribute__((always_inline)) {
                 const float base = X::SHIFT - m;
-                u32x4 pb[2];
                 float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
                     typename Elem<T>::x8 p;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const float x = exp2_fast(fmaf(st[8 * b + j], a.scale, base));
+                        const float x = exp2_fast(fmaf(st[y][8 * b + j], a.scale, base));
                         ls[j & 3] += x;
                         p[j] = (T) x;
                     }
-                    pb[b] = __builtin_bit_cast(u32x4, p);
+                    pb[y][b] = __builtin_bit_cast(u32x4, p);
                 }
-                l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-                u32x4 vf[2][2];
-                auto read_v = [&](u32x4 (&f)[2], int d) __attribute__((always_inline)) {
+                return (ls[0] + ls[1]) + (ls[2] + ls[3]);
+            };
+            auto products = [&](int y, int d) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int b = 0; b < 2; ++b)
+                for (int b = 0; b < 2; ++b) o[d] = mfma32<T>(vf[d & 1][b], pb[y][b], o[d]);
+            };
+            auto shrink = [&](float c) __attribute__((always_inline)) {
+                if (__any(c != 1.f)) {
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                (__attribute__((address_space(3))) s16x4*) (v_get + 2 * ((buf * X::KEYS + 32 * y + 16 * b + 8 * x) * X::V_LD + 32 * d))));
-                            f[b][2 * x] = w[0];
-                            f[b][2 * x + 1] = w[1];
-                        }
-                };
-                read_v(vf[0], 0);
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    if (d + 1 < DT) read_v(vf[(d + 1) & 1], d + 1);
-                    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) o[d] = mfma32<T>(vf[d & 1][b], pb[b], o[d]);
+                    for (int d = 0; d < DT; ++d) o[d] *= c;
                 }
-                if ((y ? fl2 | fl3 : fl0 | fl1) & 2) {
-                    // the infinities and NaN that were zeroed, added to the rows that see them
+            };
+            read_k(0);
+            __builtin_amdgcn_sched_barrier(0);          // all the reads go out first: left alone, each product waits for its own
+            scores(0);
+            read_k(1);
+            const float c0 = maximum(0);
+            shrink(c0);
+            float l0 = exponentials(0);
+            scores(1);
+#pragma unroll
+            for (int c = 0; c < KS; ++c) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);       // a product, then what fills its time
+                __builtin_amdgcn_sched_group_barrier(0x002, 60 / KS, 0);
+            }
+            here(pb[0][0], pb[0][1], l0);
+            l = l * c0 + l0;
+            const float c1 = maximum(1);
+            read_v(vf[0], 0, 0);
+            read_v(vf[1], 0, 1);
+            float l1 = exponentials(1);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                products(0, d);
+                if (d + 2 < DT) read_v(vf[d & 1], 0, d + 2);
+                else read_v(vf[d & 1], 1, d + 2 - DT);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 30 / DT, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 30 / DT, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+            }
+            here(pb[1][0], pb[1][1], l1);
+            l = l * c1 + l1;
+            shrink(c1);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                products(1, d);
+                if (d + 2 < DT) read_v(vf[d & 1], 1, d + 2);
+            }
+            if ((fl0 | fl1 | fl2 | fl3) & 2) {
+                // the infinities and NaN that were zeroed, added to the rows that see them
 #pragma unroll 1
-                    for (int z = 0; z < 32; ++z) {
-                        const int key = ky + z, fl = z < 16 ? (y ? fl2 : fl0) : (y ? fl3 : fl1);
-                        if (fl != 3 || key < tile.lo || key >= tile.hi) continue;
-                        const int p = table[a.d_page.div((uint32_t) key)], in = key - (int) a.d_page.div((uint32_t) key) * a.page;
-                        gc_u16* const vk = reinterpret_cast<gc_u16*>(as_global(vh) + ((int64_t) p * a.v_ldp + (int64_t) in * a.v_ldt) * 2);
-                        const int reg = 4 * (z >> 3) + (z & 3);                    // of the 16 of st
-                        uint32_t pw = 0;
+                for (int z = 0; z < X::KEYS; ++z) {
+                    const int key = k0 + z, fl = z < 16 ? fl0 : z < 32 ? fl1 : z < 48 ? fl2 : fl3;
+                    if (fl != 3 || key < tile.lo || key >= tile.hi) continue;
+                    const int p = table[a.d_page.div((uint32_t) key)], in = key - (int) a.d_page.div((uint32_t) key) * a.page;
+                    gc_u16* const vk = reinterpret_cast<gc_u16*>(as_global(vh) + ((int64_t) p * a.v_ldp + (int64_t) in * a.v_ldt) * 2);
+                    const int reg = 4 * (z >> 3) + (z & 3);                    // of the 32 of st
+                    uint32_t pw = 0;
 #pragma unroll
-                        for (int w = 0; w < 8; ++w) pw = reg >> 1 == w ? pb[w >> 2][w & 3] : pw;
-                        pw = (uint32_t) __shfl((int) pw, 32 * ((z >> 2) & 1) + c32);
-                        const float pr = (float) __builtin_bit_cast(T, (uint16_t) (reg & 1 ? pw >> 16 : pw));
-                        const uint32_t mask = ((key <= upto) & (key > from)) ? 0xFFFFu : 0u;
+                    for (int w = 0; w < 16; ++w) pw = reg >> 1 == w ? pb[w >> 3][(w >> 2) & 1][w & 3] : pw;
+                    pw = (uint32_t) __shfl((int) pw, 32 * ((z >> 2) & 1) + c32);
+                    const float pr = (float) __builtin_bit_cast(T, (uint16_t) (reg & 1 ? pw >> 16 : pw)) * (z < 32 ? c1 : 1.f);
+                    const uint32_t mask = ((key <= upto) & (key > from)) ? 0xFFFFu : 0u;
 #pragma unroll
-                        for (int d = 0; d < DT; ++d)
+                    for (int d = 0; d < DT; ++d)
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                const uint32_t b = vk[32 * d + 8 * (i >> 2) + 4 * h2 + (i & 3)];
-                                o[d][i] += pr * (float) __builtin_bit_cast(T, (uint16_t) (b & mask & nonfinite2<T>(b)));
-                            }
-                    }
+                        for (int i = 0; i < 16; ++i) {
+                            const uint32_t b = vk[32 * d + 8 * (i >> 2) + 4 * h2 + (i & 3)];
+                            o[d][i] += pr * (float) __builtin_bit_cast(T, (uint16_t) (b & mask & nonfinite2<T>(b)));
+                        }
                 }
             }
         };

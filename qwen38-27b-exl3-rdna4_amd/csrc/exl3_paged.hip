@@ -250,6 +250,12 @@ extern "C" int exl3_rope_kv_write(const void* q, int64_t q_ldt, int64_t q_ldh, c
     if (pages < 0 || page_size < 1 || page_size > EXL3_PAGED_MAX_PAGE || (int64_t) pages * page_size > INT32_MAX) return EXL3_EINVAL;
     if (tokens == 0) return EXL3_OK;
     if (!q || !k || !v || !positions || !slots || !q_out || !k_cache || !v_cache || (rot_dim && !inv_freq)) return EXL3_EINVAL;
+    // a stride that addresses nothing may be anything
+    if (tokens == 1) q_ldt = k_ldt = v_ldt = 0;
+    if (q_heads == 1) q_ldh = 0;
+    if (kv_heads == 1) k_ldh = v_ldh = kc_ldh = vc_ldh = 0;
+    if (pages <= 1) kc_ldp = vc_ldp = 0;
+    if (page_size == 1) kc_ldt = vc_ldt = 0;
     if (!aligned16({q, k, v, q_out, k_cache, v_cache}) ||
         !multiples_of_8({q_ldt, q_ldh, k_ldt, k_ldh, v_ldt, v_ldh, kc_ldp, kc_ldt, kc_ldh, vc_ldp, vc_ldt, vc_ldh}))
         return EXL3_EINVAL;

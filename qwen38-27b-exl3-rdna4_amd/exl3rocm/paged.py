@@ -18,8 +18,9 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib as L
-from .kernels import _need, _stream
+from .kernels import _need
 
+_raw_stream = torch._C._cuda_getCurrentRawStream      # the current stream's handle on a GPU
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 HEAD_DIMS = (64, 128, 256)
 
@@ -67,18 +68,39 @@ def rope_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[dict
     return f.to(device), mscale
 
 
-def _ints(name: str, t: torch.Tensor, device, dtype, numel: Optional[int] = None):
-    if t.dtype != dtype or t.device != device or not t.is_contiguous() or (numel is not None and t.numel() != numel):
-        _need(False, f"{name} must be a contiguous {dtype} tensor on {device}" + (f" of {numel} elements" if numel is not None else ""))
+# An eager call's host time is what bounds a decode step's small launches, so the checks below read each attribute
+# once (get_device is half the time of device), a step's outputs are cut from one allocation, and the library's
+# entry points are looked up once.
+_fn: dict = {}
 
 
-def _on_gpu(t: torch.Tensor, what: str):
-    _need(t.is_cuda, f"{what}: tensors must be on a GPU (no CPU path)")
+def _entry(name: str):
+    f = _fn.get(name)
+    if f is None:
+        f = _fn[name] = getattr(L.lib(), name)
+    return f
 
 
-def _ld(t: torch.Tensor, dims: int) -> list:
-    """Strides of t's first `dims` dimensions; 0 for one of a single element, whose stride addresses nothing."""
-    return [s if n > 1 else 0 for n, s in zip(t.shape[:dims], t.stride())]
+def _ints(name: str, t: torch.Tensor, gpu: int, dtype, numel: Optional[int] = None):
+    if t.dtype is not dtype or t.get_device() != gpu or not t.is_contiguous() or (numel is not None and t.numel() != numel):
+        _need(False, f"{name} must be a contiguous {dtype} tensor on GPU {gpu}" + (f" of {numel} elements" if numel is not None else ""))
+
+
+def _gpu(t: torch.Tensor, what: str) -> int:
+    i = t.get_device()
+    _need(i >= 0, f"{what}: tensors must be on a GPU (no CPU path)")
+    return i
+
+
+def _table(what: str, t: torch.Tensor, gpu: int, requests: int):
+    """(columns, row stride) of a block table."""
+    shape = t.shape
+    if t.dtype is not torch.int32 or t.get_device() != gpu or len(shape) != 2 or shape[0] != requests:
+        _need(False, f"{what}: block_table must be int32 [{requests}, columns] on GPU {gpu}")
+    cols = shape[1]
+    ld, one = t.stride()
+    _need(one == 1 or cols <= 1, f"{what}: block_table needs unit column stride")
+    return cols, ld if requests > 1 else cols
 
 
 def batch_plan(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
@@ -91,38 +113,35 @@ def batch_plan(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torc
     padded for a captured graph has them.  free_left [1] is the next free_count; negative: that many pages were missing,
     and the tokens without one have slot -1 (nothing is written for them).  The stack and its count are only read:
     a repeated call gives the same result."""
-    _on_gpu(ctx_lens, "batch_plan")
-    dev, i32 = ctx_lens.device, torch.int32
+    gpu, i32 = _gpu(ctx_lens, "batch_plan"), torch.int32
     R = ctx_lens.numel()
-    _ints("batch_plan: ctx_lens", ctx_lens, dev, i32)
-    _ints("batch_plan: new_lens", new_lens, dev, i32, R)
-    _ints("batch_plan: free_pages", free_pages, dev, i32)
-    _ints("batch_plan: free_count", free_count, dev, i32, 1)
-    _need(block_table.dtype == i32 and block_table.device == dev and block_table.dim() == 2 and block_table.shape[0] == R
-          and (block_table.shape[1] <= 1 or block_table.stride(1) == 1),
-          f"batch_plan: block_table must be int32 [{R}, columns] on {dev} with unit column stride")
+    _ints("batch_plan: ctx_lens", ctx_lens, gpu, i32)
+    _ints("batch_plan: new_lens", new_lens, gpu, i32, R)
+    _ints("batch_plan: free_pages", free_pages, gpu, i32)
+    _ints("batch_plan: free_count", free_count, gpu, i32, 1)
+    cols, ld = _table("batch_plan", block_table, gpu, R)
     _need(page_size >= 1 and num_tokens >= 0, "batch_plan: page_size from 1, num_tokens from 0")
-    cols = block_table.shape[1]
-    ld = block_table.stride(0) if R > 1 else cols
-    ints = torch.empty(2 * R + 2, dtype=i32, device=dev)          # one allocation: cu_q, seq_lens, free_left
+    dev = ctx_lens.device
+    ints = torch.empty(2 * R + 2, dtype=i32, device=dev)
     tok = torch.empty((2, num_tokens), dtype=torch.int64, device=dev)
-    cu_q, seq, left = ints[:R + 1], ints[R + 1:2 * R + 1], ints[2 * R + 1:]
-    p = ints.data_ptr()
-    t = tok.data_ptr()
-    L.check(L.lib().exl3_batch_plan(ctx_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), ld, cols, free_pages.data_ptr(),
-                                    free_pages.numel(), free_count.data_ptr(), p, p + 4 * (R + 1), t, t + 8 * num_tokens,
-                                    p + 4 * (2 * R + 1), R, page_size, num_tokens, _stream(ctx_lens)), "batch_plan")
-    return cu_q, seq, tok[0], tok[1], left
+    p, t = ints.data_ptr(), tok.data_ptr()
+    L.check(_entry("exl3_batch_plan")(ctx_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), ld, cols, free_pages.data_ptr(),
+                                      free_pages.numel(), free_count.data_ptr(), p, p + 4 * (R + 1), t, t + 8 * num_tokens,
+                                      p + 4 * (2 * R + 1), R, page_size, num_tokens, _raw_stream(gpu)), "batch_plan")
+    cu_q, seq, left = ints.split((R + 1, R, 1))
+    pos, slots = tok.unbind()
+    return cu_q, seq, pos, slots, left
 
 
-def _cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, dtype, device, hkv: int, d: int):
-    """Checks a cache against the heads that use it; its pages and page size."""
-    if not (k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype == dtype
-            and k_cache.device == v_cache.device == device and k_cache.stride(3) == v_cache.stride(3) == 1
-            and k_cache.shape[2] == hkv and k_cache.shape[3] == d):
-        _need(False, f"{what}: k_cache and v_cache must be {dtype} [pages, page_size, {hkv}, {d}] on {device} with unit last stride, "
-                     f"got {tuple(k_cache.shape)} {k_cache.dtype} and {tuple(v_cache.shape)} {v_cache.dtype}")
-    return k_cache.shape[0], k_cache.shape[1]
+def _cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, dtype, gpu: int, d: int):
+    """Checks a cache against the heads that use it; its (pages, page size, kv heads)."""
+    shape = k_cache.shape
+    if not (len(shape) == 4 and shape == v_cache.shape and k_cache.dtype is dtype and v_cache.dtype is dtype
+            and k_cache.get_device() == gpu and v_cache.get_device() == gpu and shape[3] == d
+            and k_cache.stride(3) == 1 and v_cache.stride(3) == 1):
+        _need(False, f"{what}: k_cache and v_cache must be {dtype} [pages, page_size, kv_heads, {d}] on GPU {gpu} with unit last stride, "
+                     f"got {tuple(shape)} {k_cache.dtype} and {tuple(v_cache.shape)} {v_cache.dtype}")
+    return shape[0], shape[1], shape[2]
 
 
 def rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
@@ -133,38 +152,40 @@ def rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     8, unit last stride), e.g. columns of the fused q/k/v module's output.  positions, slots: int64 [T]; a slot
     outside the cache (-1) writes nothing.  inv_freq: float64 [rot_dim / 2], mscale: rope_frequencies; interleaved:
     pairs (2 i, 2 i + 1) instead of (i, i + rot_dim / 2).  fp16 or bf16, D of 64, 128 or 256."""
-    _on_gpu(q, "rope_kv_write")
-    dev, dt = q.device, q.dtype
-    _need(q.dim() == 3 and k.dim() == 3 and v.shape == k.shape and q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2],
-          f"rope_kv_write: q [T, q_heads, D], k and v [T, kv_heads, D], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    T, hq, d = q.shape
-    hkv = k.shape[1]
-    _need(dt in _DTYPES and k.dtype == dt and v.dtype == dt and k.device == dev and v.device == dev and d in HEAD_DIMS,
-          f"rope_kv_write: q, k and v of one type, fp16 or bf16, on one GPU, heads of {HEAD_DIMS}; got {dt}, {k.dtype}, {v.dtype}, {d}")
-    _need(T == 0 or (q.stride(2) == 1 and k.stride(2) == 1 and v.stride(2) == 1), "rope_kv_write: q, k and v need unit last stride")
-    pages, page = _cache("rope_kv_write", k_cache, v_cache, dt, dev, hkv, d)
-    _ints("rope_kv_write: positions", positions, dev, torch.int64, T)
-    _ints("rope_kv_write: slots", slots, dev, torch.int64, T)
-    _ints("rope_kv_write: inv_freq", inv_freq, dev, torch.float64)
-    out = torch.empty((T, hq, d), dtype=dt, device=dev)
-    L.check(L.lib().exl3_rope_kv_write(q.data_ptr(), *_ld(q, 2), k.data_ptr(), *_ld(k, 2), v.data_ptr(),
-                                       *_ld(v, 2), positions.data_ptr(), slots.data_ptr(), out.data_ptr(),
-                                       k_cache.data_ptr(), *_ld(k_cache, 3), v_cache.data_ptr(), *_ld(v_cache, 3),
-                                       inv_freq.data_ptr(), mscale, T, hq, hkv, d, 2 * inv_freq.numel(), int(interleaved), pages, page,
-                                       _DTYPES[dt], _stream(q)), "rope_kv_write")
+    gpu, dt = _gpu(q, "rope_kv_write"), q.dtype
+    qs, ks = q.shape, k.shape
+    _need(len(qs) == 3 and len(ks) == 3 and v.shape == ks and qs[0] == ks[0] and qs[2] == ks[2],
+          "rope_kv_write: q must be [T, q_heads, D], k and v [T, kv_heads, D]")
+    T, hq, d = qs
+    hkv = ks[1]
+    _need(dt in _DTYPES and k.dtype is dt and v.dtype is dt and k.get_device() == gpu and v.get_device() == gpu and d in HEAD_DIMS,
+          "rope_kv_write: q, k and v must be fp16 or bf16, all alike, on one GPU, with heads of 64, 128 or 256")
+    qt, qh, q1 = q.stride()
+    kt, kh, k1 = k.stride()
+    vt, vh, v1 = v.stride()
+    _need(q1 == 1 and k1 == 1 and v1 == 1 or T == 0, "rope_kv_write: q, k and v need unit last stride")
+    pages, page, heads = _cache("rope_kv_write", k_cache, v_cache, dt, gpu, d)
+    _need(heads == hkv, f"rope_kv_write: a cache of {heads} kv heads, k of {hkv}")
+    _ints("rope_kv_write: positions", positions, gpu, torch.int64, T)
+    _ints("rope_kv_write: slots", slots, gpu, torch.int64, T)
+    _ints("rope_kv_write: inv_freq", inv_freq, gpu, torch.float64)
+    out = torch.empty(qs, dtype=dt, device=q.device)
+    kcp, kct, kch, _ = k_cache.stride()
+    vcp, vct, vch, _ = v_cache.stride()
+    L.check(_entry("exl3_rope_kv_write")(q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, positions.data_ptr(), slots.data_ptr(),
+                                         out.data_ptr(), k_cache.data_ptr(), kcp, kct, kch, v_cache.data_ptr(), vcp, vct, vch,
+                                         inv_freq.data_ptr(), mscale, T, hq, hkv, d, 2 * inv_freq.numel(), interleaved, pages, page,
+                                         _DTYPES[dt], _raw_stream(gpu)), "rope_kv_write")
     return out
 
 
-_workspaces: dict = {}      # (device, stream) -> zeroed workspace of paged_attention
+_workspaces: dict = {}      # (GPU, stream) -> zeroed workspace of paged_attention
 
 
 def _workspace(device: torch.device, stream: int) -> torch.Tensor:
     """The stream's workspace: one size serves every shape, so a stream that made one eager call can capture any."""
-    ws = _workspaces.get((device, stream))
-    if ws is None:
-        _need(not torch.cuda.is_current_stream_capturing(), "paged_attention: this stream made no eager call before graph capture")
-        ws = torch.zeros(int(L.lib().exl3_paged_attention_workspace_size()), dtype=torch.uint8, device=device)
-        _workspaces[(device, stream)] = ws
+    _need(not torch.cuda.is_current_stream_capturing(), "paged_attention: this stream made no eager call before graph capture")
+    ws = _workspaces[(device.index, stream)] = torch.zeros(int(L.lib().exl3_paged_attention_workspace_size()), dtype=torch.uint8, device=device)
     return ws
 
 
@@ -175,32 +196,31 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     belong to request r and are the last of its seq_lens[r] tokens, whose pages block_table[r] lists (int32, as batch_plan
     makes them).  window: keys that a token sees, itself included (0: all).  A row that sees no key is 0; what a row
     does not see has no effect on it, NaN included."""
-    _on_gpu(q, "paged_attention")
-    dev, dt = q.device, q.dtype
-    _need(q.dim() == 3 and dt in _DTYPES and q.shape[2] in HEAD_DIMS and k_cache.dim() == 4,
-          f"paged_attention: q must be fp16 or bf16 [T, q_heads, D] with D of {HEAD_DIMS}, got {dt} {tuple(q.shape)}")
-    T, hq, d = q.shape
-    hkv = k_cache.shape[2]
-    pages, page = _cache("paged_attention", k_cache, v_cache, dt, dev, hkv, d)
+    gpu, dt = _gpu(q, "paged_attention"), q.dtype
+    qs = q.shape
+    _need(len(qs) == 3 and dt in _DTYPES and qs[2] in HEAD_DIMS, "paged_attention: q must be fp16 or bf16 [T, q_heads, D] with D of 64, 128 or 256")
+    T, hq, d = qs
+    pages, page, hkv = _cache("paged_attention", k_cache, v_cache, dt, gpu, d)
     _need(hkv > 0 and hq > 0 and hq % hkv == 0, f"paged_attention: {hq} query heads are no multiple of {hkv} kv heads")
     _need(page >= 16 and page % 16 == 0, f"paged_attention: page_size must be a multiple of 16, got {page}")
-    _need(T == 0 or q.stride(2) == 1, "paged_attention: q needs unit last stride")
+    qt, qh, q1 = q.stride()
+    _need(q1 == 1 or T == 0, "paged_attention: q needs unit last stride")
     R = seq_lens.numel()
-    _ints("paged_attention: seq_lens", seq_lens, dev, torch.int32)
-    _ints("paged_attention: cu_q", cu_q, dev, torch.int32, R + 1)
-    _need(block_table.dtype == torch.int32 and block_table.device == dev and block_table.dim() == 2 and block_table.shape[0] == R
-          and (block_table.shape[1] <= 1 or block_table.stride(1) == 1),
-          f"paged_attention: block_table must be int32 [{R}, columns] on {dev} with unit column stride")
+    _ints("paged_attention: seq_lens", seq_lens, gpu, torch.int32)
+    _ints("paged_attention: cu_q", cu_q, gpu, torch.int32, R + 1)
+    cols, ld = _table("paged_attention", block_table, gpu, R)
     _need(0 <= window <= 1 << 30, "paged_attention: window from 0 (none) to 2 ** 30")
-    cols = block_table.shape[1]
-    out = torch.empty((T, hq, d), dtype=dt, device=dev)
-    st = _stream(q)
-    ws = _workspace(dev, st)
-    L.check(L.lib().exl3_paged_attention(q.data_ptr(), *_ld(q, 2), k_cache.data_ptr(), *_ld(k_cache, 3),
-                                         v_cache.data_ptr(), *_ld(v_cache, 3), block_table.data_ptr(),
-                                         block_table.stride(0) if R > 1 else cols, cols, cu_q.data_ptr(), seq_lens.data_ptr(),
-                                         out.data_ptr(), hq * d, d, T, R, hq, hkv, d, pages, page, scale, window, _DTYPES[dt],
-                                         ws.data_ptr(), ws.numel(), st), "paged_attention")
+    dev = q.device
+    out = torch.empty(qs, dtype=dt, device=dev)
+    st = _raw_stream(gpu)
+    ws = _workspaces.get((gpu, st))
+    if ws is None:
+        ws = _workspace(dev, st)
+    kcp, kct, kch, _ = k_cache.stride()
+    vcp, vct, vch, _ = v_cache.stride()
+    L.check(_entry("exl3_paged_attention")(q.data_ptr(), qt, qh, k_cache.data_ptr(), kcp, kct, kch, v_cache.data_ptr(), vcp, vct, vch,
+                                           block_table.data_ptr(), ld, cols, cu_q.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), hq * d, d,
+                                           T, R, hq, hkv, d, pages, page, scale, window, _DTYPES[dt], ws.data_ptr(), ws.numel(), st), "paged_attention")
     return out
 
 
