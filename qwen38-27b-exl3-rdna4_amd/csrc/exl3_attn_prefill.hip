@@ -41,7 +41,7 @@ template <class T, int D>
 struct Prefill {
     static constexpr int ROWS = 128, KEYS = 64, WAVES = 4, THREADS = 256;
     static constexpr int GRID = D == 256 ? 256 : 512;   // workgroups: one or two a CU
-    static constexpr int SLOT = attn_slot(ROWS, D);
+    static constexpr int SLOT = attn_slot(ROWS, D + 2); // both halves of a wave hold its rows' maxima and sums
     static_assert(GRID <= ATTN_COUNTERS && (size_t) 2 * GRID * SLOT * 4 <= ATTN_PART_BYTES);
     static constexpr int LEAST = 4;                     // steps of a share at least
     static constexpr int CH = D / 8;                    // 16-byte pieces of a row
@@ -341,45 +341,96 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_prefill_kernel(Att
         }
 
         // a wave's 32 rows, or their part
-        const bool starts = off == 0, ends = off + n_steps == tile.steps, split = !(starts && ends);
+        const bool starts = off == 0, ends = off + n_steps == tile.steps;
         float lo, hi;
         halves_x(l, lo, hi);
         l = lo + hi;
-        const __amdgpu_buffer_rsrc_t prs = __builtin_amdgcn_make_buffer_rsrc(a.part, 0, (int) ATTN_PART_BYTES, RAW_BUFFER_FLAGS);
-        auto out_at = [&](int x) __attribute__((always_inline)) {                  // row x of the tile
-            const int y = wk.t * X::ROWS + x, tk = (int) a.d_group.div((uint32_t) y);
-            return as_global(a.out) + (int64_t) (wk.tok0 + tk) * a.o_ldt + (int64_t) (wk.h * a.group + y - tk * a.group) * a.o_ldh;
-        };
-        const uint32_t slot = (2u * (uint32_t) wg + (starts ? 1u : 0u)) * (uint32_t) X::SLOT;
-        if (xl < rows) {
-            const int x = 32 * wave + c32;
-            auto* const dst = out_at(x) + 4 * h2;
+        // column tiles d0 .. d0 + N - 1 of the output
+        auto put = [&](auto D0, auto N, const f32x16* sum, float total) __attribute__((always_inline)) {
+            if (xl < rows) {
+                auto* const dst = as_global(a.out) + (int64_t) (wk.tok0 + tok) * a.o_ldt + (int64_t) (wk.h * a.group + xl - tok * a.group) * a.o_ldh + 4 * h2;
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
+                for (int d = 0; d < N; ++d)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const f32x4 v = f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-                    if (!split) store_out<T>(dst + 32 * d + 8 * i, v, l);
-                    else
-                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), prs, (slot + (uint32_t) (x * D + 32 * d + 8 * i + 4 * h2)) * 4u, 0, SC1);
-                }
-            if (split && h2 == 0) {
-                const u32x2 ml = u32x2{(uint32_t) __float_as_int(m), (uint32_t) __float_as_int(l)};
-                __builtin_amdgcn_raw_buffer_store_b64(ml, prs, (slot + (uint32_t) (X::ROWS * D + 2 * x)) * 4u, 0, SC1);
+                    for (int i = 0; i < 4; ++i)
+                        store_out<T>(dst + 32 * (D0 + d) + 8 * i, f32x4{sum[d][4 * i], sum[d][4 * i + 1], sum[d][4 * i + 2], sum[d][4 * i + 3]}, total);
             }
-        }
-        if (split) {
+        };
+        if (starts && ends) {
+            put(std::integral_constant<int, 0>{}, std::integral_constant<int, DT>{}, o, l);
+        } else {
+            // A part moves as it lies in the registers (a lane's 16 bytes of 16 d + 4 i .. next to its neighbours').  The workgroup that
+            // finds all others' parts written joins them with its own, in the order of the workgroups, and writes none.
             const int first_wg = wg - (int) (((uint32_t) off + per - 1u) / per);
             const int last_wg = wg + (int) (((uint32_t) (tile.steps - off - n_steps) + per - 1u) / per);
-            __builtin_amdgcn_s_waitcnt(0x0F70);        // vmcnt(0): the part has landed
-            __syncthreads();
+            const __amdgpu_buffer_rsrc_t prs = __builtin_amdgcn_make_buffer_rsrc(a.part, 0, (int) ATTN_PART_BYTES, RAW_BUFFER_FLAGS);
+            // slot 2 c of workgroup c, 2 c + 1 for the tile's first
+            auto slot = [&](int c) __attribute__((always_inline)) {
+                return (2u * (uint32_t) c + (c == first_wg ? 1u : 0u)) * (uint32_t) (X::SLOT * 4) + (uint32_t) wave * (uint32_t) (X::SLOT);
+            };
+            const uint32_t at = 16u * (uint32_t) lane, ml_at = (uint32_t) (4 * DT * 1024) + 8u * (uint32_t) lane;
             if (tid == 0) {
-                const uint32_t before = __hip_atomic_fetch_add(&a.counters[first_wg], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                sh.last = before == (uint32_t) (last_wg - first_wg);
-                if (sh.last) __hip_atomic_store(&a.counters[first_wg], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                sh.last = __hip_atomic_load(&a.counters[first_wg], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t) (last_wg - first_wg);
             }
             __syncthreads();
-            if (sh.last) join_parts<T, D, X::ROWS, X::THREADS, X::SLOT, 4>(prs, first_wg, last_wg, min(X::ROWS, rows - wk.t * X::ROWS), out_at);
+            bool mine = sh.last;
+            if (!mine) {
+                const uint32_t to = slot(wg);
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]}), prs,
+                                                               at + 1024u * (uint32_t) (4 * d + i), to, SC1);
+                __builtin_amdgcn_raw_buffer_store_b64(u32x2{(uint32_t) __float_as_int(m), (uint32_t) __float_as_int(l)}, prs, ml_at, to, SC1);
+                __builtin_amdgcn_s_waitcnt(0x0F70);    // vmcnt(0): the part has landed
+                __syncthreads();
+                if (tid == 0)
+                    sh.last = __hip_atomic_fetch_add(&a.counters[first_wg], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t) (last_wg - first_wg);
+                __syncthreads();
+                mine = sh.last;
+            }
+            if (mine) {
+                if (tid == 0) __hip_atomic_store(&a.counters[first_wg], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                // four column tiles at a time: more would not fit beside the workgroup's own
+                constexpr int N = DT < 4 ? DT : 4;
+                static_for(std::make_integer_sequence<int, DT / N>{}, [&](auto P) __attribute__((always_inline)) {
+                    f32x16 sum[N];
+                    float top = LOWEST, total = 0.f;
+#pragma unroll
+                    for (int d = 0; d < N; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) sum[d][i] = 0.f;
+#pragma unroll 1
+                    for (int c = first_wg; c <= last_wg; ++c) {
+                        f32x16 x[N];
+                        float mc = m, lc = l;
+                        if (c == wg) {
+#pragma unroll
+                            for (int d = 0; d < N; ++d) x[d] = o[N * P + d];
+                        } else {
+                            const uint32_t fr = slot(c);
+                            const u32x2 ml = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(prs, ml_at, fr, SC1));
+#pragma unroll
+                            for (int d = 0; d < N; ++d)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const f32x4 v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(prs, at + 1024u * (uint32_t) (4 * (N * P + d) + i), fr, SC1));
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) x[d][4 * i + e] = v[e];
+                                }
+                            mc = __int_as_float((int) ml[0]);
+                            lc = __int_as_float((int) ml[1]);
+                        }
+                        const float up = fmaxf(top, mc), f = exp2_fast(top - up), g = exp2_fast(mc - up);
+                        total = total * f + lc * g;
+                        top = up;
+#pragma unroll
+                        for (int d = 0; d < N; ++d) sum[d] = sum[d] * f + x[d] * g;
+                    }
+                    put(std::integral_constant<int, N * P>{}, std::integral_constant<int, N>{}, sum, total);
+                });
+            }
         }
         __syncthreads();
         left -= n_steps;
