@@ -127,12 +127,21 @@ struct AttnWork {
     template <int THREADS>
     __device__ __forceinline__ bool find(int wg, int least, uint64_t* lds, int& off, int64_t& left, uint32_t& per)
     {
-        const int tid = threadIdx.x, each = (a.requests + THREADS - 1) / THREADS, r0 = min(tid * each, a.requests), r1 = min(r0 + each, a.requests);
+        // few requests: several threads each, a range of its tiles a thread (2^share_log of them)
+        const int tid = threadIdx.x, each = (a.requests + THREADS - 1) / THREADS;
+        int share_log = 0;
+        while ((a.requests << (share_log + 1)) <= THREADS && share_log < 8) ++share_log;
+        const int r0 = min(share_log ? tid >> share_log : tid * each, a.requests), r1 = min(r0 + max(each, 1), a.requests);
+        auto tiles_from = [&](int m, int& j, int& end) __attribute__((always_inline)) {
+            const int c = (m + (1 << share_log) - 1) >> share_log;
+            j = min((tid & ((1 << share_log) - 1)) * c, m);
+            end = min(j + c, m);
+        };
         uint64_t sum = 0;
         for (int i = r0; i < r1; ++i) {
             request(i);
-            const int m = tiles();
-            for (int j = 0; j < m; ++j) sum += (uint64_t) tile_of(j).steps;
+            int j, end;
+            for (tiles_from(tiles(), j, end); j < end; ++j) sum += (uint64_t) tile_of(j).steps;
         }
         uint64_t upto = sum;
 #pragma unroll
@@ -160,14 +169,13 @@ struct AttnWork {
             uint64_t x = u - (upto - sum);
             for (int i = r0;; ++i) {
                 request(i);
-                const int m = tiles();
-                int j = 0, steps = 0;
-                for (; j < m; ++j) {
-                    steps = tile_of(j).steps;
-                    if (x < (uint64_t) steps) break;
-                    x -= (uint64_t) steps;
+                int j, end;
+                for (tiles_from(tiles(), j, end); j < end; ++j) {
+                    const uint64_t steps = (uint64_t) tile_of(j).steps;
+                    if (x < steps) break;
+                    x -= steps;
                 }
-                if (j == m) continue;
+                if (j == end) continue;
                 int* o = reinterpret_cast<int*>(lds + THREADS / 64);
                 o[0] = i;
                 o[1] = j;
