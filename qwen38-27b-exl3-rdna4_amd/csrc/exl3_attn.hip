@@ -7,34 +7,6 @@ using namespace exl3;
 
 namespace {
 
-template <class T> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c);
-template <> __device__ __forceinline__ f32x4 mfma16<f16>(u32x4 a, u32x4 b, f32x4 c)
-{
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-template <> __device__ __forceinline__ f32x4 mfma16<__bf16>(u32x4 a, u32x4 b, f32x4 c)
-{
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-// max / sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48
-__device__ __forceinline__ float max_quads(float x)
-{
-    float lo, hi;
-    halves_x(x, lo, hi);
-    x = fmaxf(lo, hi);
-    const auto w = __builtin_amdgcn_permlane16_swap((uint32_t) __float_as_int(x), (uint32_t) __float_as_int(x), false, false);
-    return fmaxf(__int_as_float((int) w[0]), __int_as_float((int) w[1]));
-}
-__device__ __forceinline__ float sum_quads(float x)
-{
-    float lo, hi;
-    halves_x(x, lo, hi);
-    x = lo + hi;
-    const auto w = __builtin_amdgcn_permlane16_swap((uint32_t) __float_as_int(x), (uint32_t) __float_as_int(x), false, false);
-    return __int_as_float((int) w[0]) + __int_as_float((int) w[1]);
-}
-
 template <int N> struct Words;
 template <> struct Words<4> { typedef u32x4 T; typedef gc_u32x4 G; };
 template <> struct Words<2> { typedef u32x2 T; typedef gc_u32x2 G; };
