@@ -11,7 +11,7 @@ template <int N> struct Words;
 template <> struct Words<4> { typedef u32x4 T; typedef gc_u32x4 G; };
 template <> struct Words<2> { typedef u32x2 T; typedef gc_u32x2 G; };
 
-// ---- few rows: 16 NQ rows a tile, bound by the reading of K and V --------------------------------------------
+// ---- few rows: 16 rows a tile, bound by the reading of K and V --------------------------------------------
 // Every wave takes whole steps of 32 keys of its tile, with a softmax of its own (running maximum, sum, output), and
 // loads their K and V from memory straight into matrix operands, so the loop has no LDS traffic for them and no
 // barrier.  The next step's K is requested once this one's scores are formed, its V once this one's products are, so a
@@ -21,16 +21,16 @@ template <> struct Words<2> { typedef u32x2 T; typedef gc_u32x2 G; };
 //         8 (l >> 4) + j that is already P^T, if V^T's lane holds the same keys: its loads are 16 bytes of 8 rows
 //         of V (a row's 16 lanes read it whole), paired by v_perm, and column 8 (l & 15) + e is row l & 15 of product e
 // A lane's row of S^T and of O^T is the same (l & 15), so maxima, sums and corrections never leave the lane's column.
-template <class T, int D, int NQ, int WAVES>
+template <class T, int D, int WAVES>
 struct Decode {
-    static constexpr int ROWS = 16 * NQ, THREADS = 64 * WAVES;
+    static constexpr int ROWS = 16, THREADS = 64 * WAVES;
     static constexpr int KC = D / 32;                   // 16-byte pieces of a K row that a lane holds
     static constexpr int VW = D >= 128 ? 16 : 8;        // bytes of a V row that a lane loads at once
     static constexpr int VC = D * 2 / (16 * VW);        // ... and how many times
     static constexpr int E = VW / 2;                    // V columns of one load: its products
     static constexpr int LEAST = 4;                     // steps of a share at least
     static constexpr int PAD = D + 4;                   // LDS row (floats) of the waves' outputs
-    static constexpr bool Q_LDS = NQ * KC > 4;          // Q would take more than 16 registers: read from LDS at each step
+    static constexpr bool Q_LDS = KC > 4;               // Q would take more than 16 registers: read from LDS at each step
     static constexpr int Q_PAD = D + 8;                 // its LDS row (halves)
     static constexpr int GRID = 256;                    // workgroups: one a CU
     static constexpr int SLOT = attn_slot(ROWS, D);
@@ -44,7 +44,7 @@ struct Decode {
 
     struct Shared {
         float o[WAVES][16][PAD];
-        float m[WAVES][ROWS], l[WAVES][16];
+        float m[WAVES][ROWS], l[WAVES][ROWS];
         uint16_t q[Q_LDS ? ROWS : 1][Q_PAD];
         uint64_t find[WAVES + 4];
         int last;
@@ -60,10 +60,10 @@ struct Decode {
     }
 };
 
-template <class T, int D, int NQ, int WAVES>
+template <class T, int D, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
 {
-    using X = Decode<T, D, NQ, WAVES>;
+    using X = Decode<T, D, WAVES>;
     constexpr int KC = X::KC, VC = X::VC, E = X::E, ROWS = X::ROWS;
     __shared__ typename X::Shared sh;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c16 = lane & 15, g4 = lane >> 4;
@@ -95,25 +95,19 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
         const char* const kh = reinterpret_cast<const char*>(a.k + (int64_t) wk.h * a.k_ldh);
         const char* const vh = reinterpret_cast<const char*>(a.v + (int64_t) wk.h * a.v_ldh);
 
-        // Q^T: lane's row 16 i + c16 of the tile, elements 32 c + 8 g4 ..; and the position of the row's token
+        // Q^T: lane's row c16 of the tile, elements 32 c + 8 g4 ..; and the position of the row's token
         const int rows = wk.n * a.group;
         auto q_at = [&](int x) __attribute__((always_inline)) {
             const int y = min(wk.t * ROWS + x, rows - 1), tok = (int) a.d_group.div((uint32_t) y);
             return as_global(a.q) + (int64_t) (wk.tok0 + tok) * a.q_ldt + (int64_t) (wk.h * a.group + y - tok * a.group) * a.q_ldh;
         };
-        u32x4 q[NQ][X::Q_LDS ? 1 : KC];
-        int upto[NQ], from[NQ];                         // the lane's row sees keys from < key <= upto
+        u32x4 q[X::Q_LDS ? 1 : KC];
+        const int xl = wk.t * ROWS + c16, pos = xl < rows ? wk.pos0 + (int) a.d_group.div((uint32_t) xl) : -1;  // a row past the tile's sees nothing
+        const int upto = min(pos, a.cap - 1), from = a.window ? pos - a.window : -1;                            // the row sees from < key <= upto
+        if constexpr (!X::Q_LDS) {
+            auto* const src = q_at(c16) + 8 * g4;
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-            const int x = wk.t * ROWS + 16 * i + c16;
-            const int pos = x < rows ? wk.pos0 + (int) a.d_group.div((uint32_t) x) : -1;  // a row past the tile's sees nothing
-            upto[i] = min(pos, a.cap - 1);
-            from[i] = a.window ? pos - a.window : -1;
-            if constexpr (!X::Q_LDS) {
-                auto* const src = q_at(16 * i + c16) + 8 * g4;
-#pragma unroll
-                for (int c = 0; c < KC; ++c) q[i][c] = flipped(*reinterpret_cast<gc_u32x4*>(src + 32 * c), a.flip);
-            }
+            for (int c = 0; c < KC; ++c) q[c] = flipped(*reinterpret_cast<gc_u32x4*>(src + 32 * c), a.flip);
         }
         if constexpr (X::Q_LDS) {
             for (int z = tid; z < ROWS * D / 8; z += X::THREADS)
@@ -121,17 +115,12 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
                     flipped(*reinterpret_cast<gc_u32x4*>(q_at(z / (D / 8)) + 8 * (z % (D / 8))), a.flip);
             __syncthreads();
         }
-        f32x4 o[NQ][VC][E];
-        float m[NQ], l[NQ];
+        f32x4 o[VC][E];
+        float m = LOWEST, l = 0.f;
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-            m[i] = LOWEST;
-            l[i] = 0.f;
+        for (int c = 0; c < VC; ++c)
 #pragma unroll
-            for (int c = 0; c < VC; ++c)
-#pragma unroll
-                for (int e = 0; e < E; ++e) o[i][c][e] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+            for (int e = 0; e < E; ++e) o[c][e] = f32x4{0.f, 0.f, 0.f, 0.f};
 
         // pages of this wave's next 32 steps, lane 2 x + y: the y-th 16 keys of its x-th step; -1: none
         auto pages_from = [&](int s) __attribute__((always_inline)) {
@@ -190,60 +179,50 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
                 // whether every row sees every key of the step
                 const bool whole = p0 >= 0 && p1 >= 0 && 32 * s + 31 <= wk.pos0 + tile.first && (!a.window || 32 * s > wk.pos0 + tile.last - a.window) &&
                                    32 * s + 32 <= a.cap;
-                f32x4 st[NQ][2];
+                f32x4 st[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-                for (int i = 0; i < NQ; ++i)
+                for (int c = 0; c < KC; ++c) {
+                    u32x4 qc;
+                    if constexpr (X::Q_LDS) qc = *reinterpret_cast<const u32x4*>(&sh.q[c16][32 * c + 8 * g4]);
+                    else qc = q[c];
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) st[i][y] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < KC; ++c)
-#pragma unroll
-                    for (int i = 0; i < NQ; ++i) {
-                        u32x4 qc;
-                        if constexpr (X::Q_LDS) qc = *reinterpret_cast<const u32x4*>(&sh.q[16 * i + c16][32 * c + 8 * g4]);
-                        else qc = q[i][c];
-#pragma unroll
-                        for (int y = 0; y < 2; ++y) st[i][y] = mfma16<T>(k[y][c], qc, st[i][y]);
-                    }
-                if (next < s1) load_k(k, next, n0, n1);
-                u32x4 pb[NQ];
-#pragma unroll
-                for (int i = 0; i < NQ; ++i) {
-                    float mx = m[i];
-#pragma unroll
-                    for (int y = 0; y < 2; ++y)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float x = st[i][y][e] * a.scale;
-                            if (!whole) {
-                                const int key = 32 * s + 16 * y + 4 * g4 + e, end = (y ? p1 : p0) >= 0 ? upto[i] : -1;
-                                x = ((key <= end) & (key > from[i])) ? x : -INFINITY;
-                            }
-                            st[i][y][e] = x;
-                            mx = fmaxf(mx, x);
-                        }
-                    mx = max_quads(mx);
-                    if (__any(mx > m[i])) {
-                        const float c = exp2_fast(m[i] - mx);
-                        l[i] *= c;
-#pragma unroll
-                        for (int u = 0; u < VC; ++u)
-#pragma unroll
-                            for (int e = 0; e < E; ++e) o[i][u][e] *= c;
-                        m[i] = mx;
-                    }
-                    const float base = m[i] - X::SHIFT;
-                    typename Elem<T>::x8 p;
-#pragma unroll
-                    for (int y = 0; y < 2; ++y)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float x = exp2_fast(st[i][y][e] - base);
-                            l[i] += x;
-                            p[4 * y + e] = (T) x;
-                        }
-                    pb[i] = __builtin_bit_cast(u32x4, p);
+                    for (int y = 0; y < 2; ++y) st[y] = mfma16<T>(k[y][c], qc, st[y]);
                 }
+                if (next < s1) load_k(k, next, n0, n1);
+                float mx = m;
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float x = st[y][e] * a.scale;
+                        if (!whole) {
+                            const int key = 32 * s + 16 * y + 4 * g4 + e, end = (y ? p1 : p0) >= 0 ? upto : -1;
+                            x = ((key <= end) & (key > from)) ? x : -INFINITY;
+                        }
+                        st[y][e] = x;
+                        mx = fmaxf(mx, x);
+                    }
+                mx = max_quads(mx);
+                if (__any(mx > m)) {
+                    const float c = exp2_fast(m - mx);
+                    l *= c;
+#pragma unroll
+                    for (int u = 0; u < VC; ++u)
+#pragma unroll
+                        for (int e = 0; e < E; ++e) o[u][e] *= c;
+                    m = mx;
+                }
+                const float base = m - X::SHIFT;
+                typename Elem<T>::x8 p8;
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = exp2_fast(st[y][e] - base);
+                        l += x;
+                        p8[4 * y + e] = (T) x;
+                    }
+                const u32x4 pb = __builtin_bit_cast(u32x4, p8);
                 // What V holds for keys that a row does not see must not reach it, and a probability of 0 does not hide
                 // an infinity or NaN: V of keys that no row sees is zeroed, and where rows of several tokens differ in what
                 // they see, such elements are zeroed too and added afterwards to the rows that see them.
@@ -275,33 +254,26 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
 #pragma unroll
                 for (int u = 0; u < VC; ++u)
 #pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        const u32x4 vt = X::column(v, u, e);
-#pragma unroll
-                        for (int i = 0; i < NQ; ++i) o[i][u][e] = mfma16<T>(vt, pb[i], o[i][u][e]);
-                    }
+                    for (int e = 0; e < E; ++e) o[u][e] = mfma16<T>(X::column(v, u, e), pb, o[u][e]);
                 if (odd) {
 #pragma unroll 1
                     for (int y = 0; y < 32; ++y) {
                         const int key = 32 * s + y, j = 2 * (y >> 4) + ((y & 3) >> 1);
                         if (key < tile.lo || key >= tile.hi || (y < 16 ? p0 : p1) < 0) continue;
                         gc_u16* const vr = reinterpret_cast<gc_u16*>(keys_at(vh, a.v_ldp, a.v_ldt, y < 16 ? p0 : p1, 32 * s + (y & 16)) + (int64_t) (y & 15) * a.v_ldt * 2);
+                        uint32_t pw = j == 0 ? pb[0] : j == 1 ? pb[1] : j == 2 ? pb[2] : pb[3];
+                        pw = (uint32_t) __shfl((int) pw, 16 * ((y >> 2) & 3) + c16);
+                        const float p = (float) __builtin_bit_cast(T, (uint16_t) (y & 1 ? pw >> 16 : pw));
+                        const uint32_t seen = ((key <= upto) & (key > from)) ? 0xFFFFu : 0u;
 #pragma unroll
-                        for (int i = 0; i < NQ; ++i) {
-                            uint32_t pw = j == 0 ? pb[i][0] : j == 1 ? pb[i][1] : j == 2 ? pb[i][2] : pb[i][3];
-                            pw = (uint32_t) __shfl((int) pw, 16 * ((y >> 2) & 3) + c16);
-                            const float p = (float) __builtin_bit_cast(T, (uint16_t) (y & 1 ? pw >> 16 : pw));
-                            const uint32_t seen = ((key <= upto[i]) & (key > from[i])) ? 0xFFFFu : 0u;
+                        for (int u = 0; u < VC; ++u)
 #pragma unroll
-                            for (int u = 0; u < VC; ++u)
+                            for (int e = 0; e < E; ++e)
 #pragma unroll
-                                for (int e = 0; e < E; ++e)
-#pragma unroll
-                                    for (int d = 0; d < 4; ++d) {
-                                        const uint32_t b = vr[16 * E * u + E * (4 * g4 + d) + e];
-                                        o[i][u][e][d] += p * (float) __builtin_bit_cast(T, (uint16_t) (b & seen & nonfinite2<T>(b)));
-                                    }
-                        }
+                                for (int d = 0; d < 4; ++d) {
+                                    const uint32_t b = vr[16 * E * u + E * (4 * g4 + d) + e];
+                                    o[u][e][d] += p * (float) __builtin_bit_cast(T, (uint16_t) (b & seen & nonfinite2<T>(b)));
+                                }
                     }
                 }
                 if (next >= s1) break;
@@ -312,11 +284,9 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
             }
         }
 
-        // the waves' outputs joined: maxima and sums first, then 16 rows at a time
+        // the waves' outputs joined: maxima first, then sums and outputs scaled to their maximum
         const bool starts = off == 0, ends = off + n_steps == tile.steps, split = !(starts && ends);
-#pragma unroll
-        for (int i = 0; i < NQ; ++i)
-            if (g4 == 0) sh.m[wave][16 * i + c16] = m[i];
+        if (g4 == 0) sh.m[wave][c16] = m;
         __syncthreads();
         const int first_wg = wg - (int) (((uint32_t) off + per - 1u) / per);        // workgroups back to the tile's first step
         const uint32_t slot = 2u * (uint32_t) wg + (starts ? 1u : 0u);
@@ -326,45 +296,40 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
             return as_global(a.out) + (int64_t) (wk.tok0 + tok) * a.o_ldt + (int64_t) (wk.h * a.group + y - tok * a.group) * a.o_ldh;
         };
         const int live_rows = min(ROWS, rows - wk.t * ROWS);
+        float top = LOWEST;
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-            if (16 * i >= live_rows) break;            // uniform
-            float top = LOWEST;
+        for (int x = 0; x < WAVES; ++x) top = fmaxf(top, sh.m[x][c16]);
+        const float c = exp2_fast(m - top), lt = sum_quads(l) * c;
+        if (g4 == 0) sh.l[wave][c16] = lt;
 #pragma unroll
-            for (int x = 0; x < WAVES; ++x) top = fmaxf(top, sh.m[x][16 * i + c16]);
-            const float c = exp2_fast(m[i] - top), lt = sum_quads(l[i]) * c;
-            if (i) __syncthreads();
-            if (g4 == 0) sh.l[wave][c16] = lt;
+        for (int u = 0; u < VC; ++u)
 #pragma unroll
-            for (int u = 0; u < VC; ++u)
+            for (int y = 0; y < 4; ++y)                // product e holds columns E (4 g4 + y) + e of piece u
 #pragma unroll
-                for (int y = 0; y < 4; ++y)            // product e holds columns E (4 g4 + y) + e of piece u
-#pragma unroll
-                    for (int e = 0; e < E; e += 4)
-                        *reinterpret_cast<f32x4*>(&sh.o[wave][c16][16 * E * u + E * (4 * g4 + y) + e]) =
-                            f32x4{o[i][u][e][y] * c, o[i][u][e + 1][y] * c, o[i][u][e + 2][y] * c, o[i][u][e + 3][y] * c};
-            __syncthreads();
-            for (int z = tid; z < min(16, live_rows - 16 * i) * (D / 4); z += X::THREADS) {
-                const int x = z / (D / 4), col = 4 * (z % (D / 4));
-                float lx = 0.f;
-                f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int e = 0; e < E; e += 4)
+                    *reinterpret_cast<f32x4*>(&sh.o[wave][c16][16 * E * u + E * (4 * g4 + y) + e]) =
+                        f32x4{o[u][e][y] * c, o[u][e + 1][y] * c, o[u][e + 2][y] * c, o[u][e + 3][y] * c};
+        __syncthreads();
+        for (int z = tid; z < live_rows * (D / 4); z += X::THREADS) {
+            const int x = z / (D / 4), col = 4 * (z % (D / 4));
+            float lx = 0.f;
+            f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-                for (int y = 0; y < WAVES; ++y) {
-                    lx += sh.l[y][x];
-                    sum += *reinterpret_cast<const f32x4*>(&sh.o[y][x][col]);
-                }
-                if (!split) {
-                    store_out<T>(out_at(16 * i + x) + col, sum, lx);
-                } else {
-                    const uint32_t at = (slot * X::SLOT + (uint32_t) (16 * i + x) * D + (uint32_t) col) * 4u;
-                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum), prs, at, 0, SC1);
-                    if (col == 0) {
-                        float mx = LOWEST;
+            for (int y = 0; y < WAVES; ++y) {
+                lx += sh.l[y][x];
+                sum += *reinterpret_cast<const f32x4*>(&sh.o[y][x][col]);
+            }
+            if (!split) {
+                store_out<T>(out_at(x) + col, sum, lx);
+            } else {
+                const uint32_t at = (slot * X::SLOT + (uint32_t) (x * D + col)) * 4u;
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum), prs, at, 0, SC1);
+                if (col == 0) {
+                    float mx = LOWEST;
 #pragma unroll 4
-                        for (int y = 0; y < WAVES; ++y) mx = fmaxf(mx, sh.m[y][16 * i + x]);
-                        const u32x2 ml = u32x2{(uint32_t) __float_as_int(mx), (uint32_t) __float_as_int(lx)};
-                        __builtin_amdgcn_raw_buffer_store_b64(ml, prs, (slot * X::SLOT + (uint32_t) (ROWS * D + 2 * (16 * i + x))) * 4u, 0, SC1);
-                    }
+                    for (int y = 0; y < WAVES; ++y) mx = fmaxf(mx, sh.m[y][x]);
+                    const u32x2 ml = u32x2{(uint32_t) __float_as_int(mx), (uint32_t) __float_as_int(lx)};
+                    __builtin_amdgcn_raw_buffer_store_b64(ml, prs, (slot * X::SLOT + (uint32_t) (ROWS * D + 2 * x)) * 4u, 0, SC1);
                 }
             }
         }
@@ -389,20 +354,12 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn_decode_kernel(AttnArgs a)
     }
 }
 
-template <class T, int D, int NQ, int WAVES>
-void launch_decode(const AttnArgs& a, hipStream_t s)
-{
-    hipLaunchKernelGGL((attn_decode_kernel<T, D, NQ, WAVES>), dim3(Decode<T, D, NQ, WAVES>::GRID), dim3(64 * WAVES), 0, s, a);
-}
-
 template <class T>
 void launch(const AttnArgs& a, int d, hipStream_t s)
 {
-    // rows of an average request and kv head
-    const int64_t rows = a.requests ? (int64_t) a.tokens * a.group / a.requests : 0;
-    if (d == 64) rows <= 16 ? launch_decode<T, 64, 1, 8>(a, s) : launch_decode<T, 64, 4, 8>(a, s);
-    else if (d == 128) rows <= 16 ? launch_decode<T, 128, 1, 8>(a, s) : launch_decode<T, 128, 2, 8>(a, s);
-    else rows <= 16 ? launch_decode<T, 256, 1, 4>(a, s) : launch_decode<T, 256, 2, 4>(a, s);
+    if (d == 64) hipLaunchKernelGGL((attn_decode_kernel<T, 64, 8>), dim3(Decode<T, 64, 8>::GRID), dim3(512), 0, s, a);
+    else if (d == 128) hipLaunchKernelGGL((attn_decode_kernel<T, 128, 8>), dim3(Decode<T, 128, 8>::GRID), dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((attn_decode_kernel<T, 256, 4>), dim3(Decode<T, 256, 4>::GRID), dim3(256), 0, s, a);
 }
 
 }  // namespace
@@ -443,8 +400,12 @@ extern "C" int exl3_paged_attention(const void* q, int64_t q_ldt, int64_t q_ldh,
                pages, page_size, window, pages ? table_cols * page_size : 0, std::max(std::fabs(scale) * 1.44269504f, 1e-30f), scale < 0.f ? 0x80008000u : 0u, UDiv::of((uint32_t) page_size),
                UDiv::of((uint32_t) (q_heads / kv_heads)), (uint32_t*) workspace,
                reinterpret_cast<float*>((char*) workspace + EXL3_ATTN_COUNTER_BYTES)};
-    // rows of an average request and kv head: from 64 on the products with K and V are what bounds them
-    if (requests && (int64_t) tokens * a.group / requests >= 64) launch_attn_prefill(a, dtype, head_dim, (hipStream_t) stream);
+    // Rows of an average request and kv head: up to 16 are one tile of the decode kernel.  Eight requests of 16000 tokens, 40 heads
+    // over 8 of 128, decode / chunk kernel in us: 100 / 125 at 15 rows, 141 / 125 at 20, 169 / 127 at 40; 24 over 4 of 256:
+    // 105 / 130 at 12, 174 / 129 at 18; 32 over 8 of 64: 46 / 68 at 16, 68 / 69 at 24; two of 2000 tokens: 19 / 29 at 15 rows
+    // of 128, 36 / 29 at 20.  A request of more rows than that among many of fewer takes a tile for each 16: at most as many more
+    // tiles as there are requests.
+    if (requests && (int64_t) tokens * a.group / requests > 16) launch_attn_prefill(a, dtype, head_dim, (hipStream_t) stream);
     else if (dtype == EXL3_FP16) launch<f16>(a, head_dim, (hipStream_t) stream);
     else launch<__bf16>(a, head_dim, (hipStream_t) stream);
     return hipGetLastError() == hipSuccess ? EXL3_OK : EXL3_ELAUNCH;
