@@ -403,7 +403,11 @@ __global__ void __launch_bounds__((Prefill<T, D>::THREADS), (Prefill<T, D>::THRE
             put(std::integral_constant<int, 0>{}, std::integral_constant<int, DT>{}, o, l);
         } else {
             // A part moves as it lies in the registers (a lane's 16 bytes next to its neighbours').  The workgroup that
-            // finds all others' parts written joins them with its own, in the order of the workgroups, and writes none.
+            // finds all others' parts written joins them with its own, in the order of the workgroups, and writes none.  Many
+            // parts of few rows (drafts over a long context) are all written, and every thread of the last workgroup sums some
+            // of the live rows' elements, eight parts in flight: where that takes less than half as many turns of waiting
+            // (1.5 us each) as one part after the other.
+            constexpr int Z = 2, B = 8;                // elements of a thread at once, parts in flight
             const int first_wg = wg - (int) (((uint32_t) off + per - 1u) / per);
             const int last_wg = wg + (int) (((uint32_t) (tile.steps - off - n_steps) + per - 1u) / per);
             const __amdgpu_buffer_rsrc_t prs = __builtin_amdgcn_make_buffer_rsrc(a.part, 0, (int) ATTN_PART_BYTES, RAW_BUFFER_FLAGS);
@@ -412,8 +416,11 @@ __global__ void __launch_bounds__((Prefill<T, D>::THREADS), (Prefill<T, D>::THRE
                 return (2u * (uint32_t) c + (c == first_wg ? 1u : 0u)) * (uint32_t) (X::SLOT * 4) + (uint32_t) wave * (uint32_t) (X::SLOT * 4 / X::WAVES);
             };
             const uint32_t at = 16u * (uint32_t) lane, ml_at = (uint32_t) (QD * DT * 1024) + 8u * (uint32_t) lane;
+            const int live_rows = min(X::ROWS, rows - wk.t * X::ROWS), quads = (live_rows + RW - 1) / RW * (QD * DT * 64);
+            const int turns = (quads + Z * X::THREADS - 1) / (Z * X::THREADS) * ((last_wg - first_wg + B) / B);
+            const bool few = 2 * turns > last_wg - first_wg;
             if (tid == 0) {
-                sh.last = __hip_atomic_load(&a.counters[first_wg], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t) (last_wg - first_wg);
+                sh.last = few && __hip_atomic_load(&a.counters[first_wg], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t) (last_wg - first_wg);
             }
             __syncthreads();
             bool mine = sh.last;
@@ -435,6 +442,61 @@ __global__ void __launch_bounds__((Prefill<T, D>::THREADS), (Prefill<T, D>::THRE
             }
             if (mine) {
                 if (tid == 0) __hip_atomic_store(&a.counters[first_wg], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (!few) {
+                    for (int z0 = tid; z0 < quads; z0 += Z * X::THREADS) {
+                        uint32_t from_wave[Z], at_quad[Z], at_ml[Z];
+                        f32x4 sum[Z];
+                        float top[Z], total[Z];
+#pragma unroll
+                        for (int i = 0; i < Z; ++i) {
+                            const uint32_t z = (uint32_t) min(z0 + i * X::THREADS, quads - 1), w = z / (QD * DT * 64), r = z % (QD * DT * 64);
+                            from_wave[i] = w * (uint32_t) (X::SLOT * 4 / X::WAVES);
+                            at_quad[i] = from_wave[i] + 16u * r;
+                            at_ml[i] = from_wave[i] + (uint32_t) (QD * DT * 1024) + 8u * (r & 63u);
+                            sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                            top[i] = LOWEST;
+                            total[i] = 0.f;
+                        }
+#pragma unroll 1
+                        for (int c0 = first_wg; c0 <= last_wg; c0 += B) {
+                            u32x2 ml[Z][B];
+                            f32x4 v[Z][B];
+#pragma unroll
+                            for (int b = 0; b < B; ++b) {
+                                const uint32_t fr = slot(min(c0 + b, last_wg)) - (uint32_t) wave * (uint32_t) (X::SLOT * 4 / X::WAVES);
+#pragma unroll
+                                for (int i = 0; i < Z; ++i) {
+                                    ml[i][b] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(prs, at_ml[i], fr, SC1));
+                                    v[i][b] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(prs, at_quad[i], fr, SC1));
+                                }
+                            }
+#pragma unroll
+                            for (int i = 0; i < Z; ++i) {
+                                float up = top[i];
+#pragma unroll
+                                for (int b = 0; b < B; ++b) up = fmaxf(up, __int_as_float((int) ml[i][b][0]));
+                                const float f = exp2_fast(top[i] - up);
+                                total[i] *= f;
+                                sum[i] *= f;
+                                top[i] = up;
+#pragma unroll
+                                for (int b = 0; b < B; ++b) {
+                                    const float g = c0 + b <= last_wg ? exp2_fast(__int_as_float((int) ml[i][b][0]) - up) : 0.f;
+                                    total[i] += g * __int_as_float((int) ml[i][b][1]);
+                                    sum[i] += v[i][b] * g;
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < Z; ++i) {
+                            const int z = z0 + i * X::THREADS, w = z / (QD * DT * 64), r = z % (QD * DT * 64), ln = r & 63, x = RW * w + ln % RW;
+                            if (z >= quads || x >= live_rows) continue;
+                            const int y = wk.t * X::ROWS + x, tk = (int) a.d_group.div((uint32_t) y);
+                            store_out<T>(as_global(a.out) + (int64_t) (wk.tok0 + tk) * a.o_ldt + (int64_t) (wk.h * a.group + y - tk * a.group) * a.o_ldh +
+                                             X::col_of(r / 64 / QD, r / 64 % QD) + 4 * (ln / RW), sum[i], total[i]);
+                        }
+                    }
+                } else {
                 // 64 registers of the output at a time: more would not fit beside the workgroup's own
                 constexpr int N = DT * AE < 64 ? DT : 64 / AE;
                 static_for(std::make_integer_sequence<int, DT / N>{}, [&](auto P) __attribute__((always_inline)) {
@@ -473,6 +535,7 @@ __global__ void __launch_bounds__((Prefill<T, D>::THREADS), (Prefill<T, D>::THRE
                     }
                     put(std::integral_constant<int, N * P>{}, std::integral_constant<int, N>{}, sum, total);
                 });
+                }
             }
         }
         __syncthreads();
