@@ -14,7 +14,6 @@ template <> struct Elem<f16> { typedef f16x8 x8; };
 template <> struct Elem<__bf16> { typedef bf16x8 x8; };
 
 enum { ROPE_HALF, ROPE_PAIRS, ROPE_ANY };
-constexpr int ROPE_GROUP = 4;                           // most tokens of a rotary workgroup
 
 inline bool paged_head_dim(int d) { return d == 64 || d == 128 || d == 256; }
 inline bool paged_dtype(int t) { return t == EXL3_FP16 || t == EXL3_BF16; }

@@ -39,8 +39,8 @@ __device__ __forceinline__ void here(u32x4& a, u32x4& b, float& c)
 // 16 bytes (16 keys' reads of one piece), V's by 64 (4 keys' 64 bytes) or, for 16 rows a wave, 32 (16 keys' 32 bytes);
 // padded rows, unlike permuted ones, let one address register and the instructions' offsets reach a whole step: at 128
 // columns the registers are all taken (output 64, Q 32, scores 32, K and V on the way 32).
-// 2048 tokens over 14000 (40 heads over 8 of 128): 809 us, 780 TFLOPS (a large library product takes 1160 to 1220); a
-// 2048-token prompt 100 us; 8 x 4 tokens over 1000 to 32000 (24 over 4 of 256) 84 us, 3.0 TB/s of K and V.
+// 2048 tokens over 14000 (40 heads over 8 of 128): 809 to 828 us, 760 to 780 TFLOPS (a large library product takes 1160 to 1220); a
+// 2048-token prompt 101 us; 8 x 4 tokens over 1000 to 32000 (24 over 4 of 256) 83 us, 3.0 TB/s of K and V.
 template <class T, int D>
 struct Prefill {
     static constexpr int RW = D == 256 ? 16 : 32;       // rows of a wave

@@ -119,9 +119,8 @@ struct RopeArgs {
     float mscale;
     int tokens, hq, hkv, rot, page;
     int64_t cache_slots;
-    int group;                                          // tokens of a workgroup
     int items;                                          // 8-element pieces of a token: (hq + 2 hkv) D / 8
-    UDiv d_page, d_items;
+    UDiv d_page;
 };
 
 // 8 elements of a head from column c on, rotated.  x: those elements; other: the elements they pair with (half
@@ -167,31 +166,27 @@ __device__ __forceinline__ u32x4 rotate8(u32x4 xb, const uint16_t* head, int c, 
 
 // theta = position x frequency is reduced to a fraction of a turn before it is rounded to 32 bits, so a position of a
 // million turns as exactly as position 0 (32-bit angles are 0.06 off there).  A workgroup forms the cosines and sines of
-// its tokens once, in LDS, and uses them for every head; k goes straight to its cache slot.  Bound by memory: 8192 tokens
-// of 40 + 8 heads of 128 in 49.9 us (235 MB, 4.7 TB/s; a large copy takes 4.6), 32 tokens in 3.0.
+// its token once, in LDS, and uses them for every head; k goes straight to its cache slot.  Bound by memory: 8192 tokens
+// of 40 + 8 heads of 128 in 47.2 us (235 MB, 5.0 TB/s; a large copy takes 4.6), 32 tokens in 3.1.
 template <class T, int D, int LAYOUT>
 __global__ void __launch_bounds__(256) rope_kv_write_kernel(RopeArgs a)
 {
-    __shared__ float2 cs[ROPE_GROUP * D / 2];
-    const int t0 = (int) blockIdx.x * a.group, n_tok = min(a.group, a.tokens - t0), half = a.rot / 2;
-    for (int i = threadIdx.x; i < n_tok * half; i += 256) {
-        const int t = i / half, f = i - t * half;
+    __shared__ float2 cs[D / 2];
+    const int64_t tok = blockIdx.x;
+    for (int f = threadIdx.x; f < a.rot / 2; f += 256) {
         float s, c;
-        sincospif(2.f * turn_fraction((double) a.pos[t0 + t], a.inv_freq[f]), &s, &c);
-        cs[t * half + f] = make_float2(c * a.mscale, s * a.mscale);
+        sincospif(2.f * turn_fraction((double) a.pos[tok], a.inv_freq[f]), &s, &c);
+        cs[f] = make_float2(c * a.mscale, s * a.mscale);
     }
     __syncthreads();
     constexpr int PIECES = D / 8;
-    const int all = n_tok * a.items, step = 256 * (int) gridDim.y;
-    for (int i = (int) blockIdx.y * 256 + (int) threadIdx.x; i < all; i += step) {
-        const int t = (int) a.d_items.div((uint32_t) i), item = i - t * a.items;
-        int h = item / PIECES;
-        const int c = 8 * (item % PIECES);
-        const int64_t tok = t0 + t;
+    for (int i = (int) blockIdx.y * 256 + (int) threadIdx.x; i < a.items; i += 256 * (int) gridDim.y) {
+        int h = i / PIECES;
+        const int c = 8 * (i % PIECES);
         if (h < a.hq) {
             const uint16_t* head = a.q + tok * a.q_ldt + h * a.q_ldh;
             const u32x4 x = *reinterpret_cast<gc_u32x4*>(as_global(head) + c);
-            *reinterpret_cast<g_u32x4*>(as_global(a.out) + (tok * a.hq + h) * D + c) = rotate8<T, LAYOUT>(x, head, c, a.rot, cs + t * half);
+            *reinterpret_cast<g_u32x4*>(as_global(a.out) + (tok * a.hq + h) * D + c) = rotate8<T, LAYOUT>(x, head, c, a.rot, cs);
             continue;
         }
         const int64_t slot = a.slots[tok];
@@ -202,7 +197,7 @@ __global__ void __launch_bounds__(256) rope_kv_write_kernel(RopeArgs a)
             const uint16_t* head = a.k + tok * a.k_ldt + h * a.k_ldh;
             const u32x4 x = *reinterpret_cast<gc_u32x4*>(as_global(head) + c);
             *reinterpret_cast<g_u32x4*>(as_global(a.kc) + page * a.kc_ldp + off * a.kc_ldt + h * a.kc_ldh + c) =
-                rotate8<T, LAYOUT>(x, head, c, a.rot, cs + t * half);
+                rotate8<T, LAYOUT>(x, head, c, a.rot, cs);
         } else {
             h -= a.hkv;
             const u32x4 x = *reinterpret_cast<gc_u32x4*>(as_global(a.v) + tok * a.v_ldt + h * a.v_ldh + c);
@@ -262,14 +257,14 @@ extern "C" int exl3_rope_kv_write(const void* q, int64_t q_ldt, int64_t q_ldh, c
         return EXL3_EINVAL;
     RopeArgs a{(const uint16_t*) q, (const uint16_t*) k, (const uint16_t*) v, q_ldt, q_ldh, k_ldt, k_ldh, v_ldt, v_ldh, positions, slots,
                (uint16_t*) q_out, (uint16_t*) k_cache, (uint16_t*) v_cache, kc_ldp, kc_ldt, kc_ldh, vc_ldp, vc_ldt, vc_ldh, inv_freq, mscale,
-               tokens, q_heads, kv_heads, rot_dim, page_size, (int64_t) pages * page_size, 1, (q_heads + 2 * kv_heads) * (head_dim / 8),
-               UDiv::of((uint32_t) page_size), UDiv{}};
-    a.d_items = UDiv::of((uint32_t) a.items);
+               tokens, q_heads, kv_heads, rot_dim, page_size, (int64_t) pages * page_size, (q_heads + 2 * kv_heads) * (head_dim / 8),
+               UDiv::of((uint32_t) page_size)};
     // a vector piece of 8 pairs with one other piece where half the rotated part is a multiple of 8
     const int layout = interleaved ? ROPE_PAIRS : rot_dim % 16 == 0 ? ROPE_HALF : ROPE_ANY;
-    // few tokens: a token's pieces over several workgroups, so that the heads' loads go out together
-    a.group = tokens >= 2048 ? ROPE_GROUP : 1;
-    const dim3 grid((unsigned) ((tokens + a.group - 1) / a.group), tokens <= 512 ? (unsigned) std::min(64, (a.items + 255) / 256) : 1u);
+    // Few tokens: a token's pieces over several workgroups, so that all heads' loads go out together (32 tokens 3.1 us, one
+    // workgroup a token 4.0); many fill the GPU without, and forming the angles once is cheaper (8192 tokens 39.6 us, several
+    // workgroups a token 41.3).
+    const dim3 grid((unsigned) tokens, tokens <= 512 ? (unsigned) std::min(64, (a.items + 255) / 256) : 1u);
     hipStream_t s = (hipStream_t) stream;
     if (dtype == EXL3_FP16) {
         if (head_dim == 64) launch_rope<f16, 64>(a, layout, grid, s);

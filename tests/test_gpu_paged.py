@@ -353,6 +353,27 @@ def test_long_context_is_split_and_joined():
     Batch([(40000, 100)], 4, 1, 128, F16).check()
 
 
+def test_one_kv_head_and_one_head():
+    for hq, hkv in ((64, 1), (40, 1), (1, 1)):
+        Batch([(700, 1), (33, 2), (0, 1)], hq, hkv, 128, F16, seed=hq).check()
+        Batch([(300, 50), (0, 7)], hq, hkv, 64, BF16, seed=hq).check(window=90)
+
+
+def test_strides_that_address_nothing():
+    """One token, one head, one page: torch leaves such strides at anything."""
+    b = Batch([(9, 1)], 1, 1, 64, F16, extra_pages=0)
+    want = b.check()
+    odd = lambda t, shape, strides: t.as_strided(shape, strides)  # noqa: E731
+    b.q = odd(b.q, (1, 1, 64), (3, 5, 1))
+    b.kc, b.vc = (odd(c, (1, 16, 1, 64), (7, c.stride(1), 9, 1)) for c in (b.kc, b.vc))
+    b.table = odd(b.table, (1, b.table.shape[1]), (1, 1))
+    assert torch.equal(b.run(), want)
+    f, _ = paged.rope_frequencies(64)
+    k = torch.randn(1, 1, 64, device="cuda").half()
+    q = paged.rope_kv_write(odd(k, (1, 1, 64), (3, 5, 1)), odd(k, (1, 1, 64), (11, 1, 1)), k, ints([0], torch.int64), ints([3], torch.int64), b.kc, b.vc, f)
+    assert torch.equal(q, k) and torch.equal(b.kc[0, 3], k[0]) and torch.equal(b.vc[0, 3], k[0])
+
+
 def test_large_scores():
     """Scores of hundreds: the running maximum carries them; keys far below it vanish."""
     Batch([(1000, 1), (700, 3), (0, 200)], 10, 2, 128, F16, q_scale=60.0).check()
