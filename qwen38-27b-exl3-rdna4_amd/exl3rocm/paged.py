@@ -69,8 +69,7 @@ def rope_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[dict
 
 
 # An eager call's host time is what bounds a decode step's small launches, so the checks below read each attribute
-# once (get_device is half the time of device), a step's outputs are cut from one allocation, and the library's
-# entry points are looked up once.
+# once (get_device is half the time of device), and the library's entry points are looked up once.
 _fn: dict = {}
 
 
@@ -122,14 +121,14 @@ def batch_plan(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torc
     cols, ld = _table("batch_plan", block_table, gpu, R)
     _need(page_size >= 1 and num_tokens >= 0, "batch_plan: page_size from 1, num_tokens from 0")
     dev = ctx_lens.device
-    ints = torch.empty(2 * R + 2, dtype=i32, device=dev)
-    tok = torch.empty((2, num_tokens), dtype=torch.int64, device=dev)
-    p, t = ints.data_ptr(), tok.data_ptr()
+    # an allocation each: slices of one would share storage, against the schema, and start where compiled code, which takes
+    # an op's outputs for aligned to 16 bytes, cannot read them
+    cu_q, seq, left = (torch.empty(n, dtype=i32, device=dev) for n in (R + 1, R, 1))
+    pos, slots = (torch.empty(num_tokens, dtype=torch.int64, device=dev) for _ in range(2))
     L.check(_entry("exl3_batch_plan")(ctx_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), ld, cols, free_pages.data_ptr(),
-                                      free_pages.numel(), free_count.data_ptr(), p, p + 4 * (R + 1), t, t + 8 * num_tokens,
-                                      p + 4 * (2 * R + 1), R, page_size, num_tokens, _raw_stream(gpu)), "batch_plan")
-    cu_q, seq, left = ints.split((R + 1, R, 1))
-    pos, slots = tok.unbind()
+                                      free_pages.numel(), free_count.data_ptr(), cu_q.data_ptr(), seq.data_ptr(),
+                                      pos.data_ptr(), slots.data_ptr(), left.data_ptr(), R, page_size, num_tokens, _raw_stream(gpu)),
+            "batch_plan")
     return cu_q, seq, pos, slots, left
 
 
