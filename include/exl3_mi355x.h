@@ -351,7 +351,7 @@ int exl3_gemv_mr_noalloc(const void* x, int64_t ldx, const void* trellis, void* 
 #define EXL3_ATTN_COUNTER_BYTES 2048
 
 /* One step's bookkeeping from the requests' lengths.  Request r holds ctx_lens[r] tokens in the cache and adds
- * new_lens[r] (negative lengths count as 0; all lengths together stay below 2^31):
+ * new_lens[r] (negative lengths count as 0; a request's length and the batch's counts stop at 2^31 - 1):
  *   cu_q[requests + 1]   its new tokens are [cu_q[r], cu_q[r + 1])
  *   seq_lens[requests]   ctx_lens + new_lens
  *   positions[tokens], slots[tokens]  of every new token; slot -1 where it has no page (stack or table row too

@@ -9,13 +9,17 @@ namespace {
 
 constexpr int PLAN_TOKENS = 2048;                      // tokens of one request that a workgroup writes
 
+// Counts come from the caller's GPU memory, where nothing has checked them: sums stop at 2^31 - 1 instead of passing it, in
+// any order alike, so no index formed from them is negative.
+__device__ __forceinline__ int add_count(int a, int b) { return (int) min((uint32_t) a + (uint32_t) b, (uint32_t) INT32_MAX); }
+
 // sum over the workgroup's 256 threads of two counts
 __device__ __forceinline__ int2 block_sum2(int a, int b, int* lds)
 {
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
-        a += __shfl_xor(a, m);
-        b += __shfl_xor(b, m);
+        a = add_count(a, __shfl_xor(a, m));
+        b = add_count(b, __shfl_xor(b, m));
     }
     const int wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0) {
@@ -23,7 +27,7 @@ __device__ __forceinline__ int2 block_sum2(int a, int b, int* lds)
         lds[2 * wave + 1] = b;
     }
     __syncthreads();
-    return make_int2(lds[0] + lds[2] + lds[4] + lds[6], lds[1] + lds[3] + lds[5] + lds[7]);
+    return make_int2(add_count(add_count(lds[0], lds[2]), add_count(lds[4], lds[6])), add_count(add_count(lds[1], lds[3]), add_count(lds[5], lds[7])));
 }
 
 struct PlanArgs {
@@ -54,7 +58,7 @@ __global__ void __launch_bounds__(256) batch_plan_kernel(PlanArgs a)
     const int r = blockIdx.x, t0 = (int) blockIdx.y * PLAN_TOKENS;
     const bool tail = r == a.requests;
     const int ctx = tail ? 0 : max(a.ctx[r], 0);
-    int add = tail ? 0 : max(a.add[r], 0);
+    int add = tail ? 0 : min(max(a.add[r], 0), INT32_MAX - ctx);
     if (!tail && t0 > 0 && t0 >= add) return;
     const int count = min(a.free_count[0], a.n_free);
     auto pages = [&](int tokens) __attribute__((always_inline)) {   // columns of the table that `tokens` fill
@@ -62,36 +66,35 @@ __global__ void __launch_bounds__(256) batch_plan_kernel(PlanArgs a)
     };
     int before = 0, taken = 0;
     for (int s = threadIdx.x; s < r; s += 256) {
-        const int c = max(a.ctx[s], 0), n = max(a.add[s], 0);
-        before += n;
-        taken += n ? pages(c + n) - pages(c) : 0;
+        const int c = max(a.ctx[s], 0), n = min(max(a.add[s], 0), INT32_MAX - c);
+        before = add_count(before, n);
+        taken = add_count(taken, n ? pages(c + n) - pages(c) : 0);
     }
     const int2 sums = block_sum2(before, taken, lds);
-    const int first = sums.x, had = pages(ctx), need = add ? pages(ctx + add) - had : 0, top = count - 1 - sums.y;
+    const int first = sums.x, had = pages(ctx), need = add ? pages(ctx + add) - had : 0, top = max(count, 0) - 1 - sums.y;
     if (t0 == 0) {
         if (threadIdx.x == 0) {
             a.cu_q[r] = first;
-            if (tail) a.left[0] = count - sums.y;
+            if (tail) a.left[0] = (int) max((int64_t) count - sums.y, (int64_t) INT32_MIN);
             else a.seq[r] = ctx + add;
         }
         for (int j = threadIdx.x; j < need; j += 256)
-            a.table[(int64_t) r * a.ld_table + had + j] = top - j >= 0 ? a.free_pages[top - j] : -1;
+            a.table[(int64_t) r * a.ld_table + had + j] = j <= top ? a.free_pages[top - j] : -1;
     }
     if (tail) {
-        for (int t = first + t0 + (int) threadIdx.x; t < min(a.tokens, first + t0 + PLAN_TOKENS); t += 256) {
-            a.pos[t] = 0;
-            a.slots[t] = -1;
+        for (int i = t0 + (int) threadIdx.x; i < min(a.tokens - first, t0 + PLAN_TOKENS); i += 256) {
+            a.pos[first + i] = 0;
+            a.slots[first + i] = -1;
         }
         return;
     }
     add = min(add, t0 + PLAN_TOKENS);
     for (int i = t0 + (int) threadIdx.x; i < add; i += 256) {
-        const int t = first + i;
-        if (t < 0 || t >= a.tokens) break;
-        const int p = ctx + i, col = (int) a.d_page.div((uint32_t) p);
+        if (i >= a.tokens - first) break;
+        const int t = first + i, p = ctx + i, col = (int) a.d_page.div((uint32_t) p);
         int page = -1;
         if (col < had) page = a.table[(int64_t) r * a.ld_table + col];
-        else if (col < a.cols && top - (col - had) >= 0) page = a.free_pages[top - (col - had)];
+        else if (col < a.cols && col - had <= top) page = a.free_pages[top - (col - had)];
         a.pos[t] = p;
         a.slots[t] = page < 0 ? -1 : (int64_t) page * a.page + (p - col * a.page);
     }
