@@ -31,6 +31,19 @@ def new_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=to
     return tuple(torch.zeros(pages, kv_heads, page_size, head_dim, dtype=dtype, device=device).transpose(1, 2) for _ in range(2))
 
 
+# what rope_frequencies reads of each kind's `rope_scaling`
+_ROPE_KEYS = {
+    "default": (),
+    "linear": ("factor",),
+    "yarn": ("factor", "original_max_position_embeddings", "attention_factor", "mscale", "mscale_all_dim", "beta_fast", "beta_slow", "truncate"),
+    "llama3": ("factor", "original_max_position_embeddings", "low_freq_factor", "high_freq_factor"),
+}
+# what lies beside it and changes nothing here: names, what the caller gives elsewhere (base, rot_dim), what a kind does
+# not use, and the sections of a position of several coordinates, which agree where a token has one position
+_ROPE_BESIDE = ("rope_type", "type", "rope_theta", "partial_rotary_factor", "original_max_position_embeddings", "finetuned",
+                "mrope_section", "mrope_interleaved")
+
+
 def rope_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[dict] = None, device="cuda") -> Tuple[torch.Tensor, float]:
     """(inv_freq, mscale) for rope_kv_write: radians a position adds to each of the rot_dim / 2 pairs (float64), and the
     factor on cosine and sine.  scaling (the keys of a model's `rope_scaling`):
@@ -38,33 +51,47 @@ def rope_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[dict
       "linear"   every frequency divided by factor
       "yarn"     divided by factor where a pair makes fewer than beta_slow (1) turns in
                  original_max_position_embeddings tokens, kept above beta_fast (32), a ramp over the pair's index
-                 between; mscale = attention_factor, or 0.1 ln(factor) + 1
+                 between, whose ends are whole pairs unless truncate is False; mscale = attention_factor, or
+                 0.1 ln(factor) + 1, or with mscale and mscale_all_dim the quotient (0.1 mscale ln(factor) + 1) /
+                 (0.1 mscale_all_dim ln(factor) + 1): such a model also scales its scores, which is paged_attention's `scale`
       "llama3"   divided by factor where its wavelength exceeds original / low_freq_factor, kept below original /
-                 high_freq_factor, blended between"""
+                 high_freq_factor, blended between
+    A key that is None counts as absent; one that would change the result and is not read here is refused."""
     _need(rot_dim >= 2 and rot_dim % 2 == 0, f"rope_frequencies: rot_dim must be even, got {rot_dim}")
     _need(base > 1, f"rope_frequencies: base must be above 1, got {base}")
     i = torch.arange(rot_dim // 2, dtype=torch.float64)
     f = base ** (-2.0 * i / rot_dim)
-    s = scaling or {}
+    s = {key: v for key, v in (scaling or {}).items() if v is not None}
     kind, mscale = s.get("rope_type", s.get("type", "default")), 1.0
+    _need(kind in _ROPE_KEYS, f"rope_frequencies: unknown rope_type {kind!r}")
+    unread = sorted(set(s) - set(_ROPE_KEYS[kind]) - set(_ROPE_BESIDE))
+    _need(not unread, f"rope_frequencies: rope_type {kind!r} with keys that are not read: {', '.join(unread)}")
+    _need(s.get("rope_theta", base) == base, f"rope_frequencies: base is {base}, rope_theta {s.get('rope_theta')}")
     if kind == "linear":
         f = f / s["factor"]
     elif kind == "yarn":
         factor, orig = float(s["factor"]), float(s["original_max_position_embeddings"])
         # the pair index that makes b turns in the original context
         at = lambda b: rot_dim * math.log(orig / (2 * math.pi * b)) / (2 * math.log(base))  # noqa: E731
-        low = max(math.floor(at(s.get("beta_fast", 32))), 0)
-        high = min(math.ceil(at(s.get("beta_slow", 1))), rot_dim - 1)
+        low, high = at(s.get("beta_fast", 32)), at(s.get("beta_slow", 1))
+        if s.get("truncate", True):
+            low, high = math.floor(low), math.ceil(high)
+        low, high = max(low, 0), min(high, rot_dim - 1)
         slow = ((i - low) / max(high - low, 1e-3)).clamp(0, 1)
         f = f / factor * slow + f * (1 - slow)
-        mscale = float(s.get("attention_factor") or (0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0))
+        grown = lambda m: 0.1 * m * math.log(factor) + 1.0 if factor > 1 else 1.0  # noqa: E731
+        _need(("mscale" in s) == ("mscale_all_dim" in s), "rope_frequencies: mscale and mscale_all_dim go together")
+        if "attention_factor" in s:
+            mscale = float(s["attention_factor"])
+        elif "mscale" in s:
+            mscale = grown(s["mscale"]) / grown(s["mscale_all_dim"])
+        else:
+            mscale = grown(1.0)
     elif kind == "llama3":
         lo, hi = s["low_freq_factor"], s["high_freq_factor"]
         turns = s["original_max_position_embeddings"] * f / (2 * math.pi)
         keep = ((turns - lo) / (hi - lo)).clamp(0, 1)
         f = f * keep + f / s["factor"] * (1 - keep)
-    else:
-        _need(kind == "default", f"rope_frequencies: unknown rope_type {kind!r}")
     return f.to(device), mscale
 
 
