@@ -20,7 +20,6 @@ import torch
 from . import _lib as L
 from .kernels import _need
 
-_raw_stream = torch._C._cuda_getCurrentRawStream      # the current stream's handle on a GPU
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 HEAD_DIMS = (64, 128, 256)
 
@@ -105,6 +104,11 @@ def _entry(name: str):
     if f is None:
         f = _fn[name] = getattr(L.lib(), name)
     return f
+
+
+def _raw_stream(gpu: int) -> int:
+    """The current stream's handle on a GPU (looked up at the call: a torch without a GPU backend has no such function)."""
+    return torch._C._cuda_getCurrentRawStream(gpu)
 
 
 def _ints(name: str, t: torch.Tensor, gpu: int, dtype, numel: Optional[int] = None):
