@@ -50,18 +50,23 @@ class AttentionBlock:
 class Requests:
     """A server's state on the GPU: lengths, block tables, free pages."""
 
-    def __init__(self, count, pages, page_size, max_tokens):
+    def __init__(self, count, pages, page_size, max_tokens, device="cuda"):
         self.page_size = page_size
-        self.lens = torch.zeros(count, dtype=torch.int32, device="cuda")
-        self.table = torch.full((count, -(-max_tokens // page_size)), -1, dtype=torch.int32, device="cuda")
-        self.free = torch.arange(pages, dtype=torch.int32, device="cuda")
-        self.free_count = torch.full((1,), pages, dtype=torch.int32, device="cuda")
+        self.lens = torch.zeros(count, dtype=torch.int32, device=device)
+        self.table = torch.full((count, -(-max_tokens // page_size)), -1, dtype=torch.int32, device=device)
+        self.free = torch.arange(pages, dtype=torch.int32, device=device)
+        self.free_count = torch.full((1,), pages, dtype=torch.int32, device=device)
+        self.missing = torch.zeros(1, dtype=torch.int32, device=device)    # pages that the last step lacked
 
     def step(self, new_lens, num_tokens):
-        """The plan of a step that adds new_lens tokens; the state moves on."""
+        """The plan of a step that adds new_lens tokens; the state moves on if every token has its page.  Otherwise it stays as it
+        was and the step's outputs mean nothing: `missing` says so, to be read with the step's tokens; the server then
+        releases a request (or leaves some out) and makes the step again."""
         plan = torch.ops.exl3rocm.batch_plan(self.lens, new_lens, self.table, self.free, self.free_count, self.page_size, num_tokens)
-        self.lens.copy_(plan[1])
-        self.free_count.copy_(plan[4])
+        fits = plan[4] >= 0
+        self.lens.copy_(torch.where(fits, plan[1], self.lens))
+        self.free_count.copy_(torch.where(fits, plan[4], self.free_count))
+        self.missing.copy_((-plan[4]).clamp_min(0))
         return plan
 
     def release(self, request):
@@ -85,6 +90,7 @@ def main():
     x = torch.randn(total, 5120, device="cuda", generator=g).half()
     plan = reqs.step(torch.tensor(a.prompts, dtype=torch.int32, device="cuda"), total)
     y = block(x, plan, reqs.table)
+    assert int(reqs.missing) == 0, "the cache is too small for these prompts"
     print(f"prefilled {total} tokens of {R} requests: output {tuple(y.shape)}, rms {y.float().square().mean().sqrt().item():.3f}")
 
     ones = torch.ones(R, dtype=torch.int32, device="cuda")
@@ -102,6 +108,7 @@ def main():
     for _ in range(a.steps):
         graph.replay()
     torch.cuda.synchronize()
+    assert int(reqs.missing) == 0, "the cache ran out of pages"
     print(f"decode step of {R} requests, one captured graph: {(time.perf_counter() - t) / a.steps * 1e6:.1f} us; lengths now {reqs.lens.tolist()}")
     reqs.release(0)
     print(f"free pages after the first request left: {int(reqs.free_count)}")

@@ -142,7 +142,8 @@ def batch_plan(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torc
     num_tokens: rows of the step's batch; rows past the last request get position 0 and slot -1, as a batch
     padded for a captured graph has them.  free_left [1] is the next free_count; negative: that many pages were missing,
     and the tokens without one have slot -1 (nothing is written for them).  The stack and its count are only read:
-    a repeated call gives the same result."""
+    a repeated call gives the same result, and a step that lacks pages is undone by keeping ctx_lens and free_count as they
+    were.  It is not to be kept: a later plan counts the pages of ctx_lens as held and never fills them in."""
     gpu, i32 = _gpu(ctx_lens, "batch_plan"), torch.int32
     R = ctx_lens.numel()
     _ints("batch_plan: ctx_lens", ctx_lens, gpu, i32)
