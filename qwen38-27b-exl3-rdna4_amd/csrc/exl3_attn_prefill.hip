@@ -37,10 +37,11 @@ __device__ __forceinline__ void here(u32x4& a, u32x4& b, float& c)
 // layout): 32 rows' outputs and Q alone would be 192 registers, one wave a SIMD, with nothing to run beside its waits.
 // A lane's row is the same in S^T and O^T, as in the decode kernel.  LDS rows are padded so that no bank is met twice: K's by
 // 16 bytes (16 keys' reads of one piece), V's by 64 (4 keys' 64 bytes) or, for 16 rows a wave, 32 (16 keys' 32 bytes);
-// padded rows, unlike permuted ones, let one address register and the instructions' offsets reach a whole step: at 128
-// columns the registers are all taken (output 64, Q 32, scores 32, K and V on the way 32).
-// 2048 tokens over 14000 (40 heads over 8 of 128): 809 to 828 us, 760 to 780 TFLOPS (a large library product takes 1160 to 1220); a
-// 2048-token prompt 101 us; 8 x 4 tokens over 1000 to 32000 (24 over 4 of 256) 83 us, 3.0 TB/s of K and V.
+// padded rows, unlike permuted ones, let one address register and the instructions' offsets reach a whole step, and the two
+// buffers are two copies of the loop's body for the same reason: at 128 columns the registers are all taken (output 64,
+// Q 32, scores 32, K and V on the way 32).  One copy, the buffer a register, takes 1 to 1.5 % longer over long contexts.
+// 2048 tokens over 14000 (40 heads over 8 of 128): 805 to 831 us, 755 to 780 TFLOPS (a large library product takes 1160 to 1220); a
+// 2048-token prompt 100 us; 8 x 4 tokens over 1000 to 32000 (24 over 4 of 256) 83 us, 3.0 TB/s of K and V.
 template <class T, int D>
 struct Prefill {
     static constexpr int RW = D == 256 ? 16 : 32;       // rows of a wave
@@ -60,7 +61,6 @@ struct Prefill {
     static constexpr int NB = AE * TH / 8;              // operands of its probabilities
     using Acc = std::conditional_t<RW == 32, f32x16, f32x4>;
     static constexpr float SHIFT = std::is_same_v<T, f16> ? 8.f : 0.f;   // fp16 probabilities are held times 2^8
-    static constexpr int K_BUF = 2 * KEYS * (D + 8), V_BUF = 2 * KEYS * (RW == 32 ? D + 32 : D + 16);   // bytes of a buffer
     static constexpr int K_LD = D + 8, V_LD = RW == 32 ? D + 32 : D + 16;  // LDS rows, halves
 
     struct alignas(16) Shared {
@@ -178,13 +178,12 @@ __global__ void __launch_bounds__((Prefill<T, D>::THREADS), (Prefill<T, D>::THRE
                 vr[i] = *reinterpret_cast<gc_u32x4*>(vp + (int64_t) (128 / CH * i) * a.v_ldt + v_lane);
             }
         };
-        auto store = [&](int buf, int s, int p) __attribute__((always_inline)) {
+        auto store = [&](auto BUF, int s, int p) __attribute__((always_inline)) {
             const int key0 = X::KEYS * s + KW * wave;
             // whether every row of the tile sees these keys; if not, V of keys that no row sees may hold anything and is
             // zeroed, and so are infinities and NaN, which a probability of 0 does not hide from the rows that do not see them
             const bool seen = p >= 0 && key0 + KW - 1 <= wk.pos0 + tile.first && (!a.window || key0 > wk.pos0 + tile.last - a.window) && key0 + KW <= a.cap;
-            lchar* const kw = k_put + buf * X::K_BUF;
-            lchar* const vw = v_put + buf * X::V_BUF;
+            constexpr int buf = BUF;
             int flags = p >= 0 ? 1 : 0;
             if (!seen) {
                 uint32_t f = 0;
@@ -203,14 +202,13 @@ __global__ void __launch_bounds__((Prefill<T, D>::THREADS), (Prefill<T, D>::THRE
             }
 #pragma unroll
             for (int i = 0; i < LI; ++i) {
-                *reinterpret_cast<lu32x4*>(kw + 2 * (64 / CH * i) * X::K_LD) = kr[i];
-                *reinterpret_cast<lu32x4*>(vw + 2 * (64 / CH * i) * X::V_LD) = vr[i];
+                *reinterpret_cast<lu32x4*>(k_put + 2 * (buf * X::KEYS + 64 / CH * i) * X::K_LD) = kr[i];
+                *reinterpret_cast<lu32x4*>(v_put + 2 * (buf * X::KEYS + 64 / CH * i) * X::V_LD) = vr[i];
             }
             if (lane == 0) sh.page[buf][wave] = flags;
         };
-        auto compute = [&](int buf, int s) __attribute__((always_inline)) {
-            lchar* const kg = k_get + buf * X::K_BUF;
-            lchar* const vg = v_get + buf * X::V_BUF;
+        auto compute = [&](auto BUF, int s) __attribute__((always_inline)) {
+            constexpr int buf = BUF;
             const int k0 = X::KEYS * s;
             // nothing for this wave's rows in the step
             if (!rows_here || k0 > w_last || (a.window && k0 + X::KEYS - 1 <= w_first - a.window)) return;
@@ -231,7 +229,7 @@ __global__ void __launch_bounds__((Prefill<T, D>::THREADS), (Prefill<T, D>::THRE
                 for (int t = 0; t < TH; ++t)
 #pragma unroll
                     for (int c = 0; c < KS; ++c)
-                        kf[t][c] = *reinterpret_cast<lu32x4*>(kg + 2 * ((32 * y + RW * t) * X::K_LD + X::KD * c));
+                        kf[t][c] = *reinterpret_cast<lu32x4*>(k_get + 2 * ((buf * X::KEYS + 32 * y + RW * t) * X::K_LD + X::KD * c));
             };
             auto read_v = [&](u32x4 (&f)[NB], int y, int d) __attribute__((always_inline)) {
 #pragma unroll
@@ -239,7 +237,7 @@ __global__ void __launch_bounds__((Prefill<T, D>::THREADS), (Prefill<T, D>::THRE
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (__attribute__((address_space(3))) s16x4*) (vg + 2 * ((32 * y + X::key_of(8 * b + 4 * x)) * X::V_LD + RW * d))));
+                            (__attribute__((address_space(3))) s16x4*) (v_get + 2 * ((buf * X::KEYS + 32 * y + X::key_of(8 * b + 4 * x)) * X::V_LD + RW * d))));
                         f[b][2 * x] = w[0];
                         f[b][2 * x + 1] = w[1];
                     }
@@ -371,20 +369,21 @@ __global__ void __launch_bounds__((Prefill<T, D>::THREADS), (Prefill<T, D>::THRE
         if (tile.lo < tile.hi) {
             int p0 = page_of(s0), p1 = page_of(s0 + 1), p2 = page_of(s0 + 2);
             request(s0, p0);
-            store(0, s0, p0);
+            store(std::integral_constant<int, 0>{}, s0, p0);
             if (s0 + 1 < s1) request(s0 + 1, p1);
             __syncthreads();
-            int buf = 0;
-            for (int s = s0;; ++s) {
-                compute(buf, s);
-                if (s + 1 == s1) break;
-                buf ^= 1;
-                store(buf, s + 1, p1);
+            // step s from one buffer, with step s + 1 into the other; false: it was the last
+            auto turn = [&](auto BUF, int s) __attribute__((always_inline)) {
+                compute(BUF, s);
+                if (s + 1 == s1) return false;
+                store(std::integral_constant<int, 1 - BUF>{}, s + 1, p1);
                 p1 = p2;
                 p2 = page_of(s + 3);
                 if (s + 2 < s1) request(s + 2, p1);
                 __syncthreads();
-            }
+                return true;
+            };
+            for (int s = s0; turn(std::integral_constant<int, 0>{}, s) && turn(std::integral_constant<int, 1>{}, s + 1); s += 2) {}
         }
 
         // a wave's 32 rows, or their part
