@@ -37,7 +37,11 @@ struct Decode {
     static constexpr int GRID = 256;                    // workgroups: one a CU
     static constexpr int SLOT = attn_slot(ROWS, D);
     static_assert(GRID <= ATTN_COUNTERS && (size_t) 2 * GRID * SLOT * 4 <= ATTN_PART_BYTES);
-    // fp16 probabilities are held times 2^8: the smallest that a key keeps is then 2^-33 of its row's largest
+    // Probabilities are rounded to the element type for their product with V, after the 32-bit sum has taken them as they are:
+    // the matrix unit's operands have 16 bits, and a second product for what the rounding cuts off would double those with V.
+    // The output's error against 64 bits grows by 4 to 11 % in fp16 and 8 to 18 % in bf16 over 32-bit probabilities, most of it
+    // being the output's own rounding.  fp16 ones are held times 2^8: the smallest that a key keeps is then 2^-33 of its
+    // row's largest.
     static constexpr float SHIFT = std::is_same_v<T, f16> ? 8.f : 0.f;
     using V = typename Words<VW / 4>::T;
     using GV = typename Words<VW / 4>::G;
@@ -405,8 +409,10 @@ extern "C" int exl3_paged_attention(const void* q, int64_t q_ldt, int64_t q_ldh,
     // Rows of an average request and kv head: up to 16 are one tile of the decode kernel.  Eight requests of 16000 tokens, 40 heads
     // over 8 of 128, decode / chunk kernel in us: 100 / 125 at 15 rows, 141 / 125 at 20, 169 / 127 at 40; 24 over 4 of 256:
     // 105 / 130 at 12, 174 / 129 at 18; 32 over 8 of 64: 46 / 68 at 16, 68 / 69 at 24; two of 2000 tokens: 19 / 29 at 15 rows
-    // of 128, 36 / 29 at 20.  A request of more rows than that among many of fewer takes a tile for each 16: at most as many more
-    // tiles as there are requests.
+    // of 128, 36 / 29 at 20.  The host knows the average alone, not the lengths, so a batch of unlike requests takes the kernel
+    // of the many: a 512-token prompt beside 255 empty requests (40 heads over 8 of 128) 141 us in the decode kernel, which
+    // reads its keys for each 16 rows, 30 us by itself; beside 255 decodes over 2000 tokens 575 us there, the two by themselves
+    // 30 and 366; with 24 heads over 4 of 256 (18 rows on average) 587 us in the chunk kernel, by themselves 44 and 360.
     if (requests && (int64_t) tokens * a.group / requests > 16) launch_attn_prefill(a, dtype, head_dim, (hipStream_t) stream);
     else if (dtype == EXL3_FP16) launch<f16>(a, head_dim, (hipStream_t) stream);
     else launch<__bf16>(a, head_dim, (hipStream_t) stream);

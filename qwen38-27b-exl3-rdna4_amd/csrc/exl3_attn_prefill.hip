@@ -40,7 +40,7 @@ __device__ __forceinline__ void here(u32x4& a, u32x4& b, float& c)
 // padded rows, unlike permuted ones, let one address register and the instructions' offsets reach a whole step, and the two
 // buffers are two copies of the loop's body for the same reason: at 128 columns the registers are all taken (output 64,
 // Q 32, scores 32, K and V on the way 32).  One copy, the buffer a register, takes 1 to 1.5 % longer over long contexts.
-// 2048 tokens over 14000 (40 heads over 8 of 128): 805 to 831 us, 755 to 780 TFLOPS (a large library product takes 1160 to 1220); a
+// 2048 tokens over 14000 (40 heads over 8 of 128): 786 to 831 us, 755 to 800 TFLOPS (a large library product takes 1160 to 1220); a
 // 2048-token prompt 100 us; 8 x 4 tokens over 1000 to 32000 (24 over 4 of 256) 83 us, 3.0 TB/s of K and V.
 template <class T, int D>
 struct Prefill {
@@ -60,7 +60,7 @@ struct Prefill {
     static constexpr int TH = 32 / RW;                  // key tiles of a half step (32 keys)
     static constexpr int NB = AE * TH / 8;              // operands of its probabilities
     using Acc = std::conditional_t<RW == 32, f32x16, f32x4>;
-    static constexpr float SHIFT = std::is_same_v<T, f16> ? 8.f : 0.f;   // fp16 probabilities are held times 2^8
+    static constexpr float SHIFT = std::is_same_v<T, f16> ? 8.f : 0.f;   // fp16 probabilities are held times 2^8 (Decode::SHIFT)
     static constexpr int K_LD = D + 8, V_LD = RW == 32 ? D + 32 : D + 16;  // LDS rows, halves
 
     struct alignas(16) Shared {

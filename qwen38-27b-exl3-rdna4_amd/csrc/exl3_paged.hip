@@ -170,7 +170,8 @@ __device__ __forceinline__ u32x4 rotate8(u32x4 xb, const uint16_t* head, int c, 
 // theta = position x frequency is reduced to a fraction of a turn before it is rounded to 32 bits, so a position of a
 // million turns as exactly as position 0 (32-bit angles are 0.06 off there).  A workgroup forms the cosines and sines of
 // its token once, in LDS, and uses them for every head; k goes straight to its cache slot.  Bound by memory: 8192 tokens
-// of 40 + 8 heads of 128 in 47.2 us (235 MB, 5.0 TB/s; a large copy takes 4.6), 32 tokens in 3.1.
+// of 40 + 8 heads of 128 (235 MB) in 47 us, 5.0 TB/s, where calls write two outputs in turn, 40 us where all write the same
+// one (a large copy: 4.6 TB/s); 32 tokens in 2.6 to 3.1.
 template <class T, int D, int LAYOUT>
 __global__ void __launch_bounds__(256) rope_kv_write_kernel(RopeArgs a)
 {
@@ -264,9 +265,10 @@ extern "C" int exl3_rope_kv_write(const void* q, int64_t q_ldt, int64_t q_ldh, c
                UDiv::of((uint32_t) page_size)};
     // a vector piece of 8 pairs with one other piece where half the rotated part is a multiple of 8
     const int layout = interleaved ? ROPE_PAIRS : rot_dim % 16 == 0 ? ROPE_HALF : ROPE_ANY;
-    // Few tokens: a token's pieces over several workgroups, so that all heads' loads go out together (32 tokens 3.1 us, one
-    // workgroup a token 4.0); many fill the GPU without, and forming the angles once is cheaper (8192 tokens 39.6 us, several
-    // workgroups a token 41.3).
+    // Few tokens: a token's pieces over several workgroups, so that all heads' loads go out together; many fill the GPU
+    // without, and forming the angles once is cheaper.  Several workgroups a token / one, us, in a graph of calls that write one
+    // output, 40 + 8 heads of 128: 32 tokens 2.6 / 3.3, 256 3.4 / 3.8, 512 4.8 / 4.7, 768 6.2 / 6.2, 2048 11.8 / 10.9,
+    // 8192 50 / 38; 24 + 4 of 256, a quarter rotated: 2.8 / 4.0, 3.5 / 4.1, 4.7 / 5.0, 6.4 / 6.3, 12.8 / 11.9, 56 / 46.
     const dim3 grid((unsigned) tokens, tokens <= 512 ? (unsigned) std::min(64, (a.items + 255) / 256) : 1u);
     hipStream_t s = (hipStream_t) stream;
     if (dtype == EXL3_FP16) {
