@@ -36,9 +36,10 @@
 extern "C" {
 #endif
 
-#define EXL3_ABI_VERSION 4       /* 2: exl3_gemv_f32, exl3_gemm_trellis_silu_in; 3: exl3_gemv_silu_prerot_rows,
+#define EXL3_ABI_VERSION 5       /* 2: exl3_gemv_f32, exl3_gemm_trellis_silu_in; 3: exl3_gemv_silu_prerot_rows,
                                     exl3_gemm_trellis_workspace_bound, the plain GEMV up to 64 rows;
-                                    4: exl3_batch_plan, exl3_rope_kv_write, exl3_paged_attention */
+                                    4: exl3_batch_plan, exl3_rope_kv_write, exl3_paged_attention;
+                                    5: exl3_rope_kv_write8, exl3_kv_read8, exl3_paged_attention8 */
 #define EXL3_MAX_GROUPS 4       /* groups per grouped launch (reference EXL3_GEMV_MRG_MAX) */
 #define EXL3_GEMV_MAX_ROWS 64   /* rows the plain fused GEMV takes (exl3_gemv_mr and its grouped forms) */
 #define EXL3_GEMV_FUSED_MAX_ROWS 32 /* rows of the fused-epilogue forms (SiLU input, gated, approximate) */
@@ -398,6 +399,49 @@ int exl3_paged_attention(const void* q, int64_t q_ldt, int64_t q_ldh, const void
                          int64_t ld_table, int table_cols, const int* cu_q, const int* seq_lens, void* out, int64_t o_ldt,
                          int64_t o_ldh, int tokens, int requests, int q_heads, int kv_heads, int head_dim, int pages,
                          int page_size, float scale, int window, int dtype, void* workspace, size_t ws_bytes, void* stream);
+
+/* ---- the same over a paged cache in 8 bits --------------------------------------------------------------------
+ * Half the bytes of a 16-bit cache: a decode step reads half, and a GPU holds twice the tokens.  No counterpart in the
+ * reference's linear path.  k and v are int8 codes [pages][page_size][kv_heads][head_dim]; k_scale and v_scale are fp32
+ * [pages][page_size / 16][kv_heads], one for each block of EXL3_CACHE8_BLOCK tokens of a page and kv head; a value is code * scale.
+ * exl3_rope_kv_write8's scales are powers of two from 2^-40 to 2^40.  Other positive ones may be put there (a cache that
+ * someone else quantised); they count as the nearest in that range, and as its least where they are no number.  page_size: a multiple
+ * of 16.  Alignment: k and v 16 bytes, their strides multiples of 16 (elements, token strides up to EXL3_ATTN_MAX_LDT); scales'
+ * strides any; head_dim 64, 128 or 256. */
+#define EXL3_CACHE8_BLOCK 16
+typedef struct {
+    void *k, *v, *k_scale, *v_scale;
+    int64_t k_ldp, k_ldt, k_ldh, v_ldp, v_ldt, v_ldh;             /* strides of page, token, head */
+    int64_t ks_ldp, ks_ldb, ks_ldh, vs_ldp, vs_ldb, vs_ldh;       /* strides of page, block, head */
+    int32_t pages, page_size, kv_heads, head_dim;
+} exl3_cache8;
+
+/* exl3_rope_kv_write into such a cache.  k (rotated) and v are quantised from their fp32 values, with one rounding:
+ *   a call that writes a block's first slot starts the block anew: its scale is the least power of two of which 127 reach the
+ *   largest absolute value that the call writes to the block, and rows of it that the call does not write become 0;
+ *   otherwise the scale stays, or grows to what the new rows need, and then the block's other rows are rounded to the new
+ *   step (a block of one request's tokens in order is filled that way; a rejected draft's rows are written over, but a
+ *   scale that they raised stays);
+ *   code = value / scale, rounded to even, between -127 and 127.
+ * Infinities and NaN do not count for the scale; infinities become +-127, NaN 0.  Rows of one block are consecutive in the batch
+ * (as a request's tokens are): rows of one block that others lie between race.  A slot twice in a block's rows: the last counts.
+ * A slot outside [0, pages * page_size) writes nothing.  dtype: of q, k, v and q_out.  kv_heads, head_dim: the cache's. */
+int exl3_rope_kv_write8(const void* q, int64_t q_ldt, int64_t q_ldh, const void* k, int64_t k_ldt, int64_t k_ldh, const void* v,
+                        int64_t v_ldt, int64_t v_ldh, const int64_t* positions, const int64_t* slots, void* q_out,
+                        const exl3_cache8* cache, const double* inv_freq, float mscale, int tokens, int q_heads, int rot_dim,
+                        int interleaved, int dtype, void* stream);
+
+/* The values of `tokens` slots: k_out and v_out [tokens][kv_heads][head_dim] of dtype, one rounding (none where the type holds
+ * code * scale, as bf16 always does and fp16 from a scale of 2^-24 to 2^8).  A slot outside the cache gives zeros. */
+int exl3_kv_read8(const exl3_cache8* cache, const int64_t* slots, void* k_out, void* v_out, int tokens, int dtype, void* stream);
+
+/* exl3_paged_attention over such a cache, with its arguments, limits and workspace (one workspace serves both).  A key's code is a
+ * factor of its score and a value's of the output without a rounding in between; a probability is rounded to fp16 for its
+ * product with the codes.  A bf16 q is taken in fp16, each row times a power of two: elements below 2^-28 of the row's largest
+ * are rounded to multiples of 2^-38 of it.  Unseen keys have no effect, whatever their codes and scales are. */
+int exl3_paged_attention8(const void* q, int64_t q_ldt, int64_t q_ldh, const exl3_cache8* cache, const int* block_table, int64_t ld_table,
+                          int table_cols, const int* cu_q, const int* seq_lens, void* out, int64_t o_ldt, int64_t o_ldh, int tokens,
+                          int requests, int q_heads, float scale, int window, int dtype, void* workspace, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,7 +1,6 @@
 // exl3_paged.hip -- a decoder step's bookkeeping over a paged key/value cache (exl3_batch_plan), and the
 // rotary embedding of q and k with the cache's write (exl3_rope_kv_write).
-#include "exl3_device.h"
-#include "exl3_attn.h"
+#include "exl3_rope.h"
 
 using namespace exl3;
 
@@ -100,18 +99,6 @@ __global__ void __launch_bounds__(256) batch_plan_kernel(PlanArgs a)
     }
 }
 
-// position * freq / (2 pi) less its whole turns.  1 / (2 pi) in two doubles, and each product's rounding error by
-// fma: what is lost is below 2^-100 of the angle, so the fraction is good to 32 bits for any position below 2^53.
-__device__ __forceinline__ float turn_fraction(double position, double freq)
-{
-#pragma clang fp contract(off)                          // a product that a subtraction absorbs has no error to add
-    constexpr double C_HI = 0x1.45f306dc9c883p-3, C_LO = -0x1.6b01ec5417056p-57;
-    const double g = freq * C_HI, g_err = fma(freq, C_HI, -g) + freq * C_LO;
-    const double turns = position * g, err = fma(position, g, -turns) + position * g_err;
-    const double x = (turns - floor(turns)) + err;
-    return (float) (x - floor(x));
-}
-
 struct RopeArgs {
     const uint16_t *q, *k, *v;
     int64_t q_ldt, q_ldh, k_ldt, k_ldh, v_ldt, v_ldh;
@@ -125,47 +112,6 @@ struct RopeArgs {
     int items;                                          // 8-element pieces of a token: (hq + 2 hkv) D / 8
     UDiv d_page;
 };
-
-// 8 elements of a head from column c on, rotated.  x: those elements; other: the elements they pair with (half
-// layout); cs: the token's (cos, sin) per frequency.
-template <class T, int LAYOUT>
-__device__ __forceinline__ u32x4 rotate8(u32x4 xb, const uint16_t* head, int c, int rot, const float2* cs)
-{
-    using V = typename Elem<T>::x8;
-    const V x = __builtin_bit_cast(V, xb);
-    V y = x;
-    const int half = rot / 2;
-    if constexpr (LAYOUT == ROPE_HALF) {               // half % 8 == 0: the whole piece pairs with one piece
-        if (c < rot) {
-            const bool low = c < half;
-            const V o = __builtin_bit_cast(V, *reinterpret_cast<gc_u32x4*>(as_global(head) + (low ? c + half : c - half)));
-            const float2* f = cs + (low ? c : c - half);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = (T) ((float) x[i] * f[i].x + (low ? -(float) o[i] : (float) o[i]) * f[i].y);
-        }
-    } else if constexpr (LAYOUT == ROPE_PAIRS) {       // pairs side by side
-#pragma unroll
-        for (int i = 0; i < 8; i += 2)
-            if (c + i < rot) {
-                const float2 f = cs[(c + i) / 2];
-                const float u = (float) x[i], w = (float) x[i + 1];
-                y[i] = (T) (u * f.x - w * f.y);
-                y[i + 1] = (T) (w * f.x + u * f.y);
-            }
-    } else {                                           // half layout with an odd boundary: element by element
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int e = c + i;
-            if (e < rot) {
-                const bool low = e < half;
-                const float o = (float) __builtin_bit_cast(T, (uint16_t) *(as_global(head) + (low ? e + half : e - half)));
-                const float2 f = cs[low ? e : e - half];
-                y[i] = (T) ((float) x[i] * f.x + (low ? -o : o) * f.y);
-            }
-        }
-    }
-    return __builtin_bit_cast(u32x4, y);
-}
 
 // theta = position x frequency is reduced to a fraction of a turn before it is rounded to 32 bits, so a position of a
 // million turns as exactly as position 0 (32-bit angles are 0.06 off there).  A workgroup forms the cosines and sines of
@@ -190,7 +136,7 @@ __global__ void __launch_bounds__(256) rope_kv_write_kernel(RopeArgs a)
         if (h < a.hq) {
             const uint16_t* head = a.q + tok * a.q_ldt + h * a.q_ldh;
             const u32x4 x = *reinterpret_cast<gc_u32x4*>(as_global(head) + c);
-            *reinterpret_cast<g_u32x4*>(as_global(a.out) + (tok * a.hq + h) * D + c) = rotate8<T, LAYOUT>(x, head, c, a.rot, cs);
+            *reinterpret_cast<g_u32x4*>(as_global(a.out) + (tok * a.hq + h) * D + c) = rotated8<T, LAYOUT>(x, head, c, a.rot, cs);
             continue;
         }
         const int64_t slot = a.slots[tok];
@@ -201,7 +147,7 @@ __global__ void __launch_bounds__(256) rope_kv_write_kernel(RopeArgs a)
             const uint16_t* head = a.k + tok * a.k_ldt + h * a.k_ldh;
             const u32x4 x = *reinterpret_cast<gc_u32x4*>(as_global(head) + c);
             *reinterpret_cast<g_u32x4*>(as_global(a.kc) + page * a.kc_ldp + off * a.kc_ldt + h * a.kc_ldh + c) =
-                rotate8<T, LAYOUT>(x, head, c, a.rot, cs);
+                rotated8<T, LAYOUT>(x, head, c, a.rot, cs);
         } else {
             h -= a.hkv;
             const u32x4 x = *reinterpret_cast<gc_u32x4*>(as_global(a.v) + tok * a.v_ldt + h * a.v_ldh + c);

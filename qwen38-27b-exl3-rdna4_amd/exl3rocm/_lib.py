@@ -16,7 +16,7 @@ MAX_GROUPS = 4
 GEMV_MAX_ROWS = 64
 GEMV_FUSED_MAX_ROWS = 32
 NOALLOC_SCRATCH_BYTES = 17039360
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 _p, _i, _i64, _sz, _f = C.c_void_p, C.c_int, C.c_int64, C.c_size_t, C.c_float
 _pp = C.POINTER(C.c_void_p)
@@ -66,6 +66,9 @@ SIGNATURES = {
     "exl3_paged_attention_workspace_size": (_sz, []),
     "exl3_paged_attention": (_i, [_p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i, _p, _p, _p, _i64, _i64,
                                   _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _p, _sz, _p]),
+    "exl3_rope_kv_write8": (_i, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, C.c_char_p, _p, _f, _i, _i, _i, _i, _i, _p]),
+    "exl3_kv_read8": (_i, [C.c_char_p, _p, _p, _p, _i, _i, _p]),
+    "exl3_paged_attention8": (_i, [_p, _i64, _i64, C.c_char_p, _p, _i64, _i, _p, _p, _p, _i64, _i64, _i, _i, _i, _f, _i, _i, _p, _sz, _p]),
     "exl3_gemv_mr_noalloc": (_i, [_p, _i64, _p, _p, _i64, _p, _p, _i, _i, _i, _i, _i, _i, _p]),
 }
 

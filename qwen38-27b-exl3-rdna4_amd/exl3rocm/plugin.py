@@ -385,5 +385,5 @@ class Exl3LinearMethod(LinearMethodBase):
 
 def register():
     """vLLM general-plugin entry point: importing registers the config and the custom ops."""
-    from . import ops, paged  # noqa: F401
+    from . import ops, paged, paged8  # noqa: F401
     return None
