@@ -403,7 +403,8 @@ extern "C" int exl3_paged_attention8(const void* q, int64_t q_ldt, int64_t q_ldh
     a.d_page = a.c.d_page, a.d_group = UDiv::of((uint32_t) a.group);
     a.counters = (uint32_t*) workspace;
     a.part = reinterpret_cast<float*>((char*) workspace + EXL3_ATTN_COUNTER_BYTES);
-    if (dtype == EXL3_FP16) launch<f16>(a, (hipStream_t) stream);
+    if (requests && (int64_t) tokens * a.group / requests > 16) launch_attn8_prefill(a, dtype, (hipStream_t) stream);
+    else if (dtype == EXL3_FP16) launch<f16>(a, (hipStream_t) stream);
     else launch<__bf16>(a, (hipStream_t) stream);
     return hipGetLastError() == hipSuccess ? EXL3_OK : EXL3_ELAUNCH;
 }
