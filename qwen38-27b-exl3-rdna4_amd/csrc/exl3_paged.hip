@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(256) rope_kv_write_kernel(RopeArgs a)
         if (h < a.hq) {
             const uint16_t* head = a.q + tok * a.q_ldt + h * a.q_ldh;
             const u32x4 x = *reinterpret_cast<gc_u32x4*>(as_global(head) + c);
-            *reinterpret_cast<g_u32x4*>(as_global(a.out) + (tok * a.hq + h) * D + c) = rotated8<T, LAYOUT>(x, head, c, a.rot, cs);
+            *reinterpret_cast<g_u32x4*>(as_global(a.out) + (tok * a.hq + h) * D + c) = rotated8<T, LAYOUT>(x, partner8<T, LAYOUT>(head, c, a.rot), head, c, a.rot, cs);
             continue;
         }
         const int64_t slot = a.slots[tok];
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(256) rope_kv_write_kernel(RopeArgs a)
             const uint16_t* head = a.k + tok * a.k_ldt + h * a.k_ldh;
             const u32x4 x = *reinterpret_cast<gc_u32x4*>(as_global(head) + c);
             *reinterpret_cast<g_u32x4*>(as_global(a.kc) + page * a.kc_ldp + off * a.kc_ldt + h * a.kc_ldh + c) =
-                rotated8<T, LAYOUT>(x, head, c, a.rot, cs);
+                rotated8<T, LAYOUT>(x, partner8<T, LAYOUT>(head, c, a.rot), head, c, a.rot, cs);
         } else {
             h -= a.hkv;
             const u32x4 x = *reinterpret_cast<gc_u32x4*>(as_global(a.v) + tok * a.v_ldt + h * a.v_ldh + c);

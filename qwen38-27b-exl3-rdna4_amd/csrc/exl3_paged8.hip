@@ -18,11 +18,9 @@ struct Write8Args {
     const double* inv_freq;
     float mscale;
     int tokens, hq, rot;
-    int rows, heads, head_parts;                        // a k/v workgroup's rows of the batch, its kv heads, workgroups over the heads
+    int rows, heads, head_parts, turns, turn_wgs;                 // a k/v workgroup's rows of the batch, its kv heads, workgroups over the heads; workgroups that take a window's blocks in turn
     int kv_wgs, q_parts;                                // k/v workgroups in front of the q ones; workgroups of a token's q
 };
-
-constexpr int MOST_KV_WGS = 1 << 21;                    // a launch has fewer than 2^32 threads
 
 // The smallest exponent e of a scale with 127 * 2^e >= most, within the writer's.
 __device__ __forceinline__ int exponent8(float most)
@@ -32,6 +30,11 @@ __device__ __forceinline__ int exponent8(float most)
     return min(max(e, C8_LEAST), C8_MOST);
 }
 __device__ __forceinline__ float power2(int e) { return __int_as_float((e + 127) << 23); }
+__device__ __forceinline__ float reciprocal8(float s)      // of a scale: from its exponent where it is a power of two
+{
+    const int b = __float_as_int(s);
+    return b & 0x7FFFFF ? 1.f / s : __int_as_float((254 << 23) - b);
+}
 
 __device__ __forceinline__ float finite_abs(float x)
 {
@@ -39,16 +42,22 @@ __device__ __forceinline__ float finite_abs(float x)
     return a < INFINITY ? a : 0.f;                      // NaN compares false
 }
 
-// codes of 8 values, whose quotient by the scale is exact (a power of two): rounded to even, infinities to +-127, NaN to 0
-__device__ __forceinline__ u32x2 codes_of(const float (&x)[8], float inv)
+// Codes of 8 values, whose quotient by the scale is exact (a power of two): rounded to even by the addition of 1.5 2^23, which leaves
+// the whole number in the sum's low bits; infinities to +-127, and NaN, if there may be any, to 0.
+__device__ __forceinline__ u32x2 codes_of(const float (&x)[8], float inv, bool odd)
 {
-    u32x2 r = u32x2{0u, 0u};
+    uint32_t b[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float y = fminf(fmaxf(rintf(x[i] * inv), -127.f), 127.f);
-        const int q = x[i] == x[i] ? (int) y : 0;
-        r[i >> 2] |= ((uint32_t) q & 0xFFu) << (8 * (i & 3));
+    for (int i = 0; i < 8; ++i) b[i] = (uint32_t) __float_as_int(fminf(fmaxf(x[i] * inv, -127.f), 127.f) + 12582912.f);
+    if (odd) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] = x[i] == x[i] ? b[i] : 0u;
     }
+    u32x2 r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        r[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[4 * i + 3], b[4 * i + 2], 0x0C0C0400u),
+                                     __builtin_amdgcn_perm(b[4 * i + 1], b[4 * i], 0x0C0C0400u), 0x05040100u);
     return r;
 }
 // codes of a row whose block's scale grew by 1 / f
@@ -63,144 +72,197 @@ __device__ __forceinline__ u32x2 rounded_anew(u32x2 old, float f)
     return r;
 }
 
+// The largest of a wave's 64 values, in every lane.
+__device__ __forceinline__ float wave_max(float x)
+{
+    auto with = [&](auto CTRL) __attribute__((always_inline)) {
+        x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(CTRL)::value, 0xF, 0xF, true)));
+    };
+    with(std::integral_constant<int, 0xB1>{});          // quad_perm 1 0 3 2
+    with(std::integral_constant<int, 0x4E>{});          // quad_perm 2 3 0 1
+    with(std::integral_constant<int, 0x141>{});         // row_half_mirror
+    with(std::integral_constant<int, 0x140>{});         // row_mirror
+    return max_quads(x);
+}
+
 // One launch, two kinds of workgroups.  The first kv_wgs quantise k and v: workgroup (w, p) takes the blocks whose first row
 // in the batch is one of [rows w, rows (w + 1)), for the kv heads of part p.  A block's rows are consecutive in the batch, so one
-// workgroup has all of a block's new tokens, and its scale needs no second pass and no other workgroup.  Its 256 threads
-// hold the 16 rows of k and v of one head (8 elements a piece): new rows from the batch, the others' codes from the cache, requested
-// at once whether the scale will grow or not, so a block takes one trip to memory.  The others rotate q.
+// workgroup has all of a block's new tokens, and its scale needs no second pass and no other workgroup.  A thread
+// holds 8 elements of k and v of one of the block's 16 rows: new rows from the batch, the others' codes from the cache, requested at
+// once whether the scale will grow or not, with the angles formed meanwhile: a block takes two trips to memory (its slots and
+// positions, then all else), and a further head's is under way while the head before is computed.  The other workgroups rotate q.
 template <class T, int D, int LAYOUT>
-__global__ void __launch_bounds__(256) rope_kv_write8_kernel(Write8Args a)
+__global__ void __launch_bounds__(2 * D) rope_kv_write8_kernel(Write8Args a)
 {
-    constexpr int PIECES = D / 8, KIND = C8_BLOCK * PIECES, N = 2 * KIND / 256;      // pieces of a row, of k or v; a thread's
+    constexpr int PIECES = D / 8, THREADS = C8_BLOCK * PIECES, WAVES = THREADS / 64;
+    constexpr int FREQS = (D / 2 + 63) / 64;            // frequencies of a lane
+    constexpr int QN = 3;                               // pieces of q that a thread has under way
     __shared__ float2 cs[C8_BLOCK][D / 2];
     __shared__ int src[C8_BLOCK];                       // the block's rows: their token in the batch, -1 none
-    __shared__ float tops[2][4][2];                     // largest values of k and v of each wave; heads take turns
+    __shared__ float tops[2][WAVES][2];                 // largest values of k and v of each wave; heads take turns
     using V8 = typename Elem<T>::x8;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-
-    auto angles = [&](int row, int tok) __attribute__((always_inline)) {
+    auto cos_sin = [&](int64_t pos, double freq) __attribute__((always_inline)) {
         float s, c;
-        for (int f = lane; f < a.rot / 2; f += 64) {
-            sincospif(2.f * turn_fraction((double) a.pos[tok], a.inv_freq[f]), &s, &c);
-            cs[row][f] = make_float2(c * a.mscale, s * a.mscale);
-        }
+        sincospif(2.f * turn_fraction((double) pos, freq), &s, &c);
+        return make_float2(c * a.mscale, s * a.mscale);
     };
 
     if ((int) blockIdx.x >= a.kv_wgs) {
-        const int b = (int) blockIdx.x - a.kv_wgs, tok = b / a.q_parts, part = b - tok * a.q_parts;
-        for (int f = tid; f < a.rot / 2; f += 256) {
-            float s, c;
-            sincospif(2.f * turn_fraction((double) a.pos[tok], a.inv_freq[f]), &s, &c);
-            cs[0][f] = make_float2(c * a.mscale, s * a.mscale);
-        }
-        __syncthreads();
-        for (int i = part * 256 + tid; i < a.hq * PIECES; i += 256 * a.q_parts) {
-            const int h = i / PIECES, c = 8 * (i % PIECES);
-            const uint16_t* head = a.q + (int64_t) tok * a.q_ldt + (int64_t) h * a.q_ldh;
-            const u32x4 x = *reinterpret_cast<gc_u32x4*>(as_global(head) + c);
-            *reinterpret_cast<g_u32x4*>(as_global(a.out) + ((int64_t) tok * a.hq + h) * D + c) = rotated8<T, LAYOUT>(x, head, c, a.rot, cs[0]);
+        const int b = (int) blockIdx.x - a.kv_wgs, tok = b / a.q_parts, part = b - tok * a.q_parts, items = a.hq * PIECES;
+        for (int i0 = part * THREADS + tid; i0 - tid < items; i0 += QN * THREADS * a.q_parts) {
+            u32x4 x[QN], o[QN];
+            auto head_of = [&](int i) __attribute__((always_inline)) { return a.q + (int64_t) tok * a.q_ldt + (int64_t) (i / PIECES) * a.q_ldh; };
+#pragma unroll
+            for (int j = 0; j < QN; ++j) {
+                const int i = i0 + j * THREADS * a.q_parts;
+                if (i < items) {
+                    x[j] = *reinterpret_cast<gc_u32x4*>(as_global(head_of(i)) + 8 * (i % PIECES));
+                    o[j] = partner8<T, LAYOUT>(head_of(i), 8 * (i % PIECES), a.rot);
+                }
+            }
+            if (i0 == part * THREADS + tid) {
+                for (int f = tid; f < a.rot / 2; f += THREADS) cs[0][f] = cos_sin(a.pos[tok], a.inv_freq[f]);
+                __syncthreads();
+            }
+#pragma unroll
+            for (int j = 0; j < QN; ++j) {
+                const int i = i0 + j * THREADS * a.q_parts, c = 8 * (i % PIECES);
+                if (i < items) *reinterpret_cast<g_u32x4*>(as_global(a.out) + ((int64_t) tok * items + i) * 8) = rotated8<T, LAYOUT>(x[j], o[j], head_of(i), c, a.rot, cs[0]);
+            }
         }
         return;
     }
 
-    const int w = (int) blockIdx.x / a.head_parts, h0 = ((int) blockIdx.x - w * a.head_parts) * a.heads, h1 = min(h0 + a.heads, a.c.hkv);
-    const int row0 = w * a.rows;
+    const int my_turn = (int) blockIdx.x / a.turn_wgs, z = (int) blockIdx.x - my_turn * a.turn_wgs;
+    const int w = z / a.head_parts, h0 = (z - w * a.head_parts) * a.heads, h1 = min(h0 + a.heads, a.c.hkv), row0 = w * a.rows;
     const int64_t cache_slots = (int64_t) a.c.pages * a.c.page;
-    auto block_of = [&](int t) __attribute__((always_inline)) {                      // -1: a row of the batch that goes nowhere
+    auto slot_of = [&](int t) __attribute__((always_inline)) {                       // -1: a row of the batch that goes nowhere
         if (t < 0 || t >= a.tokens) return -1;
         const int64_t s = a.slots[t];
-        return s >= 0 && s < cache_slots ? (int) (s / C8_BLOCK) : -1;
+        return s >= 0 && s < cache_slots ? (int) s : -1;
     };
-    // lane l: row row0 + l; rows a block begins at (rows <= 64)
-    const int mine = lane < a.rows ? block_of(row0 + lane) : -1, prior = block_of(row0 + lane - 1);
-    uint64_t begins = __ballot(mine >= 0 && mine != prior);
-    for (; begins; begins &= begins - 1) {
-        const int first = row0 + __builtin_ctzll(begins), block = block_of(first);
+    // lane l: rows row0 + l and the one before.  A block begins where the row before belongs to another (-1 >> 4 is -1: none).
+    const int slot = slot_of(row0 + lane), mine = slot >> 4, prior = slot_of(row0 + lane - 1) >> 4;
+    static_assert(C8_BLOCK == 16);
+    double freq[FREQS];
+#pragma unroll
+    for (int i = 0; i < FREQS; ++i) freq[i] = lane + 64 * i < a.rot / 2 ? a.inv_freq[lane + 64 * i] : 0.0;
+    uint64_t begins = __ballot(lane < a.rows && mine >= 0 && mine != prior);
+    for (int i = 0; begins; begins &= begins - 1, ++i) {
+        if (i % a.turns != my_turn) continue;
+        const int at = __builtin_ctzll(begins), block = __builtin_amdgcn_readlane(mine, at);
         __syncthreads();                                // of the block before: src, cs and tops are free
         if (tid < C8_BLOCK) src[tid] = -1;
         __syncthreads();
         if (wave == 0) {
             // a slot that comes twice in a block's rows: the last one counts
-            for (int t = first;; t += 64) {
-                const uint64_t run = __ballot(block_of(t + lane) == block);
-                const int n = ~run ? __builtin_ctzll(~run) : 64;
-                if (lane < n) atomicMax(&src[a.slots[t + lane] % C8_BLOCK], t + lane);
+            uint64_t run = __ballot(mine == block) >> at;
+            int n = ~run ? __builtin_ctzll(~run) : 64;
+            if (lane >= at && lane < at + n) atomicMax(&src[slot & 15], row0 + lane);
+            for (int t = row0 + 64; at + n >= 64; t += 64) {       // more than the lanes' rows
+                const int s = slot_of(t + lane);
+                run = __ballot(s >> 4 == block);
+                n = ~run ? __builtin_ctzll(~run) : 64;
+                if (lane < n) atomicMax(&src[s & 15], t + lane);
                 if (n < 64) break;
             }
         }
         __syncthreads();
-        for (int r = wave; r < C8_BLOCK; r += 4)
-            if (src[r] >= 0) angles(r, src[r]);
-        __syncthreads();
         const bool anew = src[0] >= 0;
         const int page = (int) a.c.d_page.div((uint32_t) block * C8_BLOCK), in = block * C8_BLOCK - page * a.c.page;
-        for (int h = h0; h < h1; ++h) {
-            float* const ks = a.c.ks + (int64_t) page * a.c.ks_ldp + (int64_t) (in / C8_BLOCK) * a.c.ks_ldb + (int64_t) h * a.c.ks_ldh;
-            float* const vs = a.c.vs + (int64_t) page * a.c.vs_ldp + (int64_t) (in / C8_BLOCK) * a.c.vs_ldb + (int64_t) h * a.c.vs_ldh;
-            int8_t* const kc = a.c.k + (int64_t) page * a.c.k_ldp + (int64_t) in * a.c.k_ldt + (int64_t) h * a.c.k_ldh;
-            int8_t* const vc = a.c.v + (int64_t) page * a.c.v_ldp + (int64_t) in * a.c.v_ldt + (int64_t) h * a.c.v_ldh;
-            const float was[2] = {*as_global(ks), *as_global(vs)};
-            u32x4 raw[N];
-            u32x2 old[N];
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const int p = tid + 256 * j, r = p % KIND / PIECES, c = 8 * (p % PIECES), t = src[r];
-                const bool is_v = p >= KIND;
-                if (t >= 0) {
-                    const uint16_t* head = is_v ? a.v + (int64_t) t * a.v_ldt + (int64_t) h * a.v_ldh : a.k + (int64_t) t * a.k_ldt + (int64_t) h * a.k_ldh;
-                    raw[j] = *reinterpret_cast<gc_u32x4*>(as_global(head) + c);
-                } else if (!anew) {
-                    old[j] = *reinterpret_cast<gc_u32x2*>(as_global(is_v ? vc + (int64_t) r * a.c.v_ldt + c : kc + (int64_t) r * a.c.k_ldt + c));
-                }
+        const int row = tid / PIECES, c = 8 * (tid % PIECES), tok = src[row];
+        float* ks = a.c.ks + ((int64_t) page * a.c.ks_ldp + (int64_t) (in / C8_BLOCK) * a.c.ks_ldb + (int64_t) h0 * a.c.ks_ldh);
+        float* vs = a.c.vs + ((int64_t) page * a.c.vs_ldp + (int64_t) (in / C8_BLOCK) * a.c.vs_ldb + (int64_t) h0 * a.c.vs_ldh);
+        int8_t* kc = a.c.k + ((int64_t) page * a.c.k_ldp + (int64_t) (in + row) * a.c.k_ldt + (int64_t) h0 * a.c.k_ldh + c);
+        int8_t* vc = a.c.v + ((int64_t) page * a.c.v_ldp + (int64_t) (in + row) * a.c.v_ldt + (int64_t) h0 * a.c.v_ldh + c);
+        const uint16_t* k = a.k + ((int64_t) tok * a.k_ldt + (int64_t) h0 * a.k_ldh);
+        const uint16_t* v = a.v + ((int64_t) tok * a.v_ldt + (int64_t) h0 * a.v_ldh);
+        struct Piece {
+            u32x4 k, v, o;                              // new elements and k's partners; or in half of it the codes of a row that stays
+            float ks, vs;
+        };
+        auto request = [&](Piece& x, int d) __attribute__((always_inline)) {       // of head h + d
+            u32x4 xk = u32x4{0u, 0u, 0u, 0u}, xv = xk, xo = xk;
+            if (tok >= 0) {
+                xk = *reinterpret_cast<gc_u32x4*>(as_global(k + d * a.k_ldh) + c);
+                xv = *reinterpret_cast<gc_u32x4*>(as_global(v + d * a.v_ldh) + c);
+                xo = partner8<T, LAYOUT>(k + d * a.k_ldh, c, a.rot);
+            } else if (!anew) {
+                const u32x2 ko = *reinterpret_cast<gc_u32x2*>(as_global(kc + d * a.c.k_ldh)), vo = *reinterpret_cast<gc_u32x2*>(as_global(vc + d * a.c.v_ldh));
+                xk = u32x4{ko[0], ko[1], 0u, 0u};
+                xv = u32x4{vo[0], vo[1], 0u, 0u};
             }
-            float x[N][8], top[2] = {0.f, 0.f};
+            x = Piece{xk, xv, xo, *as_global(ks + d * a.c.ks_ldh), *as_global(vs + d * a.c.vs_ldh)};
+        };
+        Piece now, next;
+        request(now, 0);
+        for (int r = wave; r < C8_BLOCK; r += WAVES) {
+            const int t = src[r];
+            if (t < 0) continue;
+            const int64_t pos = a.pos[t];
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const int p = tid + 256 * j, r = p % KIND / PIECES, c = 8 * (p % PIECES), t = src[r];
-                const bool is_v = p >= KIND;
-                if (t < 0) continue;
-                const V8 e = __builtin_bit_cast(V8, raw[j]);
+            for (int i = 0; i < FREQS; ++i)
+                if (lane + 64 * i < a.rot / 2) cs[r][lane + 64 * i] = cos_sin(pos, freq[i]);
+        }
+        __syncthreads();
+        for (int h = h0; h < h1; ++h) {
+            if (h + 1 < h1) request(next, 1);
+            float x[8], y[8], top_k = 0.f, top_v = 0.f;
+            bool odd = false;                           // some element of the wave's is an infinity or NaN
+            if (tok >= 0) {
+                const V8 e = __builtin_bit_cast(V8, now.k), g = __builtin_bit_cast(V8, now.v);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[j][i] = (float) e[i];
-                if (!is_v) {
-                    const uint16_t* head = a.k + (int64_t) t * a.k_ldt + (int64_t) h * a.k_ldh;
-                    rotate8<T, LAYOUT>(e, head, c, a.rot, cs[r], [&](int i, float y) __attribute__((always_inline)) { x[j][i] = y; });
+                for (int i = 0; i < 8; ++i) {
+                    x[i] = (float) e[i];
+                    y[i] = (float) g[i];
                 }
-                float m = 0.f;
+                rotate8<T, LAYOUT>(now.k, now.o, k, c, a.rot, cs[row], [&](int i, float z) __attribute__((always_inline)) { x[i] = z; });
+                float any = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(x[j][i]));
-                top[0] = fmaxf(top[0], is_v ? 0.f : m);
-                top[1] = fmaxf(top[1], is_v ? m : 0.f);
+                for (int i = 0; i < 8; ++i) {
+                    top_k = fmaxf(top_k, fabsf(x[i]));
+                    top_v = fmaxf(top_v, fabsf(y[i]));
+                    any = fmaf(x[i], 0.f, fmaf(y[i], 0.f, any));
+                }
+                if (any != any) {
+                    odd = true;
+                    top_k = top_v = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        top_k = fmaxf(top_k, finite_abs(x[i]));
+                        top_v = fmaxf(top_v, finite_abs(y[i]));
+                    }
+                }
             }
             const int turn = (h - h0) & 1;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-#pragma unroll
-                for (int m = 1; m < 64; m <<= 1) top[i] = fmaxf(top[i], __shfl_xor(top[i], m));
-                if (lane == 0) tops[turn][wave][i] = top[i];
+            top_k = wave_max(top_k);
+            top_v = wave_max(top_v);
+            if (lane == 0) {
+                tops[turn][wave][0] = top_k;
+                tops[turn][wave][1] = top_v;
             }
             __syncthreads();
-            float now[2];
-            bool grown[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float m = tops[turn][0][i];
-#pragma unroll
-                for (int y = 1; y < 4; ++y) m = fmaxf(m, tops[turn][y][i]);
-                const float need = power2(exponent8(m)), had = scale8(was[i]);
-                grown[i] = anew || need > had;
-                now[i] = grown[i] ? need : had;
+            for (int i = 0; i < WAVES; ++i) {
+                top_k = fmaxf(top_k, tops[turn][i][0]);
+                top_v = fmaxf(top_v, tops[turn][i][1]);
             }
-            if (tid < 2 && grown[tid]) *as_global(tid ? vs : ks) = now[tid];
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const int p = tid + 256 * j, r = p % KIND / PIECES, c = 8 * (p % PIECES), t = src[r];
-                const bool is_v = p >= KIND;
-                auto* const dst = reinterpret_cast<g_u32x2*>(as_global(is_v ? vc + (int64_t) r * a.c.v_ldt + c : kc + (int64_t) r * a.c.k_ldt + c));
-                if (t >= 0) *dst = codes_of(x[j], 1.f / now[is_v]);
+            // the codes of 8 elements or of a row that stays, under the block's scale
+            auto put = [&](float* scale, float was, float top, int8_t* to, const float (&z)[8], u32x4 old) __attribute__((always_inline)) {
+                const float need = power2(exponent8(top)), had = scale8(was);
+                const bool grown = anew || need > had;
+                const float is = grown ? need : had, inv = reciprocal8(is);
+                if (tid == 0 && grown) *as_global(scale) = is;
+                auto* const dst = reinterpret_cast<g_u32x2*>(as_global(to));
+                if (tok >= 0) *dst = codes_of(z, inv, odd);
                 else if (anew) *dst = u32x2{0u, 0u};
-                else if (grown[is_v]) *dst = rounded_anew(old[j], scale8(was[is_v]) / now[is_v]);
-            }
+                else if (grown) *dst = rounded_anew(u32x2{old[0], old[1]}, had * inv);
+            };
+            put(ks, now.ks, top_k, kc, x, now.k);
+            put(vs, now.vs, top_v, vc, y, now.v);
+            now = next;
+            ks += a.c.ks_ldh, vs += a.c.vs_ldh, kc += a.c.k_ldh, vc += a.c.v_ldh, k += a.k_ldh, v += a.v_ldh;
         }
     }
 }
@@ -210,49 +272,49 @@ void launch_write8(const Write8Args& a, int layout, int wgs, hipStream_t s)
 {
     auto* kern = layout == ROPE_HALF ? rope_kv_write8_kernel<T, D, ROPE_HALF>
                  : layout == ROPE_PAIRS ? rope_kv_write8_kernel<T, D, ROPE_PAIRS> : rope_kv_write8_kernel<T, D, ROPE_ANY>;
-    hipLaunchKernelGGL(kern, dim3((unsigned) wgs), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(kern, dim3((unsigned) wgs), dim3(2 * D), 0, s, a);
 }
 
 struct Read8Args {
     Cache8 c;
     const int64_t* slots;
     uint16_t *k, *v;
-    int tokens, rows;                                   // rows of the batch that a workgroup reads
+    int tokens, items;                                  // 16-code pieces of a token's k and v
+    UDiv d_items;
 };
 
-// Tokens' k and v as fp16 or bf16 values: a thread turns 16 codes into 32 bytes.
+// Tokens' k and v as fp16 or bf16 values: a thread turns 16 codes into 32 bytes.  Bound by memory: 120641 tokens of 4 heads of 256 (370 MB) in
+// 72 us, 5.1 TB/s; two and four pieces a thread, all requested at once: 79 and 83.
 template <class T, int D>
 __global__ void __launch_bounds__(256) kv_read8_kernel(Read8Args a)
 {
     constexpr int PIECES = D / 16;
     using V8 = typename Elem<T>::x8;
-    const int items = 2 * a.c.hkv * PIECES, t0 = (int) blockIdx.x * a.rows, t1 = min(t0 + a.rows, a.tokens);
-    const int64_t cache_slots = (int64_t) a.c.pages * a.c.page;
-    for (int t = t0; t < t1; ++t) {
-        const int64_t slot = a.slots[t];
-        const bool held = slot >= 0 && slot < cache_slots;
-        const int page = held ? (int) a.c.d_page.div((uint32_t) slot) : 0, in = held ? (int) slot - page * a.c.page : 0;
-        for (int i = threadIdx.x; i < items; i += 256) {
-            const int p = i % PIECES, y = i / PIECES;
-            const bool is_v = y >= a.c.hkv;
-            const int h = is_v ? y - a.c.hkv : y;
-            u32x4 codes = u32x4{0u, 0u, 0u, 0u};
-            float s = 1.f;
-            if (held) {
-                const int8_t* src = is_v ? a.c.v + page * a.c.v_ldp + in * a.c.v_ldt + h * a.c.v_ldh : a.c.k + page * a.c.k_ldp + in * a.c.k_ldt + h * a.c.k_ldh;
-                codes = *reinterpret_cast<gc_u32x4*>(as_global(src) + 16 * p);
-                s = scale8(*as_global(is_v ? a.c.vs + page * a.c.vs_ldp + in / C8_BLOCK * a.c.vs_ldb + h * a.c.vs_ldh
-                                           : a.c.ks + page * a.c.ks_ldp + in / C8_BLOCK * a.c.ks_ldb + h * a.c.ks_ldh));
-            }
-            auto* const dst = as_global(is_v ? a.v : a.k) + ((int64_t) t * a.c.hkv + h) * D + 16 * p;
+    const int64_t first = (int64_t) blockIdx.x * 256, cache_slots = (int64_t) a.c.pages * a.c.page;
+    const int t0 = (int) (first / a.items);             // uniform
+    const uint32_t z = (uint32_t) (first - (int64_t) t0 * a.items) + threadIdx.x, dt = a.d_items.div(z);
+    const int t = t0 + (int) dt, i = (int) (z - dt * (uint32_t) a.items), p = i % PIECES, y = i / PIECES;
+    if (t >= a.tokens) return;
+    const bool is_v = y >= a.c.hkv;
+    const int h = is_v ? y - a.c.hkv : y;
+    u32x4 codes = u32x4{0u, 0u, 0u, 0u};
+    float s = 1.f;
+    const int64_t slot = a.slots[t];
+    if (slot >= 0 && slot < cache_slots) {
+        const int page = (int) a.c.d_page.div((uint32_t) slot), in = (int) slot - page * a.c.page;
+        codes = *reinterpret_cast<gc_u32x4*>(as_global(is_v ? a.c.v + page * a.c.v_ldp + in * a.c.v_ldt + h * a.c.v_ldh
+                                                            : a.c.k + page * a.c.k_ldp + in * a.c.k_ldt + h * a.c.k_ldh) + 16 * p);
+        s = *as_global(is_v ? a.c.vs + page * a.c.vs_ldp + in / C8_BLOCK * a.c.vs_ldb + h * a.c.vs_ldh
+                            : a.c.ks + page * a.c.ks_ldp + in / C8_BLOCK * a.c.ks_ldb + h * a.c.ks_ldh);
+    }
+    auto* const dst = as_global(is_v ? a.v : a.k) + ((int64_t) t * a.c.hkv + h) * D + 16 * p;
+    const float f = scale8(s);
 #pragma unroll
-            for (int z = 0; z < 2; ++z) {
-                V8 x;
+    for (int j = 0; j < 2; ++j) {
+        V8 x;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = (T) ((float) (int8_t) (uint8_t) (codes[2 * z + (e >> 2)] >> (8 * (e & 3))) * s);
-                *reinterpret_cast<g_u32x4*>(dst + 8 * z) = __builtin_bit_cast(u32x4, x);
-            }
-        }
+        for (int e = 0; e < 8; ++e) x[e] = (T) ((float) (int8_t) (uint8_t) (codes[2 * j + (e >> 2)] >> (8 * (e & 3))) * f);
+        *reinterpret_cast<g_u32x4*>(dst + 8 * j) = __builtin_bit_cast(u32x4, x);
     }
 }
 
@@ -260,7 +322,7 @@ template <class T>
 void launch_read8(const Read8Args& a, hipStream_t s)
 {
     auto* kern = a.c.d == 64 ? kv_read8_kernel<T, 64> : a.c.d == 128 ? kv_read8_kernel<T, 128> : kv_read8_kernel<T, 256>;
-    hipLaunchKernelGGL(kern, dim3((unsigned) ((a.tokens + a.rows - 1) / a.rows)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(kern, dim3((unsigned) (((int64_t) a.tokens * a.items + 255) / 256)), dim3(256), 0, s, a);
 }
 
 }  // namespace
@@ -285,13 +347,20 @@ extern "C" int exl3_rope_kv_write8(const void* q, int64_t q_ldt, int64_t q_ldh, 
     a.q_ldt = q_ldt, a.q_ldh = q_ldh, a.k_ldt = k_ldt, a.k_ldh = k_ldh, a.v_ldt = v_ldt, a.v_ldh = v_ldh;
     a.pos = positions, a.slots = slots, a.out = (uint16_t*) q_out, a.inv_freq = inv_freq, a.mscale = mscale;
     a.tokens = tokens, a.hq = q_heads, a.rot = rot_dim;
-    const bool few = tokens <= 512;
+    // Few tokens: a workgroup for each row and head, so that all blocks of a batch of decodes are under way at once.  More: windows
+    // of 16 rows, in which a prompt begins one or two blocks, and four workgroups that take them in turn; so many heads a
+    // workgroup that about 1024 have work, since its angles serve all of them.  One row / 16 rows a window, us, 40 + 8 heads of 128: a prompt's
+    // 128 tokens 10.9 / 7.6, 128 decodes 9.5 / 15.9; 512 tokens 16.5 / 9.9, 512 decodes 29 / 24; 32 decodes 6.5 / 15.  One, two,
+    // four and eight heads of 8192 tokens: 66, 58, 53, 50; of 1000 tokens, one and two: 15.3 and 13.5.
+    const bool few = (int64_t) tokens * hkv <= 1024;
     a.rows = few ? 1 : C8_BLOCK;
+    a.turns = few ? 1 : 4;
     const int windows = (tokens + a.rows - 1) / a.rows;
-    a.heads = (int) (((int64_t) windows * hkv + MOST_KV_WGS - 1) / MOST_KV_WGS);
+    a.heads = few ? 1 : (int) std::min((int64_t) hkv, ((int64_t) windows * hkv + 255) / 256);
     a.head_parts = (hkv + a.heads - 1) / a.heads;
-    a.kv_wgs = windows * a.head_parts;
-    a.q_parts = few ? std::min(64, (q_heads * (d / 8) + 255) / 256) : 1;
+    a.turn_wgs = windows * a.head_parts;
+    a.kv_wgs = a.turn_wgs * a.turns;                    // with the q ones fewer than 2^32 threads for 2^22 tokens
+    a.q_parts = tokens <= 512 ? std::min(64, (q_heads * (d / 8) + 2 * d - 1) / (2 * d)) : 1;
     const int layout = interleaved ? ROPE_PAIRS : rot_dim % 16 == 0 ? ROPE_HALF : ROPE_ANY, wgs = a.kv_wgs + tokens * a.q_parts;
     hipStream_t s = (hipStream_t) stream;
     if (dtype == EXL3_FP16) {
@@ -313,7 +382,9 @@ extern "C" int exl3_kv_read8(const exl3_cache8* cache, const int64_t* slots, voi
     if (tokens == 0) return EXL3_OK;
     if (!slots || !k_out || !v_out || !aligned16({k_out, v_out})) return EXL3_EINVAL;
     a.slots = slots, a.k = (uint16_t*) k_out, a.v = (uint16_t*) v_out, a.tokens = tokens;
-    a.rows = 1;
+    a.items = 2 * a.c.hkv * (a.c.d / 16);
+    a.d_items = UDiv::of((uint32_t) a.items);
+    if ((int64_t) tokens * a.items > UINT32_MAX - 256) return EXL3_EINVAL;         // a launch has fewer than 2^32 threads: 137 GB of values
     if (dtype == EXL3_FP16) launch_read8<f16>(a, (hipStream_t) stream);
     else launch_read8<__bf16>(a, (hipStream_t) stream);
     return hipGetLastError() == hipSuccess ? EXL3_OK : EXL3_ELAUNCH;

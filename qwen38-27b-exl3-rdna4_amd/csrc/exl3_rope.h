@@ -16,16 +16,28 @@ __device__ __forceinline__ float turn_fraction(double position, double freq)
     return (float) (x - floor(x));
 }
 
-// The rotated ones of 8 elements of a head from column c on: put(i, value), values in fp32.  x: those elements; the elements
-// they pair with are read from `head` (half layout); cs: the token's (cos, sin) per frequency.
-template <class T, int LAYOUT, class Put>
-__device__ __forceinline__ void rotate8(typename Elem<T>::x8 x, const uint16_t* head, int c, int rot, const float2* cs, Put&& put)
+// What 8 elements of a head from column c on pair with (half layout with whole pieces; else nothing): requested with them, so
+// that it is there when the angles are.
+template <class T, int LAYOUT>
+__device__ __forceinline__ u32x4 partner8(const uint16_t* head, int c, int rot)
 {
+    if constexpr (LAYOUT == ROPE_HALF)
+        if (c < rot) return *reinterpret_cast<gc_u32x4*>(as_global(head) + (c < rot / 2 ? c + rot / 2 : c - rot / 2));
+    return u32x4{0u, 0u, 0u, 0u};
+}
+
+// The rotated ones of 8 elements x of a head from column c on: put(i, value), values in fp32.  other: partner8's; cs: the
+// token's (cos, sin) per frequency.
+template <class T, int LAYOUT, class Put>
+__device__ __forceinline__ void rotate8(u32x4 xb, u32x4 other, const uint16_t* head, int c, int rot, const float2* cs, Put&& put)
+{
+    using V = typename Elem<T>::x8;
+    const V x = __builtin_bit_cast(V, xb);
     const int half = rot / 2;
     if constexpr (LAYOUT == ROPE_HALF) {               // half % 8 == 0: the whole piece pairs with one piece
         if (c < rot) {
             const bool low = c < half;
-            const auto o = __builtin_bit_cast(typename Elem<T>::x8, *reinterpret_cast<gc_u32x4*>(as_global(head) + (low ? c + half : c - half)));
+            const V o = __builtin_bit_cast(V, other);
             const float2* f = cs + (low ? c : c - half);
 #pragma unroll
             for (int i = 0; i < 8; ++i) put(i, (float) x[i] * f[i].x + (low ? -(float) o[i] : (float) o[i]) * f[i].y);
@@ -55,11 +67,10 @@ __device__ __forceinline__ void rotate8(typename Elem<T>::x8 x, const uint16_t* 
 
 // ... rounded to the element type, the others as they were
 template <class T, int LAYOUT>
-__device__ __forceinline__ u32x4 rotated8(u32x4 xb, const uint16_t* head, int c, int rot, const float2* cs)
+__device__ __forceinline__ u32x4 rotated8(u32x4 xb, u32x4 other, const uint16_t* head, int c, int rot, const float2* cs)
 {
-    const auto x = __builtin_bit_cast(typename Elem<T>::x8, xb);
-    auto y = x;
-    rotate8<T, LAYOUT>(x, head, c, rot, cs, [&](int i, float v) __attribute__((always_inline)) { y[i] = (T) v; });
+    auto y = __builtin_bit_cast(typename Elem<T>::x8, xb);
+    rotate8<T, LAYOUT>(xb, other, head, c, rot, cs, [&](int i, float v) __attribute__((always_inline)) { y[i] = (T) v; });
     return __builtin_bit_cast(u32x4, y);
 }
 
