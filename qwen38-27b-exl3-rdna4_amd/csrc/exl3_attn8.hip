@@ -32,11 +32,11 @@ struct Decode8 {
     static constexpr int AHEAD = 64 / NB;               // steps whose pages and scales a wave's lanes hold
     static constexpr int KC = D / 64;                   // 16-byte pieces of a K row that a lane holds: two products each
     static constexpr int E = D / 16;                    // V columns of a lane: its products
-    static constexpr int LEAST = 4;                     // steps of a share at least
+    static constexpr int LEAST = 256 / KEYS;            // steps of a share at least
     static constexpr int PAD = D + 4;                   // LDS row (floats) of the waves' outputs
     static constexpr bool Q_LDS = D > 128;              // Q would take more than 16 registers: read from LDS at each step
     static constexpr int Q_PAD = D + 8;                 // its LDS row (halves)
-    static constexpr int GRID = 256;                    // workgroups: one a CU
+    static constexpr int WGS = 8 / WAVES, GRID = 256 * WGS;             // workgroups: WGS a CU
     static constexpr int SLOT = attn_slot(ROWS, D);
     static_assert(GRID <= ATTN_COUNTERS && (size_t) 2 * GRID * SLOT * 4 <= ATTN_PART_BYTES);
     static constexpr float SHIFT = 8.f;                 // fp16 probabilities are held times 2^8
@@ -56,7 +56,7 @@ struct Decode8 {
 };
 
 template <class T, int D, int WAVES, int KEYS>
-__global__ void __launch_bounds__(64 * WAVES, 1) attn8_decode_kernel(Attn8Args a)
+__global__ void __launch_bounds__(64 * WAVES, 2) attn8_decode_kernel(Attn8Args a)
 {
     using X = Decode8<T, D, WAVES, KEYS>;
     constexpr int KC = X::KC, E = X::E, ROWS = X::ROWS, NB = X::NB, AHEAD = X::AHEAD;
@@ -70,7 +70,8 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn8_decode_kernel(Attn8Args a
         for (int i = tid; i < a.group * a.hkv * (D / 8); i += X::THREADS)
             *reinterpret_cast<g_u32x4*>(as_global(a.out) + (int64_t) t * a.o_ldt + (i / (D / 8)) * a.o_ldh + 8 * (i % (D / 8))) = u32x4{0u, 0u, 0u, 0u};
 
-    AttnWork<ROWS, KEYS, X::GRID> wk(a);
+    using Work = AttnWork<ROWS, KEYS, X::GRID>;
+    Work wk(a);
     int64_t left;
     int off;
     uint32_t per;
@@ -81,37 +82,120 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn8_decode_kernel(Attn8Args a
 #pragma unroll
     for (int i = 0; i < 4; ++i) v_lane[i] = (uint32_t) ((4 * g4 + i) * (int) a.c.v_ldt + E * c16);
 
-    while (true) {
-        wk.settle();
-        const AttnTile tile = wk.tile;
-        const int n_steps = __builtin_amdgcn_readfirstlane((int) min((int64_t) (tile.steps - off), left));
-        const int s0 = tile.step0 + off, s1 = s0 + n_steps;
-        const int* const row = a.table + (int64_t) wk.r * a.ld_table;
-        const int8_t* const kh = a.c.k + (int64_t) wk.h * a.c.k_ldh;
-        const int8_t* const vh = a.c.v + (int64_t) wk.h * a.c.v_ldh;
-        const float* const ksh = a.c.ks + (int64_t) wk.h * a.c.ks_ldh;
-        const float* const vsh = a.c.vs + (int64_t) wk.h * a.c.vs_ldh;
-
-        // Q^T in fp16: lane's row c16 of the tile, elements 64 c + 16 g4 + 8 h ..; and the position of the row's token
-        const int rows = wk.n * a.group;
-        auto q_at = [&](int x) __attribute__((always_inline)) {
-            const int y = min(wk.t * ROWS + x, rows - 1), tok = (int) a.d_group.div((uint32_t) y);
-            return as_global(a.q) + (int64_t) (wk.tok0 + tok) * a.q_ldt + (int64_t) (wk.h * a.group + y - tok * a.group) * a.q_ldh;
+    // What a tile's first steps need is requested before the tile before is done, so that its trips to memory (lengths, table, then
+    // keys) pass beside the other's work; `x` is a tile's work in all of these.
+    auto rows_of = [&](const Work& x) __attribute__((always_inline)) { return x.n * a.group; };
+    // pages of this wave's next AHEAD steps, lane NB x + y: block y of its x-th step; -1: none
+    auto pages_from = [&](const Work& x, int s) __attribute__((always_inline)) {
+        const int key = KEYS * (s + WAVES * (lane / NB)) + C8_BLOCK * (lane % NB);
+        int p = -1;
+        if (key < x.tile.hi) {
+            p = (a.table + (int64_t) x.r * a.ld_table)[a.d_page.div((uint32_t) key)];
+            if ((unsigned) p >= (unsigned) a.pages) p = -1;
+        }
+        return p;
+    };
+    // ... and their scales
+    struct Scales { float k, v; };
+    auto scales_of = [&](const Work& x, int s, int p) __attribute__((always_inline)) {
+        const int key = KEYS * (s + WAVES * (lane / NB)) + C8_BLOCK * (lane % NB);
+        float k = 1.f, v = 1.f;
+        if (p >= 0) {
+            const int b = (key - (int) a.d_page.div((uint32_t) key) * a.page) / C8_BLOCK;
+            k = *as_global(a.c.ks + (int64_t) x.h * a.c.ks_ldh + (int64_t) p * a.c.ks_ldp + (int64_t) b * a.c.ks_ldb);
+            v = *as_global(a.c.vs + (int64_t) x.h * a.c.vs_ldh + (int64_t) p * a.c.vs_ldp + (int64_t) b * a.c.vs_ldb);
+        }
+        return Scales{k, v};
+    };
+    // the first of 16 keys from `key` on of page p of a cache; -1 reads page 0, and its keys are seen by nobody
+    auto keys_at = [&](const int8_t* base, int64_t ldp, int64_t ldt, int p, int key) __attribute__((always_inline)) {
+        const int in = key - (int) a.d_page.div((uint32_t) key) * a.page;
+        return as_global(base) + ((int64_t) max(p, 0) * ldp + (int64_t) in * ldt);
+    };
+    typename X::KS k;
+    typename X::VS v;
+    auto load_k = [&](const Work& x, int s, const int (&p)[NB]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int y = 0; y < NB; ++y) {
+            auto* const kp = keys_at(a.c.k + (int64_t) x.h * a.c.k_ldh, a.c.k_ldp, a.c.k_ldt, p[y], KEYS * s + C8_BLOCK * y);
+#pragma unroll
+            for (int c = 0; c < KC; ++c) k[y][c] = __builtin_nontemporal_load(reinterpret_cast<gc_u32x4*>(kp + k_lane + 64 * c));
+        }
+    };
+    auto load_v = [&](const Work& x, int s, const int (&p)[NB]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int y = 0; y < NB; ++y) {
+            auto* const vp = keys_at(a.c.v + (int64_t) x.h * a.c.v_ldh, a.c.v_ldp, a.c.v_ldt, p[y], KEYS * s + C8_BLOCK * y);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 * y + i] = __builtin_nontemporal_load(reinterpret_cast<typename X::GV*>(vp + v_lane[i]));
+        }
+    };
+    // Q^T: lane's row c16 of the tile, elements 64 c + 16 g4 + 8 h ..; or a thread's pieces of Q on their way to LDS
+    constexpr int NQ = X::Q_LDS ? ROWS * D / 8 / X::THREADS : 2 * KC;
+    u32x4 q[NQ];
+    auto load_q = [&](const Work& x) __attribute__((always_inline)) {
+        auto at = [&](int z) __attribute__((always_inline)) {
+            const int y = min(x.t * ROWS + z, rows_of(x) - 1), tok = (int) a.d_group.div((uint32_t) y);
+            return as_global(a.q) + (int64_t) (x.tok0 + tok) * a.q_ldt + (int64_t) (x.h * a.group + y - tok * a.group) * a.q_ldh;
         };
-        u32x4 q[X::Q_LDS ? 1 : 2 * KC];
+#pragma unroll
+        for (int c = 0; c < NQ; ++c) {
+            const int z = tid + X::THREADS * c;
+            q[c] = X::Q_LDS ? *reinterpret_cast<gc_u32x4*>(at(z / (D / 8)) + 8 * (z % (D / 8)))
+                            : *reinterpret_cast<gc_u32x4*>(at(c16) + 16 * g4 + 64 * (c / 2) + 8 * (c % 2));
+        }
+    };
+    int pg = -1;
+    Scales sc{1.f, 1.f};
+    auto steps_of = [&](const Work& x, int off, int64_t left) __attribute__((always_inline)) {
+        return __builtin_amdgcn_readfirstlane((int) min((int64_t) (x.tile.steps - off), left));
+    };
+    // the first step of a wave of the tile's steps s0 .. s1 - 1, whose pages are in pg
+    auto begin = [&](const Work& x, int s0, int s1) __attribute__((always_inline)) {
+        load_q(x);
+        const int s = s0 + wave;
+        if (s < s1 && x.tile.lo < x.tile.hi) {
+            int p[NB];
+#pragma unroll
+            for (int y = 0; y < NB; ++y) p[y] = __builtin_amdgcn_readlane(pg, y);
+            load_k(x, s, p);
+            sc = scales_of(x, s, pg);
+            load_v(x, s, p);
+        }
+    };
+
+    wk.settle();
+    int n_steps = steps_of(wk, off, left);
+    pg = pages_from(wk, wk.tile.step0 + off + wave);
+    begin(wk, wk.tile.step0 + off, wk.tile.step0 + off + n_steps);
+    while (true) {
+        const AttnTile tile = wk.tile;
+        const int s0 = tile.step0 + off, s1 = s0 + n_steps, rows = rows_of(wk);
+        // the next tile's lengths, and its first pages on their way
+        const int64_t after = left - n_steps;
+        Work nx(a);
+        int pg_nx = -1, n_nx = 0;
+        nx.r = wk.r, nx.t = wk.t, nx.h = wk.h, nx.tok0 = wk.tok0, nx.n = wk.n, nx.pos0 = wk.pos0;
+        if (after > 0) {
+            nx.next();
+            nx.settle();
+            n_nx = steps_of(nx, 0, after);
+            pg_nx = pages_from(nx, nx.tile.step0 + wave);
+        }
+
+        // Q in fp16, and the position of the row's token
         const int xl = wk.t * ROWS + c16, pos = xl < rows ? wk.pos0 + (int) a.d_group.div((uint32_t) xl) : -1;  // a row past the tile's sees nothing
         const int upto = min(pos, a.cap - 1), from = a.window ? pos - a.window : -1;                            // the row sees from < key <= upto
         float qs;                                       // what the row's fp16 elements are to be multiplied by
-        if constexpr (!X::Q_LDS) {
-            auto* const src = q_at(c16) + 16 * g4;
 #pragma unroll
-            for (int c = 0; c < 2 * KC; ++c) q[c] = flipped(*reinterpret_cast<gc_u32x4*>(src + 64 * (c / 2) + 8 * (c % 2)), a.flip);
-            qs = fp16_rows<T>(q, [](float m) __attribute__((always_inline)) { return max_quads(m); });
-        }
+        for (int c = 0; c < NQ; ++c) q[c] = flipped(q[c], a.flip);
+        if constexpr (!X::Q_LDS) qs = fp16_rows<T>(q, [](float m) __attribute__((always_inline)) { return max_quads(m); });
         if constexpr (X::Q_LDS) {
             // D / 8 lanes hold a row
-            for (int z = tid; z < ROWS * D / 8; z += X::THREADS) {
-                u32x4 x[1] = {flipped(*reinterpret_cast<gc_u32x4*>(q_at(z / (D / 8)) + 8 * (z % (D / 8))), a.flip)};
+#pragma unroll
+            for (int c = 0; c < NQ; ++c) {
+                const int z = tid + X::THREADS * c;
+                u32x4 x[1] = {q[c]};
                 const float f = fp16_rows<T>(x, [](float m) __attribute__((always_inline)) {
 #pragma unroll
                     for (int d = 1; d < D / 8; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
@@ -129,78 +213,36 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn8_decode_kernel(Attn8Args a
         for (int e = 0; e < E; ++e) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
         const float row_scale = row_scale_of(a.scale, qs);
 
-        // pages of this wave's next AHEAD steps, lane NB x + y: block y of its x-th step; -1: none
-        auto pages_from = [&](int s) __attribute__((always_inline)) {
-            const int key = KEYS * (s + WAVES * (lane / NB)) + C8_BLOCK * (lane % NB);
-            int p = -1;
-            if (key < tile.hi) {
-                p = row[a.d_page.div((uint32_t) key)];
-                if ((unsigned) p >= (unsigned) a.pages) p = -1;
-            }
-            return p;
-        };
-        // ... and their scales: K's, and V's logarithm
-        struct Scales { float k, v; };
-        auto scales_of = [&](int s, int p) __attribute__((always_inline)) {
-            const int key = KEYS * (s + WAVES * (lane / NB)) + C8_BLOCK * (lane % NB);
-            Scales x{1.f, 1.f};
-            if (p >= 0) {
-                const int in = key - (int) a.d_page.div((uint32_t) key) * a.page;
-                x.k = *as_global(ksh + (int64_t) p * a.c.ks_ldp + (int64_t) (in / C8_BLOCK) * a.c.ks_ldb);
-                x.v = *as_global(vsh + (int64_t) p * a.c.vs_ldp + (int64_t) (in / C8_BLOCK) * a.c.vs_ldb);
-            }
-            return x;
-        };
-        // the first of 16 keys from `key` on of page p of a cache; -1 reads page 0, and its keys are seen by nobody
-        auto keys_at = [&](const int8_t* base, int64_t ldp, int64_t ldt, int p, int key) __attribute__((always_inline)) {
-            const int in = key - (int) a.d_page.div((uint32_t) key) * a.page;
-            return as_global(base) + ((int64_t) max(p, 0) * ldp + (int64_t) in * ldt);
-        };
-        auto load_k = [&](typename X::KS& x, int s, const int (&p)[NB]) __attribute__((always_inline)) {
-#pragma unroll
-            for (int y = 0; y < NB; ++y) {
-                auto* const kp = keys_at(kh, a.c.k_ldp, a.c.k_ldt, p[y], KEYS * s + C8_BLOCK * y);
-#pragma unroll
-                for (int c = 0; c < KC; ++c) x[y][c] = *reinterpret_cast<gc_u32x4*>(kp + k_lane + 64 * c);
-            }
-        };
-        auto load_v = [&](typename X::VS& x, int s, const int (&p)[NB]) __attribute__((always_inline)) {
-#pragma unroll
-            for (int y = 0; y < NB; ++y) {
-                auto* const vp = keys_at(vh, a.c.v_ldp, a.c.v_ldt, p[y], KEYS * s + C8_BLOCK * y);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[4 * y + i] = *reinterpret_cast<typename X::GV*>(vp + v_lane[i]);
-            }
-        };
-
         int s = s0 + wave;
         if (s < s1 && tile.lo < tile.hi) {
-            typename X::KS k;
-            typename X::VS v;
-            int pg = pages_from(s), at = 0, p[NB];
+            int at = 0, p[NB];
 #pragma unroll
             for (int y = 0; y < NB; ++y) p[y] = __builtin_amdgcn_readlane(pg, y);
-            load_k(k, s, p);
-            load_v(v, s, p);
-            Scales sc = scales_of(s, pg), sc_next = sc;
-            int pg_next = pages_from(s + AHEAD * WAVES);
+            int pg_next = pages_from(wk, s + AHEAD * WAVES);
+            // a lane's block: K's scale, V's logarithm and 1 / V's
+            float ska = scale8(sc.k), lva = log2_fast(scale8(sc.v)), iva = exp2_fast(-lva);
+            Scales sc_next{1.f, 1.f};
             while (true) {
                 const int next = s + WAVES;
                 int n[NB];
-                float sk[NB], lv[NB];
+                float sk[NB], lv[NB], iv[NB];
+                auto of_block = [&](float x, int y) __attribute__((always_inline)) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), NB * at + y)); };
 #pragma unroll
                 for (int y = 0; y < NB; ++y) {
-                    sk[y] = scale8(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(sc.k), NB * at + y)));
-                    lv[y] = log2_fast(scale8(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(sc.v), NB * at + y))));
+                    sk[y] = of_block(ska, y);
+                    lv[y] = of_block(lva, y);
+                    iv[y] = of_block(iva, y);
                     n[y] = 0;
                 }
                 // the next lanes' scales half way, when their pages have long been there
-                if (at == AHEAD / 2) sc_next = scales_of(next + (AHEAD - 1 - at) * WAVES, pg_next);
+                if (at == AHEAD / 2) sc_next = scales_of(wk, next + (AHEAD - 1 - at) * WAVES, pg_next);
                 if (next < s1) {
                     if (++at == AHEAD) {
                         pg = pg_next;
-                        sc = sc_next;
-                        pg_next = pages_from(next + AHEAD * WAVES);
+                        ska = scale8(sc_next.k);
+                        lva = log2_fast(scale8(sc_next.v));
+                        iva = exp2_fast(-lva);
+                        pg_next = pages_from(wk, next + AHEAD * WAVES);
                         at = 0;
                     }
 #pragma unroll
@@ -224,7 +266,7 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn8_decode_kernel(Attn8Args a
                         st[y] = mfma16<f16>(u32x4{codes2(w0, 0), codes2(w0, 1), codes2(w1, 0), codes2(w1, 1)}, qc, st[y]);
                     }
                 }
-                if (next < s1) load_k(k, next, n);
+                if (next < s1) load_k(wk, next, n);
                 float mx = m;
 #pragma unroll
                 for (int y = 0; y < NB; ++y) {
@@ -266,7 +308,7 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn8_decode_kernel(Attn8Args a
                             sum += x;
                             p8[4 * z + e] = (f16) x;
                         }
-                        l += sum * exp2_fast(-lv[y]);
+                        l = fmaf(sum, iv[y], l);
                     }
                     pb[b] = __builtin_bit_cast(u32x4, p8);
                 }
@@ -283,11 +325,15 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn8_decode_kernel(Attn8Args a
                         o[e] = mfma16<f16>(x, pb[b], o[e]);
                     }
                 if (next >= s1) break;
-                load_v(v, next, n);
+                load_v(wk, next, n);
                 s = next;
 #pragma unroll
                 for (int y = 0; y < NB; ++y) p[y] = n[y];
             }
+        }
+        if (after > 0) {
+            pg = pg_nx;
+            begin(nx, nx.tile.step0, nx.tile.step0 + n_nx);
         }
 
         // the waves' outputs joined: maxima first, then sums and outputs scaled to their maximum
@@ -350,10 +396,11 @@ __global__ void __launch_bounds__(64 * WAVES, 1) attn8_decode_kernel(Attn8Args a
             if (sh.last) join_parts<T, D, ROWS, X::THREADS, X::SLOT, 8>(prs, first_wg, last_wg, live_rows, out_at);
         }
         __syncthreads();
-        left -= n_steps;
-        if (left <= 0) break;
+        if (after <= 0) break;
+        left = after;
         off = 0;
-        wk.next();
+        n_steps = n_nx;
+        wk.r = nx.r, wk.t = nx.t, wk.h = nx.h, wk.tok0 = nx.tok0, wk.n = nx.n, wk.pos0 = nx.pos0, wk.tile = nx.tile;
     }
 }
 
@@ -367,9 +414,14 @@ void launch_one(const Attn8Args& a, hipStream_t s)
 template <class T>
 void launch(const Attn8Args& a, hipStream_t s)
 {
-    if (a.c.d == 64) launch_one<T, 64, 8, 64>(a, s);
-    else if (a.c.d == 128) launch_one<T, 128, 8, 64>(a, s);
-    else launch_one<T, 256, 4, 64>(a, s);
+    // Four waves a workgroup and two workgroups a CU: one streams while the other ends a tile and begins the next (512 requests of 200
+    // tokens, 40 heads over 8 of 128: 64 us, with one workgroup of eight waves 90).  Heads of 256 and few tiles, so that hardly
+    // any end, take eight waves: two and four requests' tiles over 131000 tokens 101 us against 112, but 256 requests of 1000 110
+    // against 100.
+    if (a.c.d == 64) launch_one<T, 64, 4, 64>(a, s);
+    else if (a.c.d == 128) launch_one<T, 128, 4, 64>(a, s);
+    else if ((int64_t) a.requests * a.hkv >= 256) launch_one<T, 256, 4, 32>(a, s);
+    else launch_one<T, 256, 8, 32>(a, s);
 }
 
 }  // namespace
