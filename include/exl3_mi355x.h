@@ -349,7 +349,7 @@ int exl3_gemv_mr_noalloc(const void* x, int64_t ldx, const void* trellis, void* 
 #define EXL3_PAGED_MAX_PAGE 65536 /* tokens of a page */
 #define EXL3_ATTN_MAX_LDT 67108864 /* token stride of a cache, elements */
 #define EXL3_ATTN_MAX_WINDOW 1073741824
-#define EXL3_ATTN_COUNTER_BYTES 2048
+#define EXL3_ATTN_COUNTER_BYTES 4096
 
 /* One step's bookkeeping from the requests' lengths.  Request r holds ctx_lens[r] tokens in the cache and adds
  * new_lens[r] (negative lengths count as 0; a request's length and the batch's counts stop at 2^31 - 1):

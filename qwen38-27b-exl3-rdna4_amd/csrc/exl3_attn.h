@@ -104,7 +104,7 @@ struct AttnArgs {
 
 // a partial tile, floats: rows x D outputs, then (maximum, sum) a row; two for each workgroup of a grid
 constexpr int attn_slot(int rows, int d) { return rows * (d + 2); }
-constexpr int ATTN_COUNTERS = EXL3_ATTN_COUNTER_BYTES / 4;                      // the largest grid
+constexpr int ATTN_COUNTERS = EXL3_ATTN_COUNTER_BYTES / 4;                      // the largest grid, twice
 constexpr size_t ATTN_PART_BYTES = (size_t) 2 * 512 * attn_slot(128, 130) * 4;  // the largest grid times slot (all kernels assert it)
 
 // A request's new rows for one kv head, (token, head of the group) in token order, are cut into tiles of `rows`; a tile

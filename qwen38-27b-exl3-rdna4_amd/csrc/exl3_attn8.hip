@@ -21,13 +21,15 @@ template <> struct Codes<4> { typedef u32x4 T; typedef gc_u32x4 G; };
 // s_j + log2 sv_j, the kernel sums e_j cv_j and e_j / sv_j, e_j = 2^(s_j + log2 sv_j - r), a multiplication a block and no
 // more operations an element than without scales.  e is in [0, 1], so fp16 holds it (times 2^8, as in the 16-bit kernel),
 // and scales within 2^-40 .. 2^40 leave the sums of e / sv in fp32's range.
+// More than 16 rows: a tile is S sets of 16, and S workgroups on one XCD, each with a set, work through the same keys at
+// the same time, so that all but the first read them from its L2 (12 requests of 24 rows: 198 MB of memory traffic for 188 MB of keys).
 // Layout of the products as in the 16-bit cache's kernel: S^T = K Q^T leaves P^T as the next product's operand, a wave takes whole
 // steps with a softmax of its own, K and V go from memory into registers and are made operands there.
 //   K: a lane holds key l & 15, bytes 64 c + 16 (l >> 4) .. + 15: two products' 8 elements each, so q's lane holds the same columns
 //   V: a lane holds E = D / 16 columns E (l & 15) .. of its keys, and product e is made of column e of pairs of keys
-template <class T, int D, int WAVES, int KEYS>
+template <class T, int D, int WAVES, int KEYS, int S>
 struct Decode8 {
-    static constexpr int ROWS = 16, THREADS = 64 * WAVES;
+    static constexpr int ROWS = 16, TILE = ROWS * S, THREADS = 64 * WAVES;
     static constexpr int NB = KEYS / C8_BLOCK;          // blocks of a step
     static constexpr int AHEAD = 64 / NB;               // steps whose pages and scales a wave's lanes hold
     static constexpr int KC = D / 64;                   // 16-byte pieces of a K row that a lane holds: two products each
@@ -37,8 +39,9 @@ struct Decode8 {
     static constexpr bool Q_LDS = D > 128;              // Q would take more than 16 registers: read from LDS at each step
     static constexpr int Q_PAD = D + 8;                 // its LDS row (halves)
     static constexpr int WGS = 8 / WAVES, GRID = 256 * WGS;             // workgroups: WGS a CU
+    static constexpr int SHARES = GRID / S;             // S workgroups have a share of the work, 16 rows of its tiles each
     static constexpr int SLOT = attn_slot(ROWS, D);
-    static_assert(GRID <= ATTN_COUNTERS && (size_t) 2 * GRID * SLOT * 4 <= ATTN_PART_BYTES);
+    static_assert(GRID <= ATTN_COUNTERS / 2 && (size_t) 2 * GRID * SLOT * 4 <= ATTN_PART_BYTES);
     static constexpr float SHIFT = 8.f;                 // fp16 probabilities are held times 2^8
     using V = typename Codes<E / 4>::T;
     using GV = typename Codes<E / 4>::G;
@@ -55,22 +58,81 @@ struct Decode8 {
     };
 };
 
-template <class T, int D, int WAVES, int KEYS>
+// Parts of a tile summed in order: part i at slot_at(i) (floats), rows x D outputs, then (maximum, sum) a row.  Z elements of a thread
+// and B parts of each are in flight.
+template <int D, int ROWS, int THREADS, class SlotAt, class Put>
+__device__ __forceinline__ void join8(__amdgpu_buffer_rsrc_t prs, int parts, int rows, SlotAt&& slot_at, Put&& put)
+{
+    constexpr int Z = 2, B = 8;
+    const int all = rows * (D / 4);
+    for (int z0 = threadIdx.x; z0 < all; z0 += Z * THREADS) {
+        uint32_t at[Z], ml[Z];
+        float m[Z], l[Z];
+        f32x4 sum[Z];
+#pragma unroll
+        for (int i = 0; i < Z; ++i) {
+            const int z = min(z0 + i * THREADS, all - 1);
+            at[i] = 16u * (uint32_t) z;
+            ml[i] = (uint32_t) (ROWS * D + 2 * (z / (D / 4))) * 4u;
+            m[i] = LOWEST;
+            l[i] = 0.f;
+            sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+#pragma unroll 1
+        for (int c0 = 0; c0 < parts; c0 += B) {
+            u32x2 mls[Z][B];
+            f32x4 v[Z][B];
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const uint32_t s = 4u * (uint32_t) __builtin_amdgcn_readfirstlane((int) slot_at(min(c0 + b, parts - 1)));
+#pragma unroll
+                for (int i = 0; i < Z; ++i) {
+                    mls[i][b] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(prs, ml[i], s, SC1));
+                    v[i][b] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(prs, at[i], s, SC1));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < Z; ++i) {
+                float top = m[i];
+#pragma unroll
+                for (int b = 0; b < B; ++b) top = fmaxf(top, __int_as_float((int) mls[i][b][0]));
+                const float c = exp2_fast(m[i] - top);
+                l[i] *= c;
+                sum[i] *= c;
+                m[i] = top;
+#pragma unroll
+                for (int b = 0; b < B; ++b) {
+                    const float f = c0 + b < parts ? exp2_fast(__int_as_float((int) mls[i][b][0]) - top) : 0.f;
+                    l[i] += f * __int_as_float((int) mls[i][b][1]);
+                    sum[i] += v[i][b] * f;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < Z; ++i) {
+            const int z = z0 + i * THREADS;
+            if (z < all) put(z / (D / 4), 4 * (z % (D / 4)), sum[i], m[i], l[i]);
+        }
+    }
+}
+
+template <class T, int D, int WAVES, int KEYS, int S>
 __global__ void __launch_bounds__(64 * WAVES, 2) attn8_decode_kernel(Attn8Args a)
 {
-    using X = Decode8<T, D, WAVES, KEYS>;
+    using X = Decode8<T, D, WAVES, KEYS, S>;
     constexpr int KC = X::KC, E = X::E, ROWS = X::ROWS, NB = X::NB, AHEAD = X::AHEAD;
     __shared__ typename X::Shared sh;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c16 = lane & 15, g4 = lane >> 4;
-    const int wg = blockIdx.x;
+    // workgroups go round the 8 XCDs: b and b + 8 are on one
+    const int set = S == 1 ? 0 : (int) blockIdx.x / 8 % S, wg = S == 1 ? (int) blockIdx.x : (int) blockIdx.x / (8 * S) * 8 + (int) blockIdx.x % 8;
 
     // rows of no request
     const int used = a.requests ? min(max(a.cu_q[a.requests], 0), a.tokens) : 0;
-    for (int t = used + wg; t < a.tokens; t += X::GRID)
+    for (int t = used + (int) blockIdx.x; t < a.tokens; t += X::GRID)
         for (int i = tid; i < a.group * a.hkv * (D / 8); i += X::THREADS)
             *reinterpret_cast<g_u32x4*>(as_global(a.out) + (int64_t) t * a.o_ldt + (i / (D / 8)) * a.o_ldh + 8 * (i % (D / 8))) = u32x4{0u, 0u, 0u, 0u};
 
-    using Work = AttnWork<ROWS, KEYS, X::GRID>;
+    using Work = AttnWork<X::TILE, KEYS, X::SHARES>;
     Work wk(a);
     int64_t left;
     int off;
@@ -112,6 +174,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attn8_decode_kernel(Attn8Args a
         const int in = key - (int) a.d_page.div((uint32_t) key) * a.page;
         return as_global(base) + ((int64_t) max(p, 0) * ldp + (int64_t) in * ldt);
     };
+    // Keys that one workgroup alone reads leave the caches to others: 5 to 12 % faster.
+    auto load_once = [&](auto* p) __attribute__((always_inline)) {
+        if constexpr (S == 1) return __builtin_nontemporal_load(p);
+        else return *p;
+    };
     typename X::KS k;
     typename X::VS v;
     auto load_k = [&](const Work& x, int s, const int (&p)[NB]) __attribute__((always_inline)) {
@@ -119,7 +186,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attn8_decode_kernel(Attn8Args a
         for (int y = 0; y < NB; ++y) {
             auto* const kp = keys_at(a.c.k + (int64_t) x.h * a.c.k_ldh, a.c.k_ldp, a.c.k_ldt, p[y], KEYS * s + C8_BLOCK * y);
 #pragma unroll
-            for (int c = 0; c < KC; ++c) k[y][c] = __builtin_nontemporal_load(reinterpret_cast<gc_u32x4*>(kp + k_lane + 64 * c));
+            for (int c = 0; c < KC; ++c) k[y][c] = load_once(reinterpret_cast<gc_u32x4*>(kp + k_lane + 64 * c));
         }
     };
     auto load_v = [&](const Work& x, int s, const int (&p)[NB]) __attribute__((always_inline)) {
@@ -127,7 +194,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attn8_decode_kernel(Attn8Args a
         for (int y = 0; y < NB; ++y) {
             auto* const vp = keys_at(a.c.v + (int64_t) x.h * a.c.v_ldh, a.c.v_ldp, a.c.v_ldt, p[y], KEYS * s + C8_BLOCK * y);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[4 * y + i] = __builtin_nontemporal_load(reinterpret_cast<typename X::GV*>(vp + v_lane[i]));
+            for (int i = 0; i < 4; ++i) v[4 * y + i] = load_once(reinterpret_cast<typename X::GV*>(vp + v_lane[i]));
         }
     };
     // Q^T: lane's row c16 of the tile, elements 64 c + 16 g4 + 8 h ..; or a thread's pieces of Q on their way to LDS
@@ -135,7 +202,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attn8_decode_kernel(Attn8Args a
     u32x4 q[NQ];
     auto load_q = [&](const Work& x) __attribute__((always_inline)) {
         auto at = [&](int z) __attribute__((always_inline)) {
-            const int y = min(x.t * ROWS + z, rows_of(x) - 1), tok = (int) a.d_group.div((uint32_t) y);
+            const int y = min(x.t * X::TILE + ROWS * set + z, rows_of(x) - 1), tok = (int) a.d_group.div((uint32_t) y);
             return as_global(a.q) + (int64_t) (x.tok0 + tok) * a.q_ldt + (int64_t) (x.h * a.group + y - tok * a.group) * a.q_ldh;
         };
 #pragma unroll
@@ -183,8 +250,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attn8_decode_kernel(Attn8Args a
             pg_nx = pages_from(nx, nx.tile.step0 + wave);
         }
 
+        const int live_rows = max(min(ROWS, rows - wk.t * X::TILE - ROWS * set), 0);
         // Q in fp16, and the position of the row's token
-        const int xl = wk.t * ROWS + c16, pos = xl < rows ? wk.pos0 + (int) a.d_group.div((uint32_t) xl) : -1;  // a row past the tile's sees nothing
+        const int xl = wk.t * X::TILE + ROWS * set + c16, pos = xl < rows ? wk.pos0 + (int) a.d_group.div((uint32_t) xl) : -1;  // a row past the tile's sees nothing
         const int upto = min(pos, a.cap - 1), from = a.window ? pos - a.window : -1;                            // the row sees from < key <= upto
         float qs;                                       // what the row's fp16 elements are to be multiplied by
 #pragma unroll
@@ -214,7 +282,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attn8_decode_kernel(Attn8Args a
         const float row_scale = row_scale_of(a.scale, qs);
 
         int s = s0 + wave;
-        if (s < s1 && tile.lo < tile.hi) {
+        if (s < s1 && tile.lo < tile.hi && live_rows > 0) {
             int at = 0, p[NB];
 #pragma unroll
             for (int y = 0; y < NB; ++y) p[y] = __builtin_amdgcn_readlane(pg, y);
@@ -341,13 +409,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attn8_decode_kernel(Attn8Args a
         if (g4 == 0) sh.m[wave][c16] = m;
         __syncthreads();
         const int first_wg = wg - (int) (((uint32_t) off + per - 1u) / per);        // workgroups back to the tile's first step
-        const uint32_t slot = 2u * (uint32_t) wg + (starts ? 1u : 0u);
+        const uint32_t slot = 2u * (uint32_t) (wg + set * X::SHARES) + (starts ? 1u : 0u);
         const __amdgpu_buffer_rsrc_t prs = __builtin_amdgcn_make_buffer_rsrc(a.part, 0, (int) ATTN_PART_BYTES, RAW_BUFFER_FLAGS);
         auto out_at = [&](int x) __attribute__((always_inline)) {                  // row x of the tile
-            const int y = wk.t * ROWS + x, tok = (int) a.d_group.div((uint32_t) y);
+            const int y = wk.t * X::TILE + ROWS * set + x, tok = (int) a.d_group.div((uint32_t) y);
             return as_global(a.out) + (int64_t) (wk.tok0 + tok) * a.o_ldt + (int64_t) (wk.h * a.group + y - tok * a.group) * a.o_ldh;
         };
-        const int live_rows = min(ROWS, rows - wk.t * ROWS);
         float top = LOWEST;
 #pragma unroll
         for (int x = 0; x < WAVES; ++x) top = fmaxf(top, sh.m[x][c16]);
@@ -382,18 +449,46 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attn8_decode_kernel(Attn8Args a
                 }
             }
         }
-        if (split) {
-            // the workgroup that counts last joins the tile's parts, in the order of the workgroups
-            const int last_wg = wg + (int) (((uint32_t) (tile.steps - off - n_steps) + per - 1u) / per);
-            __builtin_amdgcn_s_waitcnt(0x0F70);        // vmcnt(0): the part has landed
-            __syncthreads();
-            if (tid == 0) {
-                const uint32_t before = __hip_atomic_fetch_add(&a.counters[first_wg], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                sh.last = before == (uint32_t) (last_wg - first_wg);
-                if (sh.last) __hip_atomic_store(&a.counters[first_wg], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (split && live_rows > 0) {
+            // Who counts last joins, in the order of the workgroups.  Many parts in two levels: groups of about their number's
+            // root, joined by the last of each at the same time, then the groups.  (A workgroup's part of one tile and of the
+            // next lie in slots 2 c and 2 c + 1 and are counted under the tiles' first workgroups.  What is joined of a group lies in a
+            // slot that neither uses: 2 c + 1 of its first workgroup c, which begins no tile, or for a tile's first group of its second.)
+            const int last_wg = wg + (int) (((uint32_t) (tile.steps - off - n_steps) + per - 1u) / per), n = last_wg - first_wg + 1;
+            const int size = n <= 12 ? n : n <= 64 ? 8 : n <= 256 ? 16 : 24, group = (wg - first_wg) / size, groups = (n + size - 1) / size;
+            const int begin_wg = first_wg + group * size, in_group = min(size, last_wg + 1 - begin_wg);
+            auto part = [&](int c) __attribute__((always_inline)) { return (uint32_t) (2 * (c + set * X::SHARES) + (c == first_wg ? 1 : 0)) * (uint32_t) X::SLOT; };
+            auto joined = [&](int g) __attribute__((always_inline)) {
+                const int c = first_wg + g * size;
+                return c == last_wg ? part(c) : (uint32_t) (2 * ((g ? c : c + 1) + set * X::SHARES) + 1) * (uint32_t) X::SLOT;
+            };
+            auto i_am_last = [&](uint32_t* counter, int of) __attribute__((always_inline)) {
+                __builtin_amdgcn_s_waitcnt(0x0F70);    // vmcnt(0): the part has landed
+                __syncthreads();
+                if (tid == 0) {
+                    sh.last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t) (of - 1);
+                    if (sh.last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+                __syncthreads();
+                return sh.last != 0;
+            };
+            bool mine = true;
+            if (groups > 1 && in_group > 1) {
+                mine = i_am_last(&a.counters[ATTN_COUNTERS / 2 + begin_wg + set * X::SHARES], in_group);
+                if (mine) {
+                    const uint32_t to = joined(group);
+                    join8<D, ROWS, X::THREADS>(prs, in_group, live_rows, [&](int i) __attribute__((always_inline)) { return part(begin_wg + i); },
+                                               [&](int x, int col, f32x4 sum, float top, float l) __attribute__((always_inline)) {
+                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum), prs, (to + (uint32_t) (x * D + col)) * 4u, 0, SC1);
+                        if (col == 0)
+                            __builtin_amdgcn_raw_buffer_store_b64(u32x2{(uint32_t) __float_as_int(top), (uint32_t) __float_as_int(l)}, prs, (to + (uint32_t) (ROWS * D + 2 * x)) * 4u, 0, SC1);
+                    });
+                }
             }
-            __syncthreads();
-            if (sh.last) join_parts<T, D, ROWS, X::THREADS, X::SLOT, 8>(prs, first_wg, last_wg, live_rows, out_at);
+            if (mine && i_am_last(&a.counters[first_wg + set * X::SHARES], groups > 1 ? groups : n))
+                join8<D, ROWS, X::THREADS>(prs, groups > 1 ? groups : n, live_rows,
+                                           [&](int i) __attribute__((always_inline)) { return groups > 1 ? joined(i) : part(first_wg + i); },
+                                           [&](int x, int col, f32x4 sum, float, float l) __attribute__((always_inline)) { store_out<T>(out_at(x) + col, sum, l); });
         }
         __syncthreads();
         if (after <= 0) break;
@@ -404,24 +499,28 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attn8_decode_kernel(Attn8Args a
     }
 }
 
-template <class T, int D, int WAVES, int KEYS>
+template <class T, int D, int WAVES, int KEYS, int S>
 void launch_one(const Attn8Args& a, hipStream_t s)
 {
-    using X = Decode8<T, D, WAVES, KEYS>;
-    hipLaunchKernelGGL((attn8_decode_kernel<T, D, WAVES, KEYS>), dim3(X::GRID), dim3(X::THREADS), 0, s, a);
+    using X = Decode8<T, D, WAVES, KEYS, S>;
+    hipLaunchKernelGGL((attn8_decode_kernel<T, D, WAVES, KEYS, S>), dim3(X::GRID), dim3(X::THREADS), 0, s, a);
 }
 
 template <class T>
-void launch(const Attn8Args& a, hipStream_t s)
+void launch(const Attn8Args& a, int rows, hipStream_t s)
 {
     // Four waves a workgroup and two workgroups a CU: one streams while the other ends a tile and begins the next (512 requests of 200
     // tokens, 40 heads over 8 of 128: 64 us, with one workgroup of eight waves 90).  Heads of 256 and few tiles, so that hardly
     // any end, take eight waves: two and four requests' tiles over 131000 tokens 101 us against 112, but 256 requests of 1000 110
-    // against 100.
-    if (a.c.d == 64) launch_one<T, 64, 4, 64>(a, s);
-    else if (a.c.d == 128) launch_one<T, 128, 4, 64>(a, s);
-    else if ((int64_t) a.requests * a.hkv >= 256) launch_one<T, 256, 4, 32>(a, s);
-    else launch_one<T, 256, 8, 32>(a, s);
+    // against 100.  Up to 32 rows on average: two workgroups that share a tile's keys (TILE above).
+    if (rows > 16) {
+        if (a.c.d == 64) launch_one<T, 64, 4, 64, 2>(a, s);
+        else if (a.c.d == 128) launch_one<T, 128, 4, 32, 2>(a, s);
+        else launch_one<T, 256, 8, 32, 2>(a, s);
+    } else if (a.c.d == 64) launch_one<T, 64, 4, 64, 1>(a, s);
+    else if (a.c.d == 128) launch_one<T, 128, 4, 64, 1>(a, s);
+    else if ((int64_t) a.requests * a.hkv >= 256) launch_one<T, 256, 4, 32, 1>(a, s);
+    else launch_one<T, 256, 8, 32, 1>(a, s);
 }
 
 }  // namespace
@@ -455,8 +554,15 @@ extern "C" int exl3_paged_attention8(const void* q, int64_t q_ldt, int64_t q_ldh
     a.d_page = a.c.d_page, a.d_group = UDiv::of((uint32_t) a.group);
     a.counters = (uint32_t*) workspace;
     a.part = reinterpret_cast<float*>((char*) workspace + EXL3_ATTN_COUNTER_BYTES);
-    if (requests && (int64_t) tokens * a.group / requests > 16) launch_attn8_prefill(a, dtype, (hipStream_t) stream);
-    else if (dtype == EXL3_FP16) launch<f16>(a, (hipStream_t) stream);
-    else launch<__bf16>(a, (hipStream_t) stream);
+    // Rows of an average request and kv head: up to 16 are one tile of the decode kernel, up to 32 two sets of 16 rows whose workgroups
+    // read the same keys at the same time.  Two sets / one set after the other / chunk kernel, us, fp16: 12 requests of 1000 to 32000 tokens,
+    // 24 rows, 24 heads over 4 of 256: 79 / 93 / 99; 16 of 4000 46 / 60 / 69, one of 1000 17 / 17 / 26; 20 rows, 40 over 8 of 128: 74 / 91 / 87,
+    // 49 / 65 / 65, 12 / 12 / 21; 24 rows, 32 over 8 of 64: 51 / 55 / 63, 38 / 40 / 45, 10 / 10 / 15.  From 33 rows the chunk kernel: eight
+    // of 16000 tokens, 40 rows of 128, 129 us against 143 with four sets; 36 rows of 256, 121 against 120, and 64 of 1000 59 against 78.
+    // The host knows the average alone, not the lengths, so a batch of unlike requests takes the kernel of the many.
+    const int64_t rows = requests ? (int64_t) tokens * a.group / requests : 0;
+    if (rows > 32) launch_attn8_prefill(a, dtype, (hipStream_t) stream);
+    else if (dtype == EXL3_FP16) launch<f16>(a, (int) rows, (hipStream_t) stream);
+    else launch<__bf16>(a, (int) rows, (hipStream_t) stream);
     return hipGetLastError() == hipSuccess ? EXL3_OK : EXL3_ELAUNCH;
 }
