@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(256) rope_kv_write_kernel(RopeArgs a)
     const int64_t tok = blockIdx.x;
     for (int f = threadIdx.x; f < a.rot / 2; f += 256) {
         float s, c;
-        sincospif(2.f * turn_fraction((double) a.pos[tok], a.inv_freq[f]), &s, &c);
+        sincospif(2.f * (float) turn_fraction((double) a.pos[tok], a.inv_freq[f]), &s, &c);
         cs[f] = make_float2(c * a.mscale, s * a.mscale);
     }
     __syncthreads();

@@ -42,16 +42,24 @@ __device__ __forceinline__ float finite_abs(float x)
     return a < INFINITY ? a : 0.f;                      // NaN compares false
 }
 
-// Codes of 8 values, whose quotient by the scale is exact (a power of two): rounded to even by the addition of 1.5 2^23, which leaves
-// the whole number in the sum's low bits; infinities to +-127, and NaN, if there may be any, to 0.
-__device__ __forceinline__ u32x2 codes_of(const float (&x)[8], float inv, bool odd)
+// Codes of 8 values, whose quotient by the scale is exact (a power of two).  Values of at most 127 steps are rounded to even by the
+// addition of 1.5 2^23, which leaves the whole number in the sum's low bits; `odd`: some may be more, infinite or NaN.
+// middle: bit i if value i may be, as far as values off by up to `off` tell, on the other side of the middle between two codes.
+__device__ __forceinline__ u32x2 codes_of(const float (&x)[8], float inv, bool odd, float off, uint32_t& middle)
 {
+    constexpr float MAGIC = 12582912.f;
+    const float limit = fmaf(off, -inv, 0.5f);
     uint32_t b[8];
+    middle = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] = (uint32_t) __float_as_int(fminf(fmaxf(x[i] * inv, -127.f), 127.f) + 12582912.f);
+    for (int i = 0; i < 8; ++i) {
+        const float sum = fmaf(x[i], inv, MAGIC), rest = fmaf(x[i], inv, -(sum - MAGIC));
+        b[i] = (uint32_t) __float_as_int(sum);
+        middle |= fabsf(rest) >= limit ? 1u << i : 0u;
+    }
     if (odd) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) b[i] = x[i] == x[i] ? b[i] : 0u;
+        for (int i = 0; i < 8; ++i) b[i] = x[i] == x[i] ? (uint32_t) (int) rintf(fminf(fmaxf(x[i] * inv, -127.f), 127.f)) : 0u;
     }
     u32x2 r;
 #pragma unroll
@@ -59,6 +67,19 @@ __device__ __forceinline__ u32x2 codes_of(const float (&x)[8], float inv, bool o
         r[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[4 * i + 3], b[4 * i + 2], 0x0C0C0400u),
                                      __builtin_amdgcn_perm(b[4 * i + 1], b[4 * i], 0x0C0C0400u), 0x05040100u);
     return r;
+}
+
+// A rotated element in float64: element e of the head at `head`, in the token at position pos.
+template <class T, int LAYOUT>
+__device__ __forceinline__ double rotated_f64(const uint16_t* head, int e, int rot, int64_t pos, const double* freq, float mscale)
+{
+    auto at = [&](int i) __attribute__((always_inline)) { return (double) (float) __builtin_bit_cast(T, (uint16_t) *(as_global(head) + i)); };
+    const int half = rot / 2;
+    const bool first = LAYOUT == ROPE_PAIRS ? e % 2 == 0 : e < half;
+    const double x = at(e), y = at(LAYOUT == ROPE_PAIRS ? e ^ 1 : first ? e + half : e - half);
+    double s, c;
+    sincospi(2.0 * turn_fraction((double) pos, freq[LAYOUT == ROPE_PAIRS ? e / 2 : first ? e : e - half]), &s, &c);
+    return (x * c + (first ? -y : y) * s) * mscale;
 }
 // codes of a row whose block's scale grew by 1 / f
 __device__ __forceinline__ u32x2 rounded_anew(u32x2 old, float f)
@@ -91,20 +112,24 @@ __device__ __forceinline__ float wave_max(float x)
 // holds 8 elements of k and v of one of the block's 16 rows: new rows from the batch, the others' codes from the cache, requested at
 // once whether the scale will grow or not, with the angles formed meanwhile: a block takes two trips to memory (its slots and
 // positions, then all else), and a further head's is under way while the head before is computed.  The other workgroups rotate q.
+// A rotated k has the code of its exact value: fp32 decides, but for elements that it leaves next to the middle between two codes, which
+// are rotated again in float64 (rotating all of them in float64 took 8192 tokens 62 us instead of 53).
 template <class T, int D, int LAYOUT>
-__global__ void __launch_bounds__(2 * D) rope_kv_write8_kernel(Write8Args a)
+__global__ void __launch_bounds__(2 * D, 4) rope_kv_write8_kernel(Write8Args a)
 {
     constexpr int PIECES = D / 8, THREADS = C8_BLOCK * PIECES, WAVES = THREADS / 64;
     constexpr int FREQS = (D / 2 + 63) / 64;            // frequencies of a lane
     constexpr int QN = 3;                               // pieces of q that a thread has under way
     __shared__ float2 cs[C8_BLOCK][D / 2];
     __shared__ int src[C8_BLOCK];                       // the block's rows: their token in the batch, -1 none
+    __shared__ int64_t pos[C8_BLOCK];                   // ... and its position
+    __shared__ double freqs[D / 2];
     __shared__ float tops[2][WAVES][2];                 // largest values of k and v of each wave; heads take turns
     using V8 = typename Elem<T>::x8;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     auto cos_sin = [&](int64_t pos, double freq) __attribute__((always_inline)) {
         float s, c;
-        sincospif(2.f * turn_fraction((double) pos, freq), &s, &c);
+        sincospif(2.f * (float) turn_fraction((double) pos, freq), &s, &c);
         return make_float2(c * a.mscale, s * a.mscale);
     };
 
@@ -148,6 +173,10 @@ __global__ void __launch_bounds__(2 * D) rope_kv_write8_kernel(Write8Args a)
     double freq[FREQS];
 #pragma unroll
     for (int i = 0; i < FREQS; ++i) freq[i] = lane + 64 * i < a.rot / 2 ? a.inv_freq[lane + 64 * i] : 0.0;
+    if (wave == 0)
+#pragma unroll
+        for (int i = 0; i < FREQS; ++i)
+            if (lane + 64 * i < D / 2) freqs[lane + 64 * i] = freq[i];
     uint64_t begins = __ballot(lane < a.rows && mine >= 0 && mine != prior);
     for (int i = 0; begins; begins &= begins - 1, ++i) {
         if (i % a.turns != my_turn) continue;
@@ -200,22 +229,31 @@ __global__ void __launch_bounds__(2 * D) rope_kv_write8_kernel(Write8Args a)
         for (int r = wave; r < C8_BLOCK; r += WAVES) {
             const int t = src[r];
             if (t < 0) continue;
-            const int64_t pos = a.pos[t];
+            const int64_t p = a.pos[t];
+            if (lane == 0) pos[r] = p;
 #pragma unroll
             for (int i = 0; i < FREQS; ++i)
-                if (lane + 64 * i < a.rot / 2) cs[r][lane + 64 * i] = cos_sin(pos, freq[i]);
+                if (lane + 64 * i < a.rot / 2) cs[r][lane + 64 * i] = cos_sin(p, freq[i]);
         }
         __syncthreads();
         for (int h = h0; h < h1; ++h) {
             if (h + 1 < h1) request(next, 1);
-            float x[8], y[8], top_k = 0.f, top_v = 0.f;
-            bool odd = false;                           // some element of the wave's is an infinity or NaN
+            float x[8], y[8], top_k = 0.f, top_v = 0.f, top_in = 0.f;
+            bool odd = false;                           // some of the thread's elements are infinite, NaN or past all scales
             if (tok >= 0) {
                 const V8 e = __builtin_bit_cast(V8, now.k), g = __builtin_bit_cast(V8, now.v);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     x[i] = (float) e[i];
                     y[i] = (float) g[i];
+                    top_in = fmaxf(top_in, fabsf(x[i]));
+                }
+                if constexpr (LAYOUT == ROPE_HALF) {
+                    const V8 o = __builtin_bit_cast(V8, now.o);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) top_in = fmaxf(top_in, fabsf((float) o[i]));
+                } else if constexpr (LAYOUT == ROPE_ANY) {
+                    top_in = INFINITY;                  // its partners lie anywhere: all are rotated again
                 }
                 rotate8<T, LAYOUT>(now.k, now.o, k, c, a.rot, cs[row], [&](int i, float z) __attribute__((always_inline)) { x[i] = z; });
                 float any = 0.f;
@@ -225,8 +263,8 @@ __global__ void __launch_bounds__(2 * D) rope_kv_write8_kernel(Write8Args a)
                     top_v = fmaxf(top_v, fabsf(y[i]));
                     any = fmaf(x[i], 0.f, fmaf(y[i], 0.f, any));
                 }
+                odd = any != any || fmaxf(top_k, top_v) > 127.f * power2(C8_MOST);
                 if (any != any) {
-                    odd = true;
                     top_k = top_v = 0.f;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -248,19 +286,35 @@ __global__ void __launch_bounds__(2 * D) rope_kv_write8_kernel(Write8Args a)
                 top_k = fmaxf(top_k, tops[turn][i][0]);
                 top_v = fmaxf(top_v, tops[turn][i][1]);
             }
+            // A rotated pair (a, b) in fp32 is off by at most 2^-21 (|a| + |b|) mscale: cosine and sine by 2^-22, products and sum by 2^-23.
+            const float off = 0x1p-20f * top_in * fabsf(a.mscale);
             // the codes of 8 elements or of a row that stays, under the block's scale
-            auto put = [&](float* scale, float was, float top, int8_t* to, const float (&z)[8], u32x4 old) __attribute__((always_inline)) {
+            auto put = [&](auto IS_K, float* scale, float was, float top, int8_t* to, const float (&z)[8], u32x4 old) __attribute__((always_inline)) {
                 const float need = power2(exponent8(top)), had = scale8(was);
                 const bool grown = anew || need > had;
                 const float is = grown ? need : had, inv = reciprocal8(is);
                 if (tid == 0 && grown) *as_global(scale) = is;
                 auto* const dst = reinterpret_cast<g_u32x2*>(as_global(to));
-                if (tok >= 0) *dst = codes_of(z, inv, odd);
-                else if (anew) *dst = u32x2{0u, 0u};
+                if (tok >= 0) {
+                    uint32_t middle;
+                    u32x2 codes = codes_of(z, inv, odd, IS_K ? off : 0.f, middle);
+                    if constexpr (IS_K) {
+                        // what fp32 leaves next to the middle between two codes; v and what is not rotated are exact
+                        middle &= odd ? 0u : (1u << min(max(a.rot - c, 0), 8)) - 1u;
+                        for (; middle; middle &= middle - 1u) {
+                            const int i = __builtin_ctz(middle);
+                            const double q = rint(rotated_f64<T, LAYOUT>(k, c + i, a.rot, pos[row], freqs, a.mscale) * (double) inv);
+                            const uint32_t m = 0xFFu << (8 * (i & 3)), b = ((uint32_t) (int) fmin(fmax(q, -127.0), 127.0) & 0xFFu) << (8 * (i & 3));
+                            codes[0] = i < 4 ? (codes[0] & ~m) | b : codes[0];
+                            codes[1] = i < 4 ? codes[1] : (codes[1] & ~m) | b;
+                        }
+                    }
+                    *dst = codes;
+                } else if (anew) *dst = u32x2{0u, 0u};
                 else if (grown) *dst = rounded_anew(u32x2{old[0], old[1]}, had * inv);
             };
-            put(ks, now.ks, top_k, kc, x, now.k);
-            put(vs, now.vs, top_v, vc, y, now.v);
+            put(std::true_type{}, ks, now.ks, top_k, kc, x, now.k);
+            put(std::false_type{}, vs, now.vs, top_v, vc, y, now.v);
             now = next;
             ks += a.c.ks_ldh, vs += a.c.vs_ldh, kc += a.c.k_ldh, vc += a.c.v_ldh, k += a.k_ldh, v += a.v_ldh;
         }

@@ -6,14 +6,14 @@ namespace exl3 {
 
 // position * freq / (2 pi) less its whole turns.  1 / (2 pi) in two doubles, and each product's rounding error by
 // fma: what is lost is below 2^-100 of the angle, so the fraction is good to 32 bits for any position below 2^53.
-__device__ __forceinline__ float turn_fraction(double position, double freq)
+__device__ __forceinline__ double turn_fraction(double position, double freq)
 {
 #pragma clang fp contract(off)                          // a product that a subtraction absorbs has no error to add
     constexpr double C_HI = 0x1.45f306dc9c883p-3, C_LO = -0x1.6b01ec5417056p-57;
     const double g = freq * C_HI, g_err = fma(freq, C_HI, -g) + freq * C_LO;
     const double turns = position * g, err = fma(position, g, -turns) + position * g_err;
     const double x = (turns - floor(turns)) + err;
-    return (float) (x - floor(x));
+    return x - floor(x);
 }
 
 // What 8 elements of a head from column c on pair with (half layout with whole pieces; else nothing): requested with them, so
