@@ -50,7 +50,7 @@ __device__ __forceinline__ float fp16_rows(u32x4 (&q)[N], RowMax&& row_max)
     }
 }
 
-// many rows a request (exl3_attn8_prefill.hip)
-void launch_attn8_prefill(const Attn8Args& a, int dtype, hipStream_t s);
+// many rows a request, `rows` for each kv head on average (exl3_attn8_prefill.hip)
+void launch_attn8_prefill(const Attn8Args& a, int64_t rows, int dtype, hipStream_t s);
 
 }  // namespace exl3

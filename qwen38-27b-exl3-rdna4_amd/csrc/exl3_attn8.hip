@@ -561,7 +561,7 @@ extern "C" int exl3_paged_attention8(const void* q, int64_t q_ldt, int64_t q_ldh
     // of 16000 tokens, 40 rows of 128, 129 us against 143 with four sets; 36 rows of 256, 121 against 120, and 64 of 1000 59 against 78.
     // The host knows the average alone, not the lengths, so a batch of unlike requests takes the kernel of the many.
     const int64_t rows = requests ? (int64_t) tokens * a.group / requests : 0;
-    if (rows > 32) launch_attn8_prefill(a, dtype, (hipStream_t) stream);
+    if (rows > 32) launch_attn8_prefill(a, rows, dtype, (hipStream_t) stream);
     else if (dtype == EXL3_FP16) launch<f16>(a, (int) rows, (hipStream_t) stream);
     else launch<__bf16>(a, (int) rows, (hipStream_t) stream);
     return hipGetLastError() == hipSuccess ? EXL3_OK : EXL3_ELAUNCH;

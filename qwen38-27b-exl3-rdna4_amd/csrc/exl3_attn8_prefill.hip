@@ -150,14 +150,16 @@ __global__ void __launch_bounds__((Prefill8<T, D, W>::THREADS), (Prefill8<T, D, 
             for (int i = 0; i < AE; ++i) o[d][i] = 0.f;
         float m = LOWEST, l = 0.f;
 
-        auto page_of = [&](int s) __attribute__((always_inline)) {
+        // every row of the wave sees every key of the steps whose first keys are whole_from .. whole_to, if their pages are pages
+        const int whole_from = a.window ? w_last - a.window + 1 : 0, whole_to = min(w_first - (X::KEYS - 1), a.cap - X::KEYS);
+        // a page is looked up a step before it is needed: a wait for it would be a trip to memory each step
+        auto look_up = [&](int s) __attribute__((always_inline)) {
             const int key = X::KEYS * s + KW * wave;
-            int p = -1;
-            if (key < tile.hi) {
-                p = table[a.d_page.div((uint32_t) key)];
-                if ((unsigned) p >= (unsigned) a.pages) p = -1;
-            }
-            return __builtin_amdgcn_readfirstlane(p);
+            return key < tile.hi ? table[a.d_page.div((uint32_t) key)] : -1;
+        };
+        auto page_of = [&](int looked_up) __attribute__((always_inline)) {
+            const int p = __builtin_amdgcn_readfirstlane(looked_up);
+            return (unsigned) p >= (unsigned) a.pages ? -1 : p;
         };
         u32x2 kr[LI], vr[LI];
         float skr, svr;
@@ -194,13 +196,10 @@ __global__ void __launch_bounds__((Prefill8<T, D, W>::THREADS), (Prefill8<T, D, 
             if (!rows_here || k0 > w_last || (a.window && k0 + X::KEYS - 1 <= w_first - a.window)) return;
             // of the step's four blocks
             f32x4 bl[4];
-            bool pages = true;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                bl[i] = sh.block[buf][i * (X::WAVES / 4)];
-                pages = pages && __builtin_amdgcn_readfirstlane(__float_as_int(bl[i][3])) != 0;
-            }
-            const bool whole = pages && k0 + X::KEYS - 1 <= w_first && (!a.window || k0 > w_last - a.window) && k0 + X::KEYS <= a.cap;
+            for (int i = 0; i < 4; ++i) bl[i] = sh.block[buf][i * (X::WAVES / 4)];
+            const int pages = __builtin_amdgcn_readfirstlane(__float_as_int(fminf(fminf(bl[0][3], bl[1][3]), fminf(bl[2][3], bl[3][3]))));
+            const bool whole = (int) (pages != 0) & (int) (k0 >= whole_from) & (int) (k0 <= whole_to);
             // Two halves of 32 keys, each of scores, softmax and products with V; the matrix unit works on the second half's scores
             // while the first's exponentials are formed, and on the first's products while the second's are.
             Acc st[2][TH];
@@ -331,7 +330,8 @@ __global__ void __launch_bounds__((Prefill8<T, D, W>::THREADS), (Prefill8<T, D, 
         };
 
         if (tile.lo < tile.hi) {
-            int p0 = page_of(s0), p1 = page_of(s0 + 1), p2 = page_of(s0 + 2);
+            const int p0 = page_of(look_up(s0));
+            int p1 = page_of(look_up(s0 + 1)), next = look_up(s0 + 2);
             request(s0, p0);
             store(std::integral_constant<int, 0>{}, s0, p0);
             if (s0 + 1 < s1) request(s0 + 1, p1);
@@ -341,8 +341,8 @@ __global__ void __launch_bounds__((Prefill8<T, D, W>::THREADS), (Prefill8<T, D, 
                 compute(BUF, s);
                 if (s + 1 == s1) return false;
                 store(std::integral_constant<int, 1 - BUF>{}, s + 1, p1);
-                p1 = p2;
-                p2 = page_of(s + 3);
+                p1 = page_of(next);
+                next = look_up(s + 3);
                 if (s + 2 < s1) request(s + 2, p1);
                 __syncthreads();
                 return true;
@@ -519,20 +519,23 @@ void launch_one(const Attn8Args& a, hipStream_t s)
 }
 
 template <class T>
-void launch(const Attn8Args& a, hipStream_t s)
+void launch(const Attn8Args& a, int64_t rows, hipStream_t s)
 {
+    // Many rows: 256 a tile, whose keys are made fp16 once for eight waves instead of four (2048 tokens over 12000, 40 heads over 8 of
+    // 128: 664 us against 733; 512 over none 38 against 32).  Heads of 64 gain less (380 against 405) and lose as much without a context.
     if (a.c.d == 64) launch_one<T, 64, 4>(a, s);
-    else if (a.c.d == 128) launch_one<T, 128, 4>(a, s);
-    else launch_one<T, 256, 8>(a, s);
+    else if (a.c.d == 256) launch_one<T, 256, 8>(a, s);
+    else if (rows > 4096) launch_one<T, 128, 8>(a, s);
+    else launch_one<T, 128, 4>(a, s);
 }
 
 }  // namespace
 
 namespace exl3 {
 
-void launch_attn8_prefill(const Attn8Args& a, int dtype, hipStream_t s)
+void launch_attn8_prefill(const Attn8Args& a, int64_t rows, int dtype, hipStream_t s)
 {
-    dtype == EXL3_FP16 ? launch<f16>(a, s) : launch<__bf16>(a, s);
+    dtype == EXL3_FP16 ? launch<f16>(a, rows, s) : launch<__bf16>(a, rows, s);
 }
 
 }  // namespace exl3
