@@ -2,7 +2,7 @@
 
     x -> qkv (EXL3) -> rope_kv_write -> paged_attention -> o (EXL3) -> y
 
-with the batch's bookkeeping (batch_plan) on the GPU.  `python examples/attention_block.py` prefills ragged prompts in
+with the batch's bookkeeping (batch_plan) on the GPU, over a cache in 16 bits or, with `--cache-bits 8`, in 8.  `python examples/attention_block.py` prefills ragged prompts in
 one step, then decodes: eagerly, and by replaying one captured HIP graph whose lengths grow on the GPU.  Weights are
 seeded synthetic ones (exl3rocm.synth).
 """
@@ -16,14 +16,14 @@ import torch
 
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "qwen38-27b-exl3-rdna4_amd"))
 
-from exl3rocm import ops, paged, synth  # noqa: E402,F401
+from exl3rocm import ops, paged, paged8, synth  # noqa: E402,F401
 
 
 class AttentionBlock:
-    """qkv, attention over a paged cache, o; mul1 codebook, fp16."""
+    """qkv, attention over a paged cache (fp16, or int8 with a scale for each 16 tokens and head), o; mul1 codebook, fp16."""
 
     def __init__(self, hidden=5120, q_heads=40, kv_heads=8, head_dim=128, bits=4, rot_dim=None, base=1e6, scaling=None,
-                 pages=4096, page_size=16, name="attention_block"):
+                 pages=4096, page_size=16, name="attention_block", cache_bits=16):
         self.q_heads, self.kv_heads, self.head_dim, self.bits = q_heads, kv_heads, head_dim, bits
         widths = [q_heads * head_dim, kv_heads * head_dim, kv_heads * head_dim]
         def load(part, k, n):
@@ -34,7 +34,11 @@ class AttentionBlock:
         self.qkv = [load(f"qkv{i}", hidden, n) for i, n in enumerate(widths)]
         self.o = load("o", widths[0], hidden)
         self.inv_freq, self.mscale = paged.rope_frequencies(rot_dim or head_dim, base, scaling)
-        self.k_cache, self.v_cache = paged.new_cache(pages, page_size, kv_heads, head_dim)
+        op = torch.ops.exl3rocm
+        if cache_bits == 8:
+            self.cache, self.write, self.attend = paged8.new_cache8(pages, page_size, kv_heads, head_dim), op.rope_kv_write8, op.paged_attention8
+        else:
+            self.cache, self.write, self.attend = paged.new_cache(pages, page_size, kv_heads, head_dim), op.rope_kv_write, op.paged_attention
 
     def __call__(self, x, step, block_table):
         """x [T, hidden] fp16; step: batch_plan's result."""
@@ -42,8 +46,8 @@ class AttentionBlock:
         op, T, d = torch.ops.exl3rocm, x.shape[0], self.head_dim
         qkv = op.linear_groups(x, *(list(t) for t in zip(*self.qkv)), [self.bits] * 3, False, True)
         q, k, v = (t.view(T, -1, d) for t in qkv.split([self.q_heads * d, self.kv_heads * d, self.kv_heads * d], 1))
-        q = op.rope_kv_write(q, k, v, positions, slots, self.k_cache, self.v_cache, self.inv_freq, self.mscale)
-        a = op.paged_attention(q, self.k_cache, self.v_cache, block_table, cu_q, seq_lens, d ** -0.5)
+        q = self.write(q, k, v, positions, slots, *self.cache, self.inv_freq, self.mscale)
+        a = self.attend(q, *self.cache, block_table, cu_q, seq_lens, d ** -0.5)
         return op.linear(a.view(T, -1), *self.o, self.bits, False, True)
 
 
@@ -82,9 +86,10 @@ def main():
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     ap.add_argument("--prompts", type=int, nargs="*", default=[517, 64, 1200, 33, 2000, 801, 16, 290])
     ap.add_argument("--steps", type=int, default=64)
+    ap.add_argument("--cache-bits", type=int, default=16, choices=(8, 16))
     a = ap.parse_args()
     R, total = len(a.prompts), sum(a.prompts)
-    block = AttentionBlock()
+    block = AttentionBlock(cache_bits=a.cache_bits)
     reqs = Requests(R, 4096, 16, max(a.prompts) + a.steps + 16)
     g = torch.Generator(device="cuda").manual_seed(0)
     x = torch.randn(total, 5120, device="cuda", generator=g).half()

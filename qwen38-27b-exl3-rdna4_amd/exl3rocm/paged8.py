@@ -44,6 +44,8 @@ def new_cache8(pages: int, page_size: int, kv_heads: int, head_dim: int, device=
 
 
 _pack = Struct("=16q4i").pack           # exl3_cache8 of the C interface
+# torch.empty with a type and a device takes an eager call twice the host time of empty_like
+_like, _contiguous = torch.empty_like, torch.contiguous_format
 
 
 def _cache8(what: str, kc: torch.Tensor, vc: torch.Tensor, ks: torch.Tensor, vs: torch.Tensor, gpu: int):
@@ -99,7 +101,7 @@ def rope_kv_write8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions:
     _ints("rope_kv_write8: positions", positions, gpu, torch.int64, T)
     _ints("rope_kv_write8: slots", slots, gpu, torch.int64, T)
     _ints("rope_kv_write8: inv_freq", inv_freq, gpu, torch.float64)
-    out = torch.empty(qs, dtype=dt, device=q.device)
+    out = _like(q, memory_format=_contiguous)
     _launch("rope_kv_write8", gpu, "exl3_rope_kv_write8", q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, positions.data_ptr(),
             slots.data_ptr(), out.data_ptr(), cache, inv_freq.data_ptr(), mscale, T, hq, 2 * inv_freq.numel(), interleaved, _DTYPES[dt])
     return out
@@ -113,8 +115,9 @@ def kv_read8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor
     cache, heads, d = _cache8("kv_read8", k_cache, v_cache, k_scale, v_scale, gpu)
     _need(dtype in _DTYPES, f"kv_read8: dtype must be fp16 or bf16, got {dtype}")
     _ints("kv_read8: slots", slots, gpu, torch.int64)
-    T, dev = slots.numel(), k_cache.device
-    k, v = torch.empty(T, heads, d, dtype=dtype, device=dev), torch.empty(T, heads, d, dtype=dtype, device=dev)
+    T = slots.numel()
+    k = torch.empty(T, heads, d, dtype=dtype, device=k_cache.device)
+    v = _like(k)
     _launch("kv_read8", gpu, "exl3_kv_read8", cache, slots.data_ptr(), k.data_ptr(), v.data_ptr(), T, _DTYPES[dtype])
     return k, v
 
@@ -137,12 +140,11 @@ def paged_attention8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     _ints("paged_attention8: cu_q", cu_q, gpu, torch.int32, R + 1)
     cols, ld = _table("paged_attention8", block_table, gpu, R)
     _need(0 <= window <= 1 << 30, "paged_attention8: window from 0 (none) to 2 ** 30")
-    dev = q.device
-    out = torch.empty(qs, dtype=dt, device=dev)
+    out = _like(q, memory_format=_contiguous)
     st = paged._raw_stream(gpu)
     ws = paged._workspaces.get((gpu, st))
     if ws is None:
-        ws = paged._workspace(dev, st)
+        ws = paged._workspace(q.device, st)
     _launch("paged_attention8", gpu, "exl3_paged_attention8", q.data_ptr(), qt, qh, cache, block_table.data_ptr(), ld, cols, cu_q.data_ptr(),
             seq_lens.data_ptr(), out.data_ptr(), hq * d, d, T, R, hq, scale, window, _DTYPES[dt], ws.data_ptr(), ws.numel())
     return out
