@@ -27,6 +27,9 @@ template <> struct Codes<4> { typedef u32x4 T; typedef gc_u32x4 G; };
 // steps with a softmax of its own, K and V go from memory into registers and are made operands there.
 //   K: a lane holds key l & 15, bytes 64 c + 16 (l >> 4) .. + 15: two products' 8 elements each, so q's lane holds the same columns
 //   V: a lane holds E = D / 16 columns E (l & 15) .. of its keys, and product e is made of column e of pairs of keys
+// 16 rows: bound by memory.  96 decodes of 100 to 16000 tokens, 40 heads over 8 of 128 (535 MB), 117 us, 4.6 TB/s (ends of tiles);
+// two of 131000, 24 over 4 of 256 (728 MB), 127 us, 5.8 TB/s.  17 to 32 rows: by waits and issue, 12 requests' drafts (189 MB, 24 rows of
+// 256) 65 us, 2.9 TB/s; vector instructions take 33 % of the cycles, waits 41 % of the waves' time.
 template <class T, int D, int WAVES, int KEYS, int S>
 struct Decode8 {
     static constexpr int ROWS = 16, TILE = ROWS * S, THREADS = 64 * WAVES;
@@ -59,7 +62,7 @@ struct Decode8 {
 };
 
 // Parts of a tile summed in order: part i at slot_at(i) (floats), rows x D outputs, then (maximum, sum) a row.  Z elements of a thread
-// and B parts of each are in flight.
+// and B parts of each are in flight (16 parts: the same time).
 template <int D, int ROWS, int THREADS, class SlotAt, class Put>
 __device__ __forceinline__ void join8(__amdgpu_buffer_rsrc_t prs, int parts, int rows, SlotAt&& slot_at, Put&& put)
 {

@@ -32,6 +32,9 @@ __device__ __forceinline__ void here(u32x4& a, u32x4& b, float& c)
 //         transposing LDS reads (16 lanes read 4 keys x 16 columns, lane i gets column i of the 4)
 // Heads of 256: 16 rows a wave (16x16x32, row l & 15, keys 4 (l >> 4) + (i & 3) of two blocks).
 // A lane's row is the same in S^T and O^T.  LDS rows are padded so that no bank is met twice.
+// 2048 tokens over 12000, 40 heads over 8 of 128 (546 GFLOP): 644 to 664 us, 820 to 850 TFLOPS, bound by products and vector work that
+// overlap little, and waits.  1501 over 9001, 24 over 4 of 256 (360 GFLOP): 573 us, 630 TFLOPS, bound by LDS reads (16 rows a wave).  Not kept:
+// the step's halves pipelined over steps 826, two groups of four waves that take products and vector work in turn 729.
 template <class T, int D, int W>
 struct Prefill8 {
     static constexpr int RW = D == 256 ? 16 : 32;       // rows of a wave
@@ -84,6 +87,11 @@ struct Prefill8 {
     // place of result e of a half step's 32 keys (less 4 (l / RW)), and of quad g of column tile d
     static constexpr int key_of(int e) { return RW == 32 ? 8 * (e >> 2) + (e & 3) : 16 * (e >> 2) + (e & 3); }
     static constexpr int col_of(int d, int g) { return RW * d + 8 * g; }
+    // The columns of K and Q that lanes of group hg have in product c are q_col(hg) + Q_STEP c and the 7 after them; any order of D
+    // does.  16 lanes' 16-byte LDS reads pass at once, of two groups where a group has 16: theirs lie 128 columns (all
+    // banks) apart.
+    static constexpr int Q_STEP = RW == 32 ? 16 : 8;
+    static __device__ __forceinline__ int q_col(int hg) { return RW == 32 ? 8 * hg : 128 * (hg & 1) + 64 * (hg >> 1); }
 };
 
 template <class T, int D, int W>
@@ -117,7 +125,7 @@ __global__ void __launch_bounds__((Prefill8<T, D, W>::THREADS), (Prefill8<T, D, 
     // LDS addresses of the lane's writes and reads: what the instructions' offsets are added to
     lchar* const k_put = (lchar*) &sh.k[0][(KW * wave + st_row) * X::K_LD + 8 * st_piece];
     lchar* const v_put = (lchar*) &sh.v[0][(KW * wave + st_row) * X::V_LD + 8 * st_piece];
-    lchar* const k_get = (lchar*) &sh.k[0][cr * X::K_LD + 8 * hg];
+    lchar* const k_get = (lchar*) &sh.k[0][cr * X::K_LD + X::q_col(hg)];
     lchar* const v_get = (lchar*) &sh.v[0][(4 * hg + tr_row) * X::V_LD + 16 * tr_half + 4 * tr_q];
 
     while (true) {
@@ -138,9 +146,9 @@ __global__ void __launch_bounds__((Prefill8<T, D, W>::THREADS), (Prefill8<T, D, 
         const int upto = min(pos, a.cap - 1), from = a.window ? pos - a.window : -1;
         u32x4 q[KS];
         {
-            gc_u16* const src = as_global(a.q) + (int64_t) (wk.tok0 + tok) * a.q_ldt + (int64_t) (wk.h * a.group + min(xl, rows - 1) - tok * a.group) * a.q_ldh + 8 * hg;
+            gc_u16* const src = as_global(a.q) + (int64_t) (wk.tok0 + tok) * a.q_ldt + (int64_t) (wk.h * a.group + min(xl, rows - 1) - tok * a.group) * a.q_ldh + X::q_col(hg);
 #pragma unroll
-            for (int c = 0; c < KS; ++c) q[c] = flipped(*reinterpret_cast<gc_u32x4*>(src + X::KD * c), a.flip);
+            for (int c = 0; c < KS; ++c) q[c] = flipped(*reinterpret_cast<gc_u32x4*>(src + X::Q_STEP * c), a.flip);
         }
         const float row_scale = row_scale_of(a.scale, fp16_rows<T>(q, [](float x) __attribute__((always_inline)) { return X::row_max(x); }));
         Acc o[DT];
@@ -209,7 +217,7 @@ __global__ void __launch_bounds__((Prefill8<T, D, W>::THREADS), (Prefill8<T, D, 
                 for (int t = 0; t < TH; ++t)
 #pragma unroll
                     for (int c = 0; c < KS; ++c)
-                        kf[t][c] = *reinterpret_cast<lu32x4*>(k_get + 2 * ((buf * X::KEYS + 32 * y + RW * t) * X::K_LD + X::KD * c));
+                        kf[t][c] = *reinterpret_cast<lu32x4*>(k_get + 2 * ((buf * X::KEYS + 32 * y + RW * t) * X::K_LD + X::Q_STEP * c));
             };
             auto read_v = [&](u32x4 (&f)[NB], int y, int d) __attribute__((always_inline)) {
 #pragma unroll
