@@ -53,6 +53,7 @@ struct Prefill8 {
     static constexpr int TH = 32 / RW;                  // key tiles of a half step (32 keys)
     static constexpr int NB = AE * TH / 8;              // operands of its probabilities
     static constexpr int HALF = TH * AE / 2;            // a lane's results of each of its two blocks
+    static constexpr int VD = RW == 32 ? 2 : 4;         // column tiles of V on their way from LDS
     using Acc = std::conditional_t<RW == 32, f32x16, f32x4>;
     static constexpr float SHIFT = 8.f;                 // probabilities are held times 2^8
     static constexpr int K_LD = D + 8, V_LD = RW == 32 ? D + 32 : D + 16;  // LDS rows, halves
@@ -99,7 +100,7 @@ __global__ void __launch_bounds__((Prefill8<T, D, W>::THREADS), (Prefill8<T, D, 
 {
     using X = Prefill8<T, D, W>;
     using Acc = typename X::Acc;
-    constexpr int LI = X::LI, KS = X::KS, DT = X::DT, CH = X::CH, RW = X::RW, KW = X::KW, AE = X::AE, TH = X::TH, NB = X::NB, HALF = X::HALF, QD = AE / 4;
+    constexpr int LI = X::LI, KS = X::KS, DT = X::DT, CH = X::CH, RW = X::RW, KW = X::KW, AE = X::AE, TH = X::TH, NB = X::NB, HALF = X::HALF, VD = X::VD, QD = AE / 4;
     __shared__ typename X::Shared sh;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), cr = lane % RW, hg = lane / RW;
     // consecutive shares to one XCD (workgroups go round the 8 XCDs): they read the same head's K and V
@@ -211,7 +212,7 @@ __global__ void __launch_bounds__((Prefill8<T, D, W>::THREADS), (Prefill8<T, D, 
             // Two halves of 32 keys, each of scores, softmax and products with V; the matrix unit works on the second half's scores
             // while the first's exponentials are formed, and on the first's products while the second's are.
             Acc st[2][TH];
-            u32x4 kf[TH][KS], pb[2][NB], vf[2][NB];
+            u32x4 kf[TH][KS], pb[2][NB], vf[VD][NB];
             auto read_k = [&](int y) __attribute__((always_inline)) {
 #pragma unroll
                 for (int t = 0; t < TH; ++t)
@@ -284,7 +285,7 @@ __global__ void __launch_bounds__((Prefill8<T, D, W>::THREADS), (Prefill8<T, D, 
             };
             auto products = [&](int y, int d) __attribute__((always_inline)) {
 #pragma unroll
-                for (int b = 0; b < NB; ++b) o[d] = X::product(vf[d & 1][b], pb[y][b], o[d]);
+                for (int b = 0; b < NB; ++b) o[d] = X::product(vf[d % VD][b], pb[y][b], o[d]);
             };
             auto shrink = [&](float c) __attribute__((always_inline)) {
                 if (__any(c != 1.f)) {
@@ -308,16 +309,16 @@ __global__ void __launch_bounds__((Prefill8<T, D, W>::THREADS), (Prefill8<T, D, 
             here(pb[0][0], pb[0][NB - 1], l0);
             l = l * c0 + l0;
             const float c1 = maximum(1);
-            read_v(vf[0], 0, 0);
-            read_v(vf[1], 0, 1);
+#pragma unroll
+            for (int d = 0; d < VD; ++d) read_v(vf[d], 0, d);
             float l1 = exponentials(1);
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 products(0, d);
-                if (d + 2 < DT) read_v(vf[d & 1], 0, d + 2);
-                else read_v(vf[d & 1], 1, d + 2 - DT);
+                if (d + VD < DT) read_v(vf[d % VD], 0, d + VD);
+                else read_v(vf[d % VD], 1, d + VD - DT);
             }
-            __builtin_amdgcn_sched_group_barrier(0x100, 4 * NB, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * VD * NB, 0);
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
 #pragma unroll
@@ -333,7 +334,7 @@ __global__ void __launch_bounds__((Prefill8<T, D, W>::THREADS), (Prefill8<T, D, 
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 products(1, d);
-                if (d + 2 < DT) read_v(vf[d & 1], 1, d + 2);
+                if (d + VD < DT) read_v(vf[d % VD], 1, d + VD);
             }
         };
 
