@@ -57,7 +57,7 @@ __device__ __forceinline__ u32x2 codes_of(const float (&x)[8], float inv, bool o
         b[i] = (uint32_t) __float_as_int(sum);
         middle |= fabsf(rest) >= limit ? 1u << i : 0u;
     }
-    if (odd) {
+    if (__builtin_expect(odd, 0)) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) b[i] = x[i] == x[i] ? (uint32_t) (int) rintf(fminf(fmaxf(x[i] * inv, -127.f), 127.f)) : 0u;
     }
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(2 * D, 4) rope_kv_write8_kernel(Write8Args a)
                     any = fmaf(x[i], 0.f, fmaf(y[i], 0.f, any));
                 }
                 odd = any != any || fmaxf(top_k, top_v) > 127.f * power2(C8_MOST);
-                if (any != any) {
+                if (__builtin_expect(any != any, 0)) {
                     top_k = top_v = 0.f;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -290,8 +290,13 @@ __global__ void __launch_bounds__(2 * D, 4) rope_kv_write8_kernel(Write8Args a)
             }
             // A rotated pair (a, b) in fp32 is off by at most 2^-21 (|a| + |b|) mscale: cosine and sine by 2^-22, products and sum by 2^-23.
             const float off = 0x1p-20f * top_in * fabsf(a.mscale);
-            // the codes of 8 elements or of a row that stays, under the block's scale
-            auto put = [&](auto IS_K, float* scale, float was, float top, int8_t* to, const float (&z)[8], u32x4 old) __attribute__((always_inline)) {
+            // The codes of 8 elements or of a row that stays, under the block's scale: of k, then of v by the same code (two copies of it:
+            // 2048 tokens of 4 heads of 256 27.2 us instead of 25.8, 128 decodes over 8 of 128 8.2 instead of 7.8).
+            float top = top_k, was = now.ks, *scale = ks;
+            int8_t* to = kc;
+            u32x4 old = now.k;
+#pragma unroll 1
+            for (bool is_k = true;; is_k = false) {
                 const float need = power2(exponent8(top)), had = scale8(was);
                 const bool grown = anew || need > had;
                 const float is = grown ? need : had, inv = reciprocal8(is);
@@ -299,24 +304,24 @@ __global__ void __launch_bounds__(2 * D, 4) rope_kv_write8_kernel(Write8Args a)
                 auto* const dst = reinterpret_cast<g_u32x2*>(as_global(to));
                 if (tok >= 0) {
                     uint32_t middle;
-                    u32x2 codes = codes_of(z, inv, odd, IS_K ? off : 0.f, middle);
-                    if constexpr (IS_K) {
-                        // what fp32 leaves next to the middle between two codes; v and what is not rotated are exact
-                        middle &= odd ? 0u : (1u << min(max(a.rot - c, 0), 8)) - 1u;
-                        for (; middle; middle &= middle - 1u) {
-                            const int i = __builtin_ctz(middle);
-                            const double q = rint(rotated_f64<T, LAYOUT>(k, c + i, a.rot, pos[row], freqs, a.mscale) * (double) inv);
-                            const uint32_t m = 0xFFu << (8 * (i & 3)), b = ((uint32_t) (int) fmin(fmax(q, -127.0), 127.0) & 0xFFu) << (8 * (i & 3));
-                            codes[0] = i < 4 ? (codes[0] & ~m) | b : codes[0];
-                            codes[1] = i < 4 ? codes[1] : (codes[1] & ~m) | b;
-                        }
+                    u32x2 codes = codes_of(x, inv, odd, off, middle);
+                    // what fp32 leaves next to the middle between two codes; v and what is not rotated are exact
+                    middle &= odd || !is_k ? 0u : (1u << min(max(a.rot - c, 0), 8)) - 1u;
+                    for (; __builtin_expect(middle != 0, 0); middle &= middle - 1u) {
+                        const int i = __builtin_ctz(middle);
+                        const double q = rint(rotated_f64<T, LAYOUT>(k, c + i, a.rot, pos[row], freqs, a.mscale) * (double) inv);
+                        const uint32_t m = 0xFFu << (8 * (i & 3)), b = ((uint32_t) (int) fmin(fmax(q, -127.0), 127.0) & 0xFFu) << (8 * (i & 3));
+                        codes[0] = i < 4 ? (codes[0] & ~m) | b : codes[0];
+                        codes[1] = i < 4 ? codes[1] : (codes[1] & ~m) | b;
                     }
                     *dst = codes;
                 } else if (anew) *dst = u32x2{0u, 0u};
                 else if (grown) *dst = rounded_anew(u32x2{old[0], old[1]}, had * inv);
-            };
-            put(std::true_type{}, ks, now.ks, top_k, kc, x, now.k);
-            put(std::false_type{}, vs, now.vs, top_v, vc, y, now.v);
+                if (!is_k) break;
+                top = top_v, was = now.vs, scale = vs, to = vc, old = now.v;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = y[i];
+            }
             now = next;
             ks += a.c.ks_ldh, vs += a.c.vs_ldh, kc += a.c.k_ldh, vc += a.c.v_ldh, k += a.k_ldh, v += a.v_ldh;
         }
