@@ -559,9 +559,9 @@ extern "C" int exl3_paged_attention8(const void* q, int64_t q_ldt, int64_t q_ldh
     a.part = reinterpret_cast<float*>((char*) workspace + EXL3_ATTN_COUNTER_BYTES);
     // Rows of an average request and kv head: up to 16 are one tile of the decode kernel, up to 32 two sets of 16 rows whose workgroups
     // read the same keys at the same time.  Two sets / one set after the other / chunk kernel, us, fp16: 12 requests of 1000 to 32000 tokens,
-    // 24 rows, 24 heads over 4 of 256: 79 / 93 / 99; 16 of 4000 46 / 60 / 69, one of 1000 17 / 17 / 26; 20 rows, 40 over 8 of 128: 74 / 91 / 87,
-    // 49 / 65 / 65, 12 / 12 / 21; 24 rows, 32 over 8 of 64: 51 / 55 / 63, 38 / 40 / 45, 10 / 10 / 15.  From 33 rows the chunk kernel: eight
-    // of 16000 tokens, 40 rows of 128, 129 us against 143 with four sets; 36 rows of 256, 121 against 120, and 64 of 1000 59 against 78.
+    // 24 rows, 24 heads over 4 of 256: 77 / 93 / 89; 16 of 4000 46 / 60 / 61, one of 1000 17 / 17 / 24; 20 rows, 40 over 8 of 128: 73 / 91 / 80,
+    // 49 / 65 / 59, 12 / 12 / 20; 24 rows, 32 over 8 of 64: 50 / 55 / 57, 36 / 40 / 40, 10 / 10 / 15.  From 33 rows the chunk kernel: eight
+    // of 16000 tokens, 40 rows of 128, 119 us against 143 with four sets; 36 rows of 256, 102 against 120, and 64 of 1000 53 against 78.
     // The host knows the average alone, not the lengths, so a batch of unlike requests takes the kernel of the many.
     const int64_t rows = requests ? (int64_t) tokens * a.group / requests : 0;
     if (rows > 32) launch_attn8_prefill(a, rows, dtype, (hipStream_t) stream);

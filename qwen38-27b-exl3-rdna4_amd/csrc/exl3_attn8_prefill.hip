@@ -32,9 +32,10 @@ __device__ __forceinline__ void here(u32x4& a, u32x4& b, float& c)
 //         transposing LDS reads (16 lanes read 4 keys x 16 columns, lane i gets column i of the 4)
 // Heads of 256: 16 rows a wave (16x16x32, row l & 15, keys 4 (l >> 4) + (i & 3) of two blocks).
 // A lane's row is the same in S^T and O^T.  LDS rows are padded so that no bank is met twice.
-// 2048 tokens over 12000, 40 heads over 8 of 128 (546 GFLOP): 644 to 664 us, 820 to 850 TFLOPS, bound by products and vector work that
-// overlap little, and waits.  1501 over 9001, 24 over 4 of 256 (360 GFLOP): 573 us, 630 TFLOPS, bound by LDS reads (16 rows a wave).  Not kept:
-// the step's halves pipelined over steps 826, two groups of four waves that take products and vector work in turn 729.
+// 2048 tokens over 12000, 40 heads over 8 of 128 (546 GFLOP): 640 us, 853 TFLOPS, bound by products and vector work that
+// overlap little, and waits.  1501 over 9001, 24 over 4 of 256 (360 GFLOP): 495 us, 727 TFLOPS, bound by LDS reads (16 rows a wave).  Not kept:
+// the step's halves pipelined over steps 826, two groups of four waves that take products and vector work in turn 729, the next step's
+// codes stored beside the last products 796 (spills); 32 rows a wave for heads of 256 (one wave a SIMD, spills) 703.
 template <class T, int D, int W>
 struct Prefill8 {
     static constexpr int RW = D == 256 ? 16 : 32;       // rows of a wave
@@ -53,7 +54,7 @@ struct Prefill8 {
     static constexpr int TH = 32 / RW;                  // key tiles of a half step (32 keys)
     static constexpr int NB = AE * TH / 8;              // operands of its probabilities
     static constexpr int HALF = TH * AE / 2;            // a lane's results of each of its two blocks
-    static constexpr int VD = RW == 32 ? 2 : 4;         // column tiles of V on their way from LDS
+    static constexpr int VD = RW == 32 ? 2 : 4;         // column tiles of V on their way from LDS (two of heads of 256: 4 % slower)
     using Acc = std::conditional_t<RW == 32, f32x16, f32x4>;
     static constexpr float SHIFT = 8.f;                 // probabilities are held times 2^8
     static constexpr int K_LD = D + 8, V_LD = RW == 32 ? D + 32 : D + 16;  // LDS rows, halves
@@ -359,13 +360,24 @@ __global__ void __launch_bounds__((Prefill8<T, D, W>::THREADS), (Prefill8<T, D, 
             for (int s = s0; turn(std::integral_constant<int, 0>{}, s) && turn(std::integral_constant<int, 1>{}, s + 1); s += 2) {}
         }
 
+        // Arguments read anew, and indexes formed anew: kept in registers through the steps, what the join needs pushes out what they need
+        // (2048 tokens over 12000, heads of 256: 922 us instead of 874).
+        auto* args = (__attribute__((address_space(4))) const Attn8Args*) __builtin_amdgcn_kernarg_segment_ptr();
+        int wg_here = wg, tid_here = tid;
+        asm volatile("" : "+s"(args), "+s"(wg_here), "+v"(tid_here));
+        const int wg = wg_here, tid = tid_here, lane = tid & 63;
+        const UDiv d_group{args->d_group.m, args->d_group.s1, args->d_group.s2};
+        const int64_t o_ldt = args->o_ldt, o_ldh = args->o_ldh;
+        uint16_t* const out = args->out;
+        uint32_t* const counters = args->counters;
+        const int group_heads = args->group;
         // a wave's 32 rows, or their part
         const bool starts = off == 0, ends = off + n_steps == tile.steps;
         l = X::row_sum(l);
         // column tiles d0 .. d0 + N - 1 of the output
         auto put = [&](auto D0, auto N, const Acc* sum, float total) __attribute__((always_inline)) {
             if (xl < rows) {
-                auto* const dst = as_global(a.out) + (int64_t) (wk.tok0 + tok) * a.o_ldt + (int64_t) (wk.h * a.group + xl - tok * a.group) * a.o_ldh + 4 * hg;
+                auto* const dst = as_global(out) + (int64_t) (wk.tok0 + tok) * o_ldt + (int64_t) (wk.h * group_heads + xl - tok * group_heads) * o_ldh + 4 * hg;
 #pragma unroll
                 for (int d = 0; d < N; ++d)
 #pragma unroll
@@ -376,30 +388,50 @@ __global__ void __launch_bounds__((Prefill8<T, D, W>::THREADS), (Prefill8<T, D, 
         if (starts && ends) {
             put(std::integral_constant<int, 0>{}, std::integral_constant<int, DT>{}, o, l);
         } else {
-            // A part moves as it lies in the registers (a lane's 16 bytes next to its neighbours').  The workgroup that
-            // finds all others' parts written joins them with its own, in the order of the workgroups, and writes none.  Many
-            // parts of few rows (drafts over a long context) are all written, and every thread of the last workgroup sums some
-            // of the live rows' elements, eight parts in flight: where that takes less than half as many turns of waiting
-            // (1.5 us each) as one part after the other.
+            // A part moves as it lies in the registers (a lane's 16 bytes next to its neighbours').  Few parts of many rows: the workgroup
+            // that finds all others' parts written joins them with its own, in the order of the workgroups, and writes none.
+            // Else all are written, and every thread of a last workgroup sums some of the live rows' elements, eight parts in flight:
+            // where that takes less than half as many turns of waiting (2 us each) as there are parts (1 us each one after the other).  So
+            // do two levels, as in the decode kernel (exl3_attn8.hip), with its slots and counters: one request of 40 rows over 100000
+            // tokens 103 us against 129, over one kv head 74 against 316, but 640 rows over 8000 84 against 60.  (They cost long chunks 1 to 2 %.)
             constexpr int Z = 2, B = 8;                // elements of a thread at once, parts in flight
             const int first_wg = wg - (int) (((uint32_t) off + per - 1u) / per);
-            const int last_wg = wg + (int) (((uint32_t) (tile.steps - off - n_steps) + per - 1u) / per);
-            const __amdgpu_buffer_rsrc_t prs = __builtin_amdgcn_make_buffer_rsrc(a.part, 0, (int) ATTN_PART_BYTES, RAW_BUFFER_FLAGS);
-            // slot 2 c of workgroup c, 2 c + 1 for the tile's first
-            auto slot = [&](int c) __attribute__((always_inline)) {
-                return (2u * (uint32_t) c + (c == first_wg ? 1u : 0u)) * (uint32_t) (X::SLOT * 4) + (uint32_t) wave * (uint32_t) (X::SLOT * 4 / X::WAVES);
-            };
-            const uint32_t at = 16u * (uint32_t) lane, ml_at = (uint32_t) (QD * DT * 1024) + 8u * (uint32_t) lane;
+            const int last_wg = wg + (int) (((uint32_t) (tile.steps - off - n_steps) + per - 1u) / per), n = last_wg - first_wg + 1;
             const int live_rows = min(X::ROWS, rows - wk.t * X::ROWS), quads = (live_rows + RW - 1) / RW * (QD * DT * 64);
-            const int turns = (quads + Z * X::THREADS - 1) / (Z * X::THREADS) * ((last_wg - first_wg + B) / B);
-            const bool few = 2 * turns > last_wg - first_wg;
+            const int turns = (quads + Z * X::THREADS - 1) / (Z * X::THREADS);        // of waiting, for B parts
+            const int sizes = n <= 64 ? 8 : n <= 256 ? 16 : 24, waits = (sizes + B - 1) / B + ((n + sizes - 1) / sizes + B - 1) / B;
+            const bool two = 2 * turns * waits < n && waits < (n + B - 1) / B;
+            const int size = two ? sizes : n, groups = (n + size - 1) / size, group = (wg - first_wg) / size;
+            const int begin_wg = first_wg + group * size, in_group = min(size, last_wg + 1 - begin_wg);
+            const bool few = !two && 2 * turns * ((n + B - 1) / B) >= n;
+            const __amdgpu_buffer_rsrc_t prs = __builtin_amdgcn_make_buffer_rsrc(args->part, 0, (int) ATTN_PART_BYTES, RAW_BUFFER_FLAGS);
+            // slot 2 c of workgroup c, 2 c + 1 for the tile's first; bytes
+            auto slot = [&](int c) __attribute__((always_inline)) { return (2u * (uint32_t) c + (c == first_wg ? 1u : 0u)) * (uint32_t) (X::SLOT * 4); };
+            auto joined = [&](int g) __attribute__((always_inline)) {
+                const int c = first_wg + g * size;
+                return c == last_wg ? slot(c) : (2u * (uint32_t) (g ? c : c + 1) + 1u) * (uint32_t) (X::SLOT * 4);
+            };
+            const uint32_t my_wave = (uint32_t) wave * (uint32_t) (X::SLOT * 4 / X::WAVES);
+            const uint32_t at = 16u * (uint32_t) lane, ml_at = (uint32_t) (QD * DT * 1024) + 8u * (uint32_t) lane;
+            uint32_t* const counter = &counters[first_wg];
+            auto i_am_last = [&](uint32_t* counter, int of) __attribute__((always_inline)) {
+                __builtin_amdgcn_s_waitcnt(0x0F70);    // vmcnt(0): the part has landed
+                __syncthreads();
+                if (tid == 0) {
+                    sh.last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t) (of - 1);
+                    if (sh.last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+                __syncthreads();
+                return sh.last != 0;
+            };
             if (tid == 0) {
-                sh.last = few && __hip_atomic_load(&a.counters[first_wg], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t) (last_wg - first_wg);
+                sh.last = few && __hip_atomic_load(counter, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t) (n - 1);
+                if (sh.last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
             __syncthreads();
             bool mine = sh.last;
             if (!mine) {
-                const uint32_t to = slot(wg);
+                const uint32_t to = slot(wg) + my_wave;
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -407,37 +439,38 @@ __global__ void __launch_bounds__((Prefill8<T, D, W>::THREADS), (Prefill8<T, D, 
                         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]}), prs,
                                                                at + 1024u * (uint32_t) (QD * d + i), to, SC1);
                 __builtin_amdgcn_raw_buffer_store_b64(u32x2{(uint32_t) __float_as_int(m), (uint32_t) __float_as_int(l)}, prs, ml_at, to, SC1);
-                __builtin_amdgcn_s_waitcnt(0x0F70);    // vmcnt(0): the part has landed
-                __syncthreads();
-                if (tid == 0)
-                    sh.last = __hip_atomic_fetch_add(&a.counters[first_wg], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t) (last_wg - first_wg);
-                __syncthreads();
-                mine = sh.last;
+                // (a group of one has no counter: that of its workgroup may be the next tile's)
+                if (groups > 1) mine = in_group == 1 || i_am_last(&counters[ATTN_COUNTERS / 2 + begin_wg], in_group);
+                else mine = i_am_last(counter, n);
             }
-            if (mine) {
-                if (tid == 0) __hip_atomic_store(&a.counters[first_wg], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                if (!few) {
+            if (mine && !few) {
+#pragma unroll 1
+                for (bool last = groups == 1 || in_group == 1;; last = true) {
+                    if (last && groups > 1 && !i_am_last(counter, groups)) break;
+                    const int parts = !last ? in_group : groups > 1 ? groups : n;
+                    const uint32_t to = joined(group);
                     for (int z0 = tid; z0 < quads; z0 += Z * X::THREADS) {
-                        uint32_t from_wave[Z], at_quad[Z], at_ml[Z];
+                        uint32_t at_quad[Z], at_ml[Z];
                         f32x4 sum[Z];
                         float top[Z], total[Z];
 #pragma unroll
                         for (int i = 0; i < Z; ++i) {
                             const uint32_t z = (uint32_t) min(z0 + i * X::THREADS, quads - 1), w = z / (QD * DT * 64), r = z % (QD * DT * 64);
-                            from_wave[i] = w * (uint32_t) (X::SLOT * 4 / X::WAVES);
-                            at_quad[i] = from_wave[i] + 16u * r;
-                            at_ml[i] = from_wave[i] + (uint32_t) (QD * DT * 1024) + 8u * (r & 63u);
+                            const uint32_t from_wave = w * (uint32_t) (X::SLOT * 4 / X::WAVES);
+                            at_quad[i] = from_wave + 16u * r;
+                            at_ml[i] = from_wave + (uint32_t) (QD * DT * 1024) + 8u * (r & 63u);
                             sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
                             top[i] = LOWEST;
                             total[i] = 0.f;
                         }
 #pragma unroll 1
-                        for (int c0 = first_wg; c0 <= last_wg; c0 += B) {
+                        for (int c0 = 0; c0 < parts; c0 += B) {
                             u32x2 ml[Z][B];
                             f32x4 v[Z][B];
 #pragma unroll
                             for (int b = 0; b < B; ++b) {
-                                const uint32_t fr = slot(min(c0 + b, last_wg)) - (uint32_t) wave * (uint32_t) (X::SLOT * 4 / X::WAVES);
+                                const int c = min(c0 + b, parts - 1);
+                                const uint32_t fr = last && groups > 1 ? joined(c) : slot(begin_wg + c);
 #pragma unroll
                                 for (int i = 0; i < Z; ++i) {
                                     ml[i][b] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(prs, at_ml[i], fr, SC1));
@@ -455,7 +488,7 @@ __global__ void __launch_bounds__((Prefill8<T, D, W>::THREADS), (Prefill8<T, D, 
                                 top[i] = up;
 #pragma unroll
                                 for (int b = 0; b < B; ++b) {
-                                    const float g = c0 + b <= last_wg ? exp2_fast(__int_as_float((int) ml[i][b][0]) - up) : 0.f;
+                                    const float g = c0 + b < parts ? exp2_fast(__int_as_float((int) ml[i][b][0]) - up) : 0.f;
                                     total[i] += g * __int_as_float((int) ml[i][b][1]);
                                     sum[i] += v[i][b] * g;
                                 }
@@ -464,13 +497,21 @@ __global__ void __launch_bounds__((Prefill8<T, D, W>::THREADS), (Prefill8<T, D, 
 #pragma unroll
                         for (int i = 0; i < Z; ++i) {
                             const int z = z0 + i * X::THREADS, w = z / (QD * DT * 64), r = z % (QD * DT * 64), ln = r & 63, x = RW * w + ln % RW;
-                            if (z >= quads || x >= live_rows) continue;
-                            const int y = wk.t * X::ROWS + x, tk = (int) a.d_group.div((uint32_t) y);
-                            store_out<T>(as_global(a.out) + (int64_t) (wk.tok0 + tk) * a.o_ldt + (int64_t) (wk.h * a.group + y - tk * a.group) * a.o_ldh +
-                                             X::col_of(r / 64 / QD, r / 64 % QD) + 4 * (ln / RW), sum[i], total[i]);
+                            if (z >= quads) continue;
+                            if (!last) {
+                                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum[i]), prs, at_quad[i], to, SC1);
+                                if (r < 64)
+                                    __builtin_amdgcn_raw_buffer_store_b64(u32x2{(uint32_t) __float_as_int(top[i]), (uint32_t) __float_as_int(total[i])}, prs, at_ml[i], to, SC1);
+                            } else if (x < live_rows) {
+                                const int y = wk.t * X::ROWS + x, tk = (int) d_group.div((uint32_t) y);
+                                store_out<T>(as_global(out) + (int64_t) (wk.tok0 + tk) * o_ldt + (int64_t) (wk.h * group_heads + y - tk * group_heads) * o_ldh +
+                                                 X::col_of(r / 64 / QD, r / 64 % QD) + 4 * (ln / RW), sum[i], total[i]);
+                            }
                         }
                     }
-                } else {
+                    if (last) break;
+                }
+            } else if (mine) {
                 // 64 registers of the output at a time: more would not fit beside the workgroup's own
                 constexpr int N = DT * AE < 64 ? DT : 64 / AE;
                 static_for(std::make_integer_sequence<int, DT / N>{}, [&](auto P) __attribute__((always_inline)) {
@@ -488,7 +529,7 @@ __global__ void __launch_bounds__((Prefill8<T, D, W>::THREADS), (Prefill8<T, D, 
 #pragma unroll
                             for (int d = 0; d < N; ++d) x[d] = o[N * P + d];
                         } else {
-                            const uint32_t fr = slot(c);
+                            const uint32_t fr = slot(c) + my_wave;
                             const u32x2 ml = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(prs, ml_at, fr, SC1));
 #pragma unroll
                             for (int d = 0; d < N; ++d)
@@ -509,7 +550,6 @@ __global__ void __launch_bounds__((Prefill8<T, D, W>::THREADS), (Prefill8<T, D, 
                     }
                     put(std::integral_constant<int, N * P>{}, std::integral_constant<int, N>{}, sum, total);
                 });
-                }
             }
         }
         __syncthreads();

@@ -114,8 +114,10 @@ __device__ __forceinline__ float wave_max(float x)
 // positions, then all else), and a further head's is under way while the head before is computed.  The other workgroups rotate q.
 // A rotated k has the code of its exact value: fp32 decides, but for elements that it leaves next to the middle between two codes, which
 // are rotated again in float64 (rotating all of them in float64 took 8192 tokens 62 us instead of 53).
-// Bound by memory for prompts: 8192 tokens of 40 heads over 8 of 128 (269 MB) in 59 us, 4.6 TB/s; with fp32 alone 54.  Decodes are bound by
-// the two trips and the float64 angles: 32 in 6 us (the 16-bit cache's kernel, which has one trip, 3).
+// Prompts are bound by memory: 8192 tokens of 40 heads over 8 of 128 (218 MB) in 48 us one after the other, 4.5 TB/s, and 59 among other
+// launches; of 24 over 4 of 256 (252 MB) 81, 3.1 TB/s (two tokens a q workgroup: 78.5, but 2048 tokens 26.7 instead of 25.8).  Decodes are
+// bound by a chain of waits: 32 in 5.6 us (q alone 2.8, slots 0.3, the rest of the block's loads 1.0, codes and stores 1.5; the float64
+// ones 0.1).  The 16-bit cache's kernel, which needs no block's maximum, takes 2.8.
 template <class T, int D, int LAYOUT>
 __global__ void __launch_bounds__(2 * D, 4) rope_kv_write8_kernel(Write8Args a)
 {

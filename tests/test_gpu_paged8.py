@@ -497,6 +497,13 @@ def test_long_contexts(hq, hkv, d):
     check_attention([20000, 100], [4, 4], hq=hq, hkv=hkv, d=d, seed=3)
 
 
+@pytest.mark.parametrize("ctx,new,hq,hkv,d,dtype", [([140000], [1], 40, 1, 128, F16), ([140000], [1], 40, 1, 256, BF16), ([70000], [1], 40, 1, 64, F16),
+                                                   ([30000], [9], 12, 2, 128, BF16), ([20000, 3000], [7, 7], 24, 4, 256, F16), ([8000], [110], 40, 1, 128, F16)])
+def test_chunks_in_many_parts(ctx, new, hq, hkv, d, dtype):
+    """Tiles of prompt chunks that 13 to 512 workgroups share, in every size of the groups that are joined first."""
+    check_attention(ctx, new, hq=hq, hkv=hkv, d=d, dtype=dtype, seed=4)
+
+
 def test_many_requests():
     check_attention([(37 * i) % 300 for i in range(700)], [i % 2 for i in range(700)], hq=2, hkv=1, d=64, pad=5)
     check_attention([(37 * i) % 90 for i in range(600)], [17 + i % 3 for i in range(600)], hq=2, hkv=2, d=64)
