@@ -416,7 +416,8 @@ typedef struct {
     int32_t pages, page_size, kv_heads, head_dim;
 } exl3_cache8;
 
-/* exl3_rope_kv_write into such a cache.  k (rotated) and v are quantised from their fp32 values, with one rounding:
+/* exl3_rope_kv_write into such a cache.  A rotated k is quantised as its exact value: from fp32, and from float64 where that leaves the
+ * scale or a code open (a value past fp32's range counts as infinite); v as it is.  With one rounding:
  *   a call that writes a block's first slot starts the block anew: its scale is the least power of two of which 127 reach the
  *   largest absolute value that the call writes to the block, and rows of it that the call does not write become 0;
  *   otherwise the scale stays, or grows to what the new rows need, and then the block's other rows are rounded to the new

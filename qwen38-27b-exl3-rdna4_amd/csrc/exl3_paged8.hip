@@ -69,9 +69,10 @@ __device__ __forceinline__ u32x2 codes_of(const float (&x)[8], float inv, bool o
     return r;
 }
 
-// A rotated element in float64: element e of the head at `head`, in the token at position pos.
+// A rotated element in float64: element e of the head at `head`, in the token at position pos.  Called, not inlined: its two uses' constants
+// would spill what the block has under way (128 decodes, 40 heads over 8 of 128, 8.7 us instead of 8.0; 8192 tokens of heads of 256 70 instead of 61).
 template <class T, int LAYOUT>
-__device__ __forceinline__ double rotated_f64(const uint16_t* head, int e, int rot, int64_t pos, const double* freq, float mscale)
+__device__ __attribute__((noinline)) double rotated_f64(const uint16_t* head, int e, int rot, int64_t pos, const double* freq, float mscale)
 {
     auto at = [&](int i) __attribute__((always_inline)) { return (double) (float) __builtin_bit_cast(T, (uint16_t) *(as_global(head) + i)); };
     const int half = rot / 2;
@@ -80,6 +81,23 @@ __device__ __forceinline__ double rotated_f64(const uint16_t* head, int e, int r
     double s, c;
     sincospi(2.0 * turn_fraction((double) pos, freq[LAYOUT == ROPE_PAIRS ? e / 2 : first ? e : e - half]), &s, &c);
     return (x * c + (first ? -y : y) * s) * mscale;
+}
+// The largest finite one of 8 elements of a head from column c on, the rotated ones in float64 and rounded up: it passes 127 of a scale if and
+// only if one of them does.  x: the elements before the rotation.
+template <class T, int LAYOUT>
+__device__ __forceinline__ float exact_top(u32x4 x, const uint16_t* head, int c, int rot, int64_t pos, const double* freq, float mscale)
+{
+    const auto e = __builtin_bit_cast(typename Elem<T>::x8, x);
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, c + i < rot ? 0.f : finite_abs((float) e[i]));
+#pragma unroll 1
+    for (int i = 0; i < min(rot - c, 8); ++i) {
+        const double y = fabs(rotated_f64<T, LAYOUT>(head, c + i, rot, pos, freq, mscale));
+        const float z = (float) y;
+        top = fmaxf(top, z < INFINITY ? (double) z < y ? __int_as_float(__float_as_int(z) + 1) : z : 0.f);
+    }
+    return top;
 }
 // codes of a row whose block's scale grew by 1 / f
 __device__ __forceinline__ u32x2 rounded_anew(u32x2 old, float f)
@@ -112,8 +130,8 @@ __device__ __forceinline__ float wave_max(float x)
 // holds 8 elements of k and v of one of the block's 16 rows: new rows from the batch, the others' codes from the cache, requested at
 // once whether the scale will grow or not, with the angles formed meanwhile: a block takes two trips to memory (its slots and
 // positions, then all else), and a further head's is under way while the head before is computed.  The other workgroups rotate q.
-// A rotated k has the code of its exact value: fp32 decides, but for elements that it leaves next to the middle between two codes, which
-// are rotated again in float64 (rotating all of them in float64 took 8192 tokens 62 us instead of 53).
+// A rotated k has the scale and code of its exact value: fp32 decides, but for blocks whose largest it leaves next to 127 steps of a scale, and
+// elements next to the middle between two codes; these are rotated again in float64 (rotating all of them in float64 took 8192 tokens 62 us instead of 53).
 // Prompts are bound by memory: 8192 tokens of 40 heads over 8 of 128 (218 MB) in 48 us one after the other, 4.5 TB/s, and 59 among other
 // launches; of 24 over 4 of 256 (252 MB) 81, 3.1 TB/s (two tokens a q workgroup: 78.5, but 2048 tokens 26.7 instead of 25.8).  Decodes are
 // bound by a chain of waits: 32 in 5.6 us (q alone 2.8, slots 0.3, the rest of the block's loads 1.0, codes and stores 1.5; the float64
@@ -289,6 +307,16 @@ __global__ void __launch_bounds__(2 * D, 4) rope_kv_write8_kernel(Write8Args a)
             for (int i = 0; i < WAVES; ++i) {
                 top_k = fmaxf(top_k, tops[turn][i][0]);
                 top_v = fmaxf(top_v, tops[turn][i][1]);
+            }
+            // A pair's larger element is at least its length over 2^1/2, so fp32's error is below 2^-20 of the block's largest: it tells the
+            // scale unless that lies within 32 units of its last place (2^-19) of 127 steps.
+            if (a.rot && __builtin_expect(abs((__float_as_int(top_k) & 0x7FFFFF) - 0x7E0000) <= 32, 0)) {
+                top_k = wave_max(tok >= 0 ? exact_top<T, LAYOUT>(now.k, k, c, a.rot, pos[row], freqs, a.mscale) : 0.f);
+                __syncthreads();
+                if (lane == 0) tops[turn][wave][0] = top_k;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < WAVES; ++i) top_k = fmaxf(top_k, tops[turn][i][0]);
             }
             // A rotated pair (a, b) in fp32 is off by at most 2^-21 (|a| + |b|) mscale: cosine and sine by 2^-22, products and sum by 2^-23.
             const float off = 0x1p-20f * top_in * fabsf(a.mscale);
