@@ -335,8 +335,8 @@ __global__ void __launch_bounds__(2 * D, 4) rope_kv_write8_kernel(Write8Args a)
                 if (tok >= 0) {
                     uint32_t middle;
                     u32x2 codes = codes_of(x, inv, odd, off, middle);
-                    // what fp32 leaves next to the middle between two codes; v and what is not rotated are exact
-                    middle &= odd || !is_k ? 0u : (1u << min(max(a.rot - c, 0), 8)) - 1u;
+                    // what fp32 leaves next to the middle between two codes (never infinities and NaN); v and what is not rotated are exact
+                    middle &= !is_k ? 0u : (1u << min(max(a.rot - c, 0), 8)) - 1u;
                     for (; __builtin_expect(middle != 0, 0); middle &= middle - 1u) {
                         const int i = __builtin_ctz(middle);
                         const double q = rint(rotated_f64<T, LAYOUT>(k, c + i, a.rot, pos[row], freqs, a.mscale) * (double) inv);

@@ -84,3 +84,27 @@ def test_scale_of_a_rotated_key_is_that_of_the_exact_largest(d, rot, interleaved
             freq.append(t)
             slots.append(16 * j + rng.choice((0, 5)))
         check(k, freq, rot, interleaved, mscale, slots, dtype, turn)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("beside", [0.0, math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("d,rot,interleaved", LAYOUTS[:4] + LAYOUTS[5:])
+def test_code_of_a_rotated_key_is_that_of_its_exact_value(d, rot, interleaved, beside, dtype):
+    """An element next to the middle between two codes; a neighbour that is infinite or no number changes nothing but its own pair.  The last pair
+    (100, 0) is not turned and makes the scale 1."""
+    rng = random.Random(d + rot)
+    for turn in range(4):
+        pairs = list(range(0, 8, 2))
+        k, freq = torch.zeros(len(pairs), 2, d, dtype=torch.float64), [1.0] * (rot // 2)
+        freq[-1] = 0.0
+        lo, hi = columns(rot, interleaved, rot // 2 - 1)
+        k[..., lo] = 100.0
+        for i, j in enumerate(pairs):
+            x = rng.choice((1, -1)) * (rng.randint(1, 60) + 0.5) * (1 + NEAR[(i + turn) % 4])
+            a, b, freq[j] = pair_at(rng, x, dtype)
+            lo, hi = columns(rot, interleaved, j)
+            k[i, 0, lo], k[i, 0, hi] = a, b
+            k[i, 1, lo], k[i, 1, hi] = -a, -b
+            lo, hi = columns(rot, interleaved, j + 1)
+            k[i, 0, lo], k[i, 1, hi] = beside, beside
+        check(k, freq, rot, interleaved, 1.0, [16 * i + rng.choice((0, 5)) for i in range(len(pairs))], dtype, turn)
