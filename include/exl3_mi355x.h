@@ -423,7 +423,8 @@ typedef struct {
  *   otherwise the scale stays, or grows to what the new rows need, and then the block's other rows are rounded to the new
  *   step (a block of one request's tokens in order is filled that way; a rejected draft's rows are written over, but a
  *   scale that they raised stays);
- *   code = value / scale, rounded to even, between -127 and 127.
+ *   code = value / scale, rounded to even, between -127 and 127 (by a scale that someone else put there and that is no power of two,
+ *   a quotient within 2^-16 of the middle between two codes may go to either).
  * Infinities and NaN do not count for the scale; infinities become +-127, NaN 0.  Rows of one block are consecutive in the batch
  * (as a request's tokens are): rows of one block that others lie between race.  A slot twice in a block's rows: the last counts.
  * A slot outside [0, pages * page_size) writes nothing.  dtype: of q, k, v and q_out.  kv_heads, head_dim: the cache's. */

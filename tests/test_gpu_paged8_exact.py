@@ -1,5 +1,5 @@
-"""GPU tests of rope_kv_write8 where a rotated key lies next to a border, by less than 32 bits tell: 127 steps of a scale.  Every scale and code is
-that of the exact value.
+"""GPU tests of rope_kv_write8 where a rotated key lies next to a border, by less than 32 bits tell: 127 steps of a scale, or the middle
+between two codes.  Every scale and code is that of the exact value.
 
 A pair (a, b) = r (cos p, sin p) turned by t has the first element r cos(p + t).  At position 1 the angle is the frequency, any float64 number, so
 t = acos(x / r) - p puts the element at any x below r; what float64 loses of it (2^-50) is far below the distances 2^-30 and 2^-40 from the
@@ -13,7 +13,7 @@ import torch
 
 pytest.importorskip("exl3rocm.paged8")
 from exl3rocm import paged8  # noqa: E402
-from test_gpu_paged8 import BF16, F16, flat, gen, ints, make_cache, write_reference  # noqa: E402
+from test_gpu_paged8 import BF16, F16, flat, gen, ints, least_scale, make_cache, write_reference  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -108,3 +108,74 @@ def test_code_of_a_rotated_key_is_that_of_its_exact_value(d, rot, interleaved, b
             lo, hi = columns(rot, interleaved, j + 1)
             k[i, 0, lo], k[i, 1, hi] = beside, beside
         check(k, freq, rot, interleaved, 1.0, [16 * i + rng.choice((0, 5)) for i in range(len(pairs))], dtype, turn)
+
+
+def near_middles(rng, dtype, n):
+    """(values of dtype, scales): quotients that are the middle between two codes, or next to it by a unit of a scale's last place."""
+    x, s = [], []
+    for i in range(n):
+        v = torch.tensor(rng.uniform(0.3, 3.0)).to(dtype).float()
+        scale = v / (rng.randint(0, 125) + 0.5)
+        for _ in range(i % 3):
+            scale = torch.nextafter(scale, scale * (2.0 if i % 2 else 0.5))
+        x.append(v.item() * rng.choice((1, -1))), s.append(scale.item())
+    return torch.tensor(x, dtype=torch.float64), torch.tensor(s)
+
+
+def check_quotients(got, quotients):
+    """Codes of quotients in float64: the nearest, and either one within 2^-16 of the middle between two (127.5 steps, by a reciprocal and a product
+    that are each off by 2^-24)."""
+    q = quotients.clamp(-127, 127)
+    open_ = (q.abs().frac() - 0.5).abs() <= 2.0 ** -16
+    ok = torch.where(open_, (got - q).abs() <= 0.5 + 2.0 ** -16, got == q.round())
+    assert bool(ok.all()), ok.logical_not().nonzero()[:4].tolist()
+    assert bool(open_.any())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_quotients_by_a_scale_that_is_no_power_of_two(d, dtype):
+    """A scale that someone else put there stays where it is large enough: v, and k turned and not turned."""
+    rng, host, T, hkv, rot = random.Random(d), torch.Generator().manual_seed(d), 600, 2, 16
+    x, s = near_middles(rng, dtype, T * hkv)
+    c = make_cache("new", T, 16, hkv, d, fill=gen(d))
+    for sc in c[2:]:
+        sc.copy_(s.view(T, 1, hkv))
+    k = torch.zeros(T, hkv, d, dtype=torch.float64)
+    for i in range(rot, d):
+        k[:, :, i] = x.view(T, hkv) if i % 7 == 0 else torch.randn(T, hkv, dtype=torch.float64, generator=host) * x.view(T, hkv).abs().clamp_max(0.3) / 4
+    k = k.to(dtype).double()
+    freq = [rng.uniform(0, 6) for _ in range(rot // 2)]
+    for j in range(rot // 2):
+        a, b, freq[j] = pair_at(rng, x[2 * j].item(), dtype)
+        k[j, 0, j], k[j, 0, j + rot // 2] = a, b
+    v = k.roll(1, -1)
+    slots = [16 * t + 5 for t in range(T)]
+    y = turned(k, freq, rot, False, 1.0)
+    kt, vt = k.to(dtype).cuda(), v.to(dtype).cuda()
+    paged8.rope_kv_write8(kt, kt, vt, ints([1] * T, torch.int64), ints(slots, torch.int64), *c, torch.tensor(freq, dtype=torch.float64, device="cuda"))
+    for i, new in ((0, y), (1, v)):
+        scales = flat(c[i + 2], 16)
+        need = torch.tensor([[least_scale(m) for m in row] for row in new.abs().amax(-1).tolist()], dtype=torch.float64)
+        assert torch.equal(scales, torch.maximum(s.double().view(T, hkv), need)) and bool((scales > need).any())
+        check_quotients(flat(c[i], 16)[slots], new / scales[:, :, None])
+
+
+def test_rows_rounded_anew_from_a_scale_that_is_no_power_of_two():
+    """Codes c of a scale that makes c * scale the middle between two steps of the new scale, or next to it."""
+    rng, T = random.Random(1), 500
+    c = make_cache("new", T, 16, 1, 64)
+    for t in range(T):
+        code = rng.choice([i for i in range(-127, 128) if i])
+        s = torch.tensor(4.0 * (rng.randint(0, max(abs(code) // 4 - 1, 0)) + 0.5) / abs(code))       # the new scale is 4
+        for _ in range(t % 3):
+            s = torch.nextafter(s, s * (2.0 if t % 2 else 0.5))
+        c[0][t, :, 0, :] = code
+        c[2][t] = s.cuda()
+    k = torch.full((T, 1, 64), 500.0, device="cuda", dtype=F16)
+    new = [16 * t + t % 15 + 1 for t in range(T)]
+    old = flat(c[0], 16) * flat(c[2], 16).repeat_interleave(16, 0)[:, :, None]
+    paged8.rope_kv_write8(k, k, k, ints([0] * T, torch.int64), ints(new, torch.int64), *c, torch.zeros(0, device="cuda", dtype=torch.float64))
+    assert bool((c[2] == 4.0).all())
+    old[new] = 500.0
+    check_quotients(flat(c[0], 16), old / 4.0)
