@@ -109,7 +109,7 @@ def rope_kv_write8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions:
 
 def kv_read8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, slots: torch.Tensor,
              dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(k, v), each [T, kv_heads, D] of dtype (fp16 or bf16): the values that the slots (int64 [T]) hold.  A slot outside the
+    """(k, v), each [T, kv_heads, D] of dtype (fp16 or bf16): the values that the T slots (int64, contiguous) hold.  A slot outside the
     cache (-1) gives zeros."""
     gpu = _gpu(k_cache, "kv_read8")
     cache, heads, d = _cache8("kv_read8", k_cache, v_cache, k_scale, v_scale, gpu)
@@ -168,7 +168,7 @@ def _(q, k, v, positions, slots, k_cache, v_cache, k_scale, v_scale, inv_freq, m
 
 @torch.library.register_fake("exl3rocm::kv_read8")
 def _(k_cache, v_cache, k_scale, v_scale, slots, dtype=torch.float16):
-    shape = (slots.shape[0], *k_cache.shape[2:])
+    shape = (slots.numel(), *k_cache.shape[2:])
     return k_cache.new_empty(shape, dtype=dtype), k_cache.new_empty(shape, dtype=dtype)
 
 
