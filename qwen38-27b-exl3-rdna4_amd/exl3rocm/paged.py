@@ -270,7 +270,7 @@ for _f in (batch_plan, rope_kv_write, paged_attention):
 
 @torch.library.register_fake("exl3rocm::batch_plan")
 def _(ctx_lens, new_lens, block_table, free_pages, free_count, page_size, num_tokens):
-    R = ctx_lens.shape[0]
+    R = ctx_lens.numel()
     return (ctx_lens.new_empty(R + 1), ctx_lens.new_empty(R), ctx_lens.new_empty(num_tokens, dtype=torch.int64),
             ctx_lens.new_empty(num_tokens, dtype=torch.int64), ctx_lens.new_empty(1))
 
