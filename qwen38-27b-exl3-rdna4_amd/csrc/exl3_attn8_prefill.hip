@@ -42,7 +42,8 @@ struct Prefill8 {
     static constexpr int WAVES = W, ROWS = RW * WAVES, KEYS = 64, THREADS = 64 * WAVES;
     static constexpr int GRID = THREADS == 512 ? 256 : 512;             // workgroups: one or two a CU
     static constexpr int SLOT = attn_slot(ROWS, D + 128 / RW - 2); // every lane's maximum and sum, also where lanes share a row
-    static_assert(GRID <= ATTN_COUNTERS && (size_t) 2 * GRID * SLOT * 4 <= ATTN_PART_BYTES);
+    // two counters a workgroup: of the tile that it begins, and of the group of its parts that it begins
+    static_assert(GRID <= ATTN_COUNTERS / 2 && (size_t) 2 * GRID * SLOT * 4 <= ATTN_PART_BYTES);
     static constexpr int LEAST = 4;                     // steps of a share at least
     static constexpr int CH = D / 8;                    // 8-code pieces of a row
     static constexpr int KW = KEYS / WAVES;             // keys that a wave moves
