@@ -29,7 +29,7 @@ template <> struct Codes<4> { typedef u32x4 T; typedef gc_u32x4 G; };
 //   V: a lane holds E = D / 16 columns E (l & 15) .. of its keys, and product e is made of column e of pairs of keys
 // 16 rows: bound by memory.  96 decodes of 100 to 16000 tokens, 40 heads over 8 of 128 (535 MB), 117 us, 4.6 TB/s (ends of tiles);
 // two of 131000, 24 over 4 of 256 (728 MB), 127 us, 5.8 TB/s.  17 to 32 rows: by waits and issue, 12 requests' drafts (189 MB, 24 rows of
-// 256) 65 us, 2.9 TB/s; vector instructions take 33 % of the cycles, waits 41 % of the waves' time.
+// 256) 65 us, 2.9 TB/s; vector instructions take 34 % of the cycles, waits 40 % of the waves' time.
 template <class T, int D, int WAVES, int KEYS, int S>
 struct Decode8 {
     static constexpr int ROWS = 16, TILE = ROWS * S, THREADS = 64 * WAVES;
@@ -562,7 +562,8 @@ extern "C" int exl3_paged_attention8(const void* q, int64_t q_ldt, int64_t q_ldh
     // 24 rows, 24 heads over 4 of 256: 77 / 93 / 89; 16 of 4000 46 / 60 / 61, one of 1000 17 / 17 / 24; 20 rows, 40 over 8 of 128: 73 / 91 / 80,
     // 49 / 65 / 59, 12 / 12 / 20; 24 rows, 32 over 8 of 64: 50 / 55 / 57, 36 / 40 / 40, 10 / 10 / 15.  From 33 rows the chunk kernel: eight
     // of 16000 tokens, 40 rows of 128, 119 us against 143 with four sets; 36 rows of 256, 102 against 120, and 64 of 1000 53 against 78.
-    // The host knows the average alone, not the lengths, so a batch of unlike requests takes the kernel of the many.
+    // The host knows the average alone, not the lengths, so a batch of unlike requests takes the kernel of the many.  That costs most where a few
+    // chunks are among many decodes: 256 decodes over 4000 tokens and 512 tokens over 8000, 40 heads over 8 of 128, 904 us; in two calls 428 + 153.
     const int64_t rows = requests ? (int64_t) tokens * a.group / requests : 0;
     if (rows > 32) launch_attn8_prefill(a, rows, dtype, (hipStream_t) stream);
     else if (dtype == EXL3_FP16) launch<f16>(a, (int) rows, (hipStream_t) stream);

@@ -572,7 +572,8 @@ template <class T>
 void launch(const Attn8Args& a, int64_t rows, hipStream_t s)
 {
     // Many rows: 256 a tile, whose keys are made fp16 once for eight waves instead of four (2048 tokens over 12000, 40 heads over 8 of
-    // 128: 664 us against 733; 512 over none 38 against 32).  Heads of 64 gain less (380 against 405) and lose as much without a context.
+    // 128: 643 us against 732; 512 over none 42 against 37).  Heads of 64 gain as much over a long context (362 against 419, one after the other) but
+    // lose without one (512 tokens 26 against 24) and in small chunks beside decodes (32 against 30).
     if (a.c.d == 64) launch_one<T, 64, 4>(a, s);
     else if (a.c.d == 256) launch_one<T, 256, 8>(a, s);
     else if (rows > 4096) launch_one<T, 128, 8>(a, s);

@@ -131,11 +131,13 @@ __device__ __forceinline__ float wave_max(float x)
 // once whether the scale will grow or not, with the angles formed meanwhile: a block takes two trips to memory (its slots and
 // positions, then all else), and a further head's is under way while the head before is computed.  The other workgroups rotate q.
 // A rotated k has the scale and code of its exact value: fp32 decides, but for blocks whose largest it leaves next to 127 steps of a scale, and
-// elements next to the middle between two codes; these are rotated again in float64 (rotating all of them in float64 took 8192 tokens 62 us instead of 53).
-// Prompts are bound by memory: 8192 tokens of 40 heads over 8 of 128 (218 MB) in 48 us one after the other, 4.5 TB/s, and 59 among other
-// launches; of 24 over 4 of 256 (252 MB) 81, 3.1 TB/s (two tokens a q workgroup: 78.5, but 2048 tokens 26.7 instead of 25.8).  Decodes are
-// bound by a chain of waits: 32 in 5.6 us (q alone 2.8, slots 0.3, the rest of the block's loads 1.0, codes and stores 1.5; the float64
-// ones 0.1).  The 16-bit cache's kernel, which needs no block's maximum, takes 2.8.
+// elements next to the middle between two codes; these are rotated again in float64 (rotating all of them in float64 takes 8192 tokens 79 us
+// instead of 49).
+// Prompts are bound by memory: 8192 tokens of 40 heads over 8 of 128 (218 MB) in 47 us one after the other, 4.6 TB/s, and 60 among other
+// launches; of 24 over 4 of 256 (252 MB) 79 to 87 (pairs side by side: 61), 3.0 TB/s (two tokens a q workgroup: 78.5 instead of 81, but 2048 tokens
+// 26.7 instead of 25.8).  Decodes are
+// bound by a chain of waits: 32 in 5.8 us (q alone 2.8, slots 0.3, the rest of the block's loads 1.0, codes and stores 1.5; the exact
+// ones 0.2).  The 16-bit cache's kernel, which needs no block's maximum, takes 2.8.
 template <class T, int D, int LAYOUT>
 __global__ void __launch_bounds__(2 * D, 4) rope_kv_write8_kernel(Write8Args a)
 {
@@ -440,9 +442,9 @@ extern "C" int exl3_rope_kv_write8(const void* q, int64_t q_ldt, int64_t q_ldh, 
     a.tokens = tokens, a.hq = q_heads, a.rot = rot_dim;
     // Few tokens: a workgroup for each row and head, so that all blocks of a batch of decodes are under way at once.  More: windows
     // of 16 rows, in which a prompt begins one or two blocks, and four workgroups that take them in turn; so many heads a
-    // workgroup that about 1024 have work, since its angles serve all of them.  One row / 16 rows a window, us, 40 + 8 heads of 128: a prompt's
-    // 128 tokens 10.9 / 7.6, 128 decodes 9.5 / 15.9; 512 tokens 16.5 / 9.9, 512 decodes 29 / 24; 32 decodes 6.5 / 15.  One, two,
-    // four and eight heads of 8192 tokens: 66, 58, 53, 50; of 1000 tokens, one and two: 15.3 and 13.5.
+    // workgroup that about 1024 have work, since its angles serve all of them.  One row / 16 rows a window, us, 40 + 8 heads of 128, in a row: a prompt's
+    // 128 tokens 9.5 / 6.9, 128 decodes 8.2 / 14.6; 512 tokens 14.7 / 8.3, 512 decodes 24.6 / 21.7; 32 decodes 5.8 / 14.  One, two,
+    // four and eight heads of 8192 tokens: 79, 61, 53, 47; of 1000 tokens: 12.2, 11.6, 14.9, 22.8.
     const bool few = (int64_t) tokens * hkv <= 1024;
     a.rows = few ? 1 : C8_BLOCK;
     a.turns = few ? 1 : 4;

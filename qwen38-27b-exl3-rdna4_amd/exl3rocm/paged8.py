@@ -11,7 +11,7 @@ A value is code * scale: int8 codes, and an fp32 scale for each block of 16 toke
 block's first token starts the block anew: its scale becomes the least power of two (2 ** -40 to 2 ** 40) of which 127 reach
 the largest absolute value that the call writes there, and rows that the call does not write become 0.  A call that writes later tokens keeps
 the scale or doubles it as often as they need, and then rounds the block's other rows to the new step.  So a value is off by at
-most half a step (1 / 254 to 1 / 128 of its block's largest), and by as much again for each later doubling, the steps before it
+most half a step (1 / 254 to 1 / 127 of its block's largest), and by as much again for each later doubling, the steps before it
 being half as large.
 
 Each function is also the torch op of its name (torch.ops.exl3rocm.*).  Lengths stay on the GPU and a step's calls can be

@@ -179,3 +179,14 @@ def test_rows_rounded_anew_from_a_scale_that_is_no_power_of_two():
     assert bool((c[2] == 4.0).all())
     old[new] = 500.0
     check_quotients(flat(c[0], 16), old / 4.0)
+
+
+def test_a_value_is_off_by_up_to_a_127th_of_its_blocks_largest():
+    """63.6 needs a scale of 1, so 0.5 is stored as 0: more than a 128th of the largest off."""
+    c = make_cache("new", 1, 16, 1, 64)
+    k = torch.full((1, 1, 64), 0.5, device="cuda", dtype=F16)
+    k[..., 0] = 63.59375
+    paged8.rope_kv_write8(k, k, k, ints([0], torch.int64), ints([0], torch.int64), *c, torch.zeros(0, device="cuda", dtype=torch.float64))
+    got = paged8.kv_read8(*c, ints([0], torch.int64))[0]
+    off = (got - k).abs().max().item()
+    assert c[2].flatten().tolist() == [1.0] and 63.59375 / 128 < off <= 63.59375 / 127
