@@ -7,7 +7,7 @@ import torch
 
 pytest.importorskip("exl3rocm.paged8")
 from exl3rocm import paged8  # noqa: E402
-from test_gpu_paged8 import BF16, F16, check_attention, check_write, flat, gen, inputs, ints, make_cache, run_of, write_reference  # noqa: E402
+from test_gpu_paged8 import BF16, F16, check_attention, check_write, flat, gen, inputs, ints, make_cache, reference, run_of  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -49,6 +49,18 @@ def test_wide_tiles_scale_of_scores(scale, dtype):
 @pytest.mark.parametrize("ctx,new", [([9000], [104]), ([30000], [105]), ([2500, 12000], [104, 106])])
 def test_wide_tiles_in_many_parts(ctx, new):
     check_attention(ctx, new, hq=40, hkv=1, dtype=BF16, seed=5)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(40, 8, 128), (12, 2, 256), (8, 2, 64)])
+def test_many_decodes_beside_a_chunk_in_one_call_and_in_two(hq, hkv, d):
+    """One call takes the decode kernel for all; of two, the second takes the prompt kernel."""
+    R = 60
+    ctx, new = [(53 * i) % 700 for i in range(R)] + [900], [1] * R + [120]
+    got, (q, c, table, cu, seq, scale, window) = check_attention(ctx, new, hq=hq, hkv=hkv, d=d)
+    want, tol = reference(q, c, table, cu, seq, scale, window, F16)
+    for rows, reqs in ((slice(0, R), slice(0, R)), (slice(R, R + 120), slice(R, R + 1))):
+        part = paged8.paged_attention8(q[rows], *c, table[reqs], cu[reqs.start:reqs.stop + 1] - cu[reqs.start], seq[reqs], scale, window)
+        assert bool(((part.double() - want[rows]).abs() <= tol[rows]).all())
 
 
 # ---- decodes and drafts over tiles that more than 64 and more than 256 workgroups share ----
